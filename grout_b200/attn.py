@@ -93,9 +93,21 @@ class PrefillPagedArgs(ctypes.Structure):
     ]
 
 
+class Fp8Pages(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
 # Every symbol include/grout_attn.h declares, with its ctypes signature.
 _vp, _i32, _i64, _f32, _sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 _DIMS = ctypes.POINTER(AttnDims)
+_FP8 = ctypes.POINTER(Fp8Pages)
 SIGNATURES = {
     "grout_attn_last_error": (ctypes.c_char_p, []),
     "grout_attn_version": (ctypes.c_char_p, []),
@@ -143,6 +155,25 @@ SIGNATURES = {
     "grout_qk_norm_rope_kv_prefill_paged": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp,
                                                            _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32,
                                                            _DIMS, _vp]),
+    "grout_qk_norm_rope_kv_decode_paged_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _FP8, _vp, _i32,
+                                                              _vp, _i32, _DIMS, _vp]),
+    "grout_qk_norm_rope_kv_prefill_paged_fp8": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp,
+                                                               _vp, _FP8, _vp, _i32, _i32, _DIMS, _vp]),
+    "grout_kv_read_paged_fp8": (ctypes.c_int, [_FP8, _vp, _i32, _vp, _vp, _i32, _i64, _vp, _vp, _i64,
+                                               _DIMS, _vp]),
+    "grout_attn_decode_window_splits": (_i32, [_i32, _i32, _i32, _i32, _DIMS]),
+    "grout_attn_decode_window_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _DIMS]),
+    "grout_attn_decode_window": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _i32,
+                                                _i32, _i32, _DIMS, _vp, _sz, _vp]),
+    "grout_attn_decode_paged_window": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp,
+                                                      _i32, _i32, _i32, _i32, _i32, _DIMS, _vp, _sz,
+                                                      _vp]),
+    "grout_attn_decode_paged_fp8": (ctypes.c_int, [_vp, _FP8, _vp, _i32, _vp, _vp, _i32, _i32, _i32,
+                                                   _i32, _i32, _DIMS, _vp, _sz, _vp]),
+    "grout_attn_prefill_varlen_window": (ctypes.c_int, [ctypes.POINTER(PrefillVarlenArgs), _i32, _i32,
+                                                        _DIMS, _vp]),
+    "grout_attn_prefill_paged_window": (ctypes.c_int, [ctypes.POINTER(PrefillPagedArgs), _i32, _i32,
+                                                       _DIMS, _vp]),
 }
 
 _lib = None
@@ -662,6 +693,323 @@ def attention_decode_noalloc(q, k_cache, v_cache, position, out, max_kv_len, qk_
     _check(lib().grout_attn_decode_noalloc(
         _ptr(q), _ptr(k_cache), _ptr(v_cache), hkv * max_seq * HEAD_DIM, max_seq * HEAD_DIM,
         _ptr(position), _ptr(out), B, int(max_kv_len), ctypes.byref(dims), _stream(q)))
+    return out
+
+
+# ------------------------------------- 8-bit paged cache, sliding windows
+
+
+def _enqueue(dev, fn, *args):
+    """Calls fn(*args, stream) on the current stream of the tensors' device."""
+    if dev.index == torch.cuda.current_device():
+        _check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(*args, torch.cuda.current_stream().cuda_stream))
+
+
+def _cuda(t, name, dtype, dev=None):
+    """t is a contiguous CUDA tensor of the type (and on the device); returns its device."""
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+    _need(t.is_contiguous(), f"{name} must be contiguous")
+    _need(dev is None or t.device == dev, f"{name} is on {t.device}, not on {dev}")
+    return t.device
+
+
+def _positions(t, n, dev):
+    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in (torch.int32, torch.uint32)
+          and t.is_contiguous() and t.numel() >= n and t.device == dev,
+          "position must be a contiguous device int32/uint32 tensor with one entry per sequence")
+
+
+def _table(t, batch, dev):
+    """[batch, table_stride] page table; returns the stride."""
+    _cuda(t, "page_table", torch.int32, dev)
+    _need(t.dim() == 2 and t.shape[0] >= batch, f"page_table must be [batch, table_stride]: {tuple(t.shape)}")
+    return t.shape[1]
+
+
+def _kv_pages(k_pages, v_pages, dtype, dev):
+    _cuda(k_pages, "k_pages", dtype, dev)
+    _cuda(v_pages, "v_pages", dtype, dev)
+    _need(k_pages.dim() == 4 and k_pages.shape[3] == HEAD_DIM,
+          f"k_pages must be [num_pages, Hkv, page_size, 128]: {tuple(k_pages.shape)}")
+    _need(v_pages.shape == k_pages.shape, "v_pages shape mismatch")
+    return k_pages.shape[:3]
+
+
+def _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev):
+    """The C struct of an 8-bit page pool, its KV heads and page size."""
+    num_pages, hkv, page_size = _kv_pages(k_pages, v_pages, torch.float8_e4m3fn, dev)
+    for t, n in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+        _cuda(t, n, torch.float32, dev)
+        _need(t.shape == k_pages.shape[:3], f"{n} must be [num_pages, Hkv, page_size]: {tuple(t.shape)}")
+    return Fp8Pages(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                    num_pages, page_size), hkv, page_size
+
+
+def _rope(t, max_seq, dev):
+    _cuda(t, "rope_table", torch.float32, dev)
+    _need(t.dim() == 2 and t.shape[1] == HEAD_DIM and t.shape[0] >= max_seq,
+          f"rope_table must be [>= max_seq={max_seq}, 128] f32: {tuple(t.shape)}")
+
+
+def _norm_weights(q_norm_w, k_norm_w, dev):
+    for t, n in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+        _cuda(t, n, torch.float16, dev)
+        _need(t.numel() == HEAD_DIM, f"{n} must have 128 entries")
+
+
+def qk_norm_rope_kv_decode_paged_fp8(qkv, q_norm_w, k_norm_w, rope_table, q_out, k_pages, v_pages,
+                                     k_scales, v_scales, page_table, position, num_q_heads,
+                                     num_kv_heads, eps, max_seq=None):
+    """qk_norm_rope_kv_decode_paged into the 8-bit paged cache: k_pages,
+    v_pages [num_pages, Hkv, page_size, 128] float8_e4m3fn with one f32 scale
+    per row in k_scales, v_scales [num_pages, Hkv, page_size].  A row y is
+    stored as scale = max|y| / 448, code = e4m3(y * (448 / max|y|))."""
+    dev = _cuda(qkv, "qkv", torch.float16)
+    _cuda(q_out, "q_out", torch.float16, dev)
+    _norm_weights(q_norm_w, k_norm_w, dev)
+    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
+    hq = num_q_heads
+    _need(hkv == num_kv_heads, "k_pages head count mismatch")
+    B = qkv.shape[0] if qkv.dim() == 2 else 1
+    _need(qkv.numel() == B * (hq + 2 * hkv) * HEAD_DIM, f"qkv shape mismatch: {tuple(qkv.shape)}")
+    _need(q_out.numel() == B * hq * HEAD_DIM, f"q_out shape mismatch: {tuple(q_out.shape)}")
+    _positions(position, B, dev)
+    stride = _table(page_table, B, dev)
+    if max_seq is None:
+        max_seq = stride * page_size
+    _rope(rope_table, max_seq, dev)
+    _enqueue(dev, lib().grout_qk_norm_rope_kv_decode_paged_fp8, qkv.data_ptr(), q_norm_w.data_ptr(),
+             k_norm_w.data_ptr(), rope_table.data_ptr(), q_out.data_ptr(), pages,
+             page_table.data_ptr(), stride, position.data_ptr(), B,
+             AttnDims(hq, hkv, HEAD_DIM, max_seq, eps, 0.0, 0))
+    return q_out
+
+
+def qk_norm_rope_kv_prefill_paged_fp8(q, k, v, q_norm_w, k_norm_w, rope_table, q_out, k_pages,
+                                      v_pages, k_scales, v_scales, page_table_row, position_start,
+                                      eps, max_seq=None):
+    """qk_norm_rope_kv_prefill_paged into the 8-bit paged cache (see
+    qk_norm_rope_kv_decode_paged_fp8): one sequence, page_table_row is its row
+    of the page table."""
+    dev = _cuda(q, "q", torch.float16)
+    for t, n in ((k, "k"), (v, "v"), (q_out, "q_out")):
+        _cuda(t, n, torch.float16, dev)
+    _norm_weights(q_norm_w, k_norm_w, dev)
+    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
+    _need(q.dim() == 3 and q.shape[2] == HEAD_DIM, f"q shape mismatch: {tuple(q.shape)}")
+    S, hq, _ = q.shape
+    _need(k.shape == (S, hkv, HEAD_DIM) and v.shape == k.shape, "k/v shape mismatch")
+    _need(q_out.shape == q.shape, "q_out shape mismatch")
+    _cuda(page_table_row, "page_table_row", torch.int32, dev)
+    if max_seq is None:
+        max_seq = page_table_row.numel() * page_size
+    _need(page_table_row.numel() * page_size >= max_seq, "page_table_row shorter than max_seq")
+    _rope(rope_table, max_seq, dev)
+    _enqueue(dev, lib().grout_qk_norm_rope_kv_prefill_paged_fp8, q.data_ptr(), k.data_ptr(),
+             v.data_ptr(), hq * HEAD_DIM, hkv * HEAD_DIM, q_norm_w.data_ptr(), k_norm_w.data_ptr(),
+             rope_table.data_ptr(), q_out.data_ptr(), pages, page_table_row.data_ptr(),
+             int(position_start), S, AttnDims(hq, hkv, HEAD_DIM, max_seq, eps, 0.0, 0))
+    return q_out
+
+
+def _cu_seqlens(t, dev):
+    """Device int32 [batch + 1]; returns the batch."""
+    _cuda(t, "cu_seqlens", torch.int32, dev)
+    _need(t.dim() == 1 and t.numel() >= 1, f"cu_seqlens must be [batch + 1]: {tuple(t.shape)}")
+    return t.numel() - 1
+
+
+def _starts(t, batch, dev, name="position_start"):
+    if t is None:
+        return None
+    _cuda(t, name, torch.int32, dev)
+    _need(t.numel() >= batch, f"{name} needs one entry per sequence")
+    return t.data_ptr()
+
+
+def kv_read_paged_fp8(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v_out, cu_seqlens,
+                      position_start=None, max_seq=None):
+    """Reads rows of the 8-bit paged cache back to f16: packed k_out, v_out
+    [rows, Hkv, 128], rows cu_seqlens[b] .. cu_seqlens[b+1] of sequence b from
+    position position_start[b] (default 0) on; cu_seqlens, position_start
+    device int32.  Rows behind the last sequence are left as they are.
+    attention_prefill_varlen(_window) takes the result with kv_row_stride =
+    Hkv * 128, kv_head_stride = 128, kv_start = cu_seqlens[:-1]: attention of
+    a chunk of new tokens over the 8-bit cache."""
+    dev = _cuda(k_out, "k_out", torch.float16)
+    _cuda(v_out, "v_out", torch.float16, dev)
+    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
+    _need(k_out.dim() == 3 and k_out.shape[1:] == (hkv, HEAD_DIM),
+          f"k_out must be [rows, {hkv}, 128]: {tuple(k_out.shape)}")
+    _need(v_out.shape == k_out.shape, "v_out shape mismatch")
+    B = _cu_seqlens(cu_seqlens, dev)
+    start = _starts(position_start, B, dev)
+    stride = _table(page_table, B, dev)
+    if max_seq is None:
+        max_seq = stride * page_size
+    _enqueue(dev, lib().grout_kv_read_paged_fp8, pages, page_table.data_ptr(), stride,
+             cu_seqlens.data_ptr(), start, B, k_out.shape[0], k_out.data_ptr(), v_out.data_ptr(),
+             hkv * HEAD_DIM, AttnDims(hkv, hkv, HEAD_DIM, max_seq, 0.0, 0.0, 0))
+    return k_out, v_out
+
+
+def decode_window_splits(batch, max_kv_len, window, sinks, num_q_heads, num_kv_heads, max_seq):
+    """Split count of the window decode calls (window 0: the whole context)."""
+    dims = make_dims(num_q_heads, num_kv_heads, max_seq)
+    return lib().grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, dims)
+
+
+def decode_window_workspace_bytes(batch, max_kv_len, window, sinks, num_q_heads, num_kv_heads,
+                                  max_seq, num_splits=0):
+    """Workspace bytes of the window decode calls (num_splits 0: the automatic count)."""
+    dims = make_dims(num_q_heads, num_kv_heads, max_seq)
+    return lib().grout_attn_decode_window_workspace_bytes(batch, max_kv_len, window, sinks,
+                                                          num_splits, dims)
+
+
+def _decode_window(fn, cache_args, q, out, dev, position, max_kv_len, window, sinks, num_splits,
+                   workspace, hkv, max_seq, qk_scale, scale_f16):
+    """The tail of the window decode calls: fn(q, *cache_args, position, out, ...)."""
+    B, hq = q.shape[0], q.shape[1]
+    _cuda(out, "out", torch.float16, dev)
+    _need(out.shape == q.shape, "out shape mismatch")
+    _positions(position, B, dev)
+    dims = AttnDims(hq, hkv, HEAD_DIM, max_seq, 0.0, float(qk_scale) if qk_scale else 0.0,
+                    FLAG_DECODE_SCALE_F16 if scale_f16 else 0)
+    num_splits = int(num_splits or 0)
+    need = lib().grout_attn_decode_window_workspace_bytes(B, max_kv_len, window, sinks, num_splits, dims)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        _need(workspace.is_cuda and workspace.device == dev and workspace.is_contiguous(),
+              "workspace must be a contiguous tensor on the call's device")
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _enqueue(dev, fn, q.data_ptr(), *cache_args, position.data_ptr(), out.data_ptr(), B, max_kv_len,
+             window, sinks, num_splits, dims, ws, ws_bytes)
+    return out
+
+
+def _decode_query(q):
+    dev = _cuda(q, "q", torch.float16)
+    _need(q.dim() == 3 and q.shape[2] == HEAD_DIM, f"q must be [B, Hq, 128]: {tuple(q.shape)}")
+    return dev
+
+
+def attention_decode_window(q, k_cache, v_cache, position, out, max_kv_len, window, sinks=0,
+                            workspace=None, num_splits=None, qk_scale=None, scale_f16=True):
+    """attention_decode over a sliding window: the query at position p sees the
+    keys n <= p with n > p - window or n < sinks.  q, out [B, Hq, 128]; caches
+    [B, Hkv, max_seq, 128]; only 64-key blocks that hold a visible key are
+    read, the other rows may hold anything."""
+    dev = _decode_query(q)
+    _cuda(k_cache, "k_cache", torch.float16, dev)
+    _cuda(v_cache, "v_cache", torch.float16, dev)
+    _need(k_cache.dim() == 4 and k_cache.shape[0] >= q.shape[0] and k_cache.shape[3] == HEAD_DIM,
+          f"k_cache must be [B, Hkv, max_seq, 128]: {tuple(k_cache.shape)}")
+    _need(v_cache.shape == k_cache.shape, "v_cache shape mismatch")
+    hkv, max_seq = k_cache.shape[1], k_cache.shape[2]
+    return _decode_window(lib().grout_attn_decode_window,
+                          (k_cache.data_ptr(), v_cache.data_ptr(), hkv * max_seq * HEAD_DIM, max_seq * HEAD_DIM),
+                          q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
+                          max_seq, qk_scale, scale_f16)
+
+
+def attention_decode_paged_window(q, k_pages, v_pages, page_table, position, out, max_kv_len, window,
+                                  sinks=0, max_seq=None, workspace=None, num_splits=None,
+                                  qk_scale=None, scale_f16=True):
+    """attention_decode_paged over a sliding window (see
+    attention_decode_window).  Pages that hold no visible key may be freed:
+    their table entries are not looked at."""
+    dev = _decode_query(q)
+    num_pages, hkv, page_size = _kv_pages(k_pages, v_pages, torch.float16, dev)
+    stride = _table(page_table, q.shape[0], dev)
+    return _decode_window(lib().grout_attn_decode_paged_window,
+                          (k_pages.data_ptr(), v_pages.data_ptr(), num_pages, page_size,
+                           page_table.data_ptr(), stride),
+                          q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
+                          stride * page_size if max_seq is None else max_seq, qk_scale, scale_f16)
+
+
+def attention_decode_paged_fp8(q, k_pages, v_pages, k_scales, v_scales, page_table, position, out,
+                               max_kv_len, window=0, sinks=0, max_seq=None, workspace=None,
+                               num_splits=None, qk_scale=None, scale_f16=True):
+    """Split-K GQA decode over the 8-bit paged cache (see
+    qk_norm_rope_kv_decode_paged_fp8); window 0 attends to the whole context,
+    else as attention_decode_paged_window."""
+    dev = _decode_query(q)
+    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
+    stride = _table(page_table, q.shape[0], dev)
+    return _decode_window(lib().grout_attn_decode_paged_fp8, (pages, page_table.data_ptr(), stride),
+                          q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
+                          stride * page_size if max_seq is None else max_seq, qk_scale, scale_f16)
+
+
+def _chunk_query(q, out):
+    dev = _cuda(q, "q", torch.float16)
+    _need(q.dim() == 3 and q.shape[2] == HEAD_DIM, f"q must be [q_rows, Hq, 128]: {tuple(q.shape)}")
+    _cuda(out, "out", torch.float16, dev)
+    _need(out.shape == q.shape, "out shape mismatch")
+    return dev
+
+
+def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads,
+                                    kv_row_stride, kv_head_stride, window, sinks=0,
+                                    kv_batch_stride=0, kv_rows=None, position_start=None,
+                                    kv_start=None, qk_scale=None):
+    """attention_prefill_varlen over a sliding window: the row at position p
+    sees the keys n <= p with n > p - window or n < sinks.  Arguments as there;
+    cu_seqlens_q None: one sequence of all q rows."""
+    dev = _chunk_query(q, out)
+    _cuda(k, "k", torch.float16, dev)
+    _cuda(v, "v", torch.float16, dev)
+    rows, hq = q.shape[0], q.shape[1]
+    B = 1 if cu_seqlens_q is None else _cu_seqlens(cu_seqlens_q, dev)
+    if cu_seqlens_q is None:
+        max_q_len = rows if max_q_len is None else max_q_len
+    _need(max_q_len is not None, "max_q_len is required with cu_seqlens_q")
+    _need(kv_row_stride > 0 and kv_head_stride > 0 and kv_batch_stride >= 0, "bad kv strides")
+    # the furthest element that the strides address lies in k and v
+    fixed = max(0, B - 1) * kv_batch_stride + (num_kv_heads - 1) * kv_head_stride + HEAD_DIM
+    most = (min(k.numel(), v.numel()) - fixed) // kv_row_stride + 1
+    if kv_rows is None:
+        kv_rows = most
+    _need(0 < kv_rows <= most, f"kv_rows={kv_rows}: k and v hold {most} rows at these strides")
+    args = PrefillVarlenArgs(
+        q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k.data_ptr(), v.data_ptr(),
+        kv_batch_stride, kv_row_stride, kv_head_stride, kv_rows,
+        None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+        _starts(position_start, B, dev), _starts(kv_start, B, dev, "kv_start"), B, max_q_len)
+    _enqueue(dev, lib().grout_attn_prefill_varlen_window, args, window, sinks,
+             make_dims(hq, num_kv_heads, 1 << 30, qk_scale=qk_scale))
+    return out
+
+
+def attention_prefill_paged_window(q, k_pages, v_pages, page_table, out, window, sinks=0,
+                                   cu_seqlens_q=None, position_start=None, max_q_len=None,
+                                   max_seq=None, qk_scale=None):
+    """attention_prefill_paged over a sliding window (see
+    attention_prefill_varlen_window).  Pages that hold no key a row of the
+    chunk sees may be freed: their table entries are not looked at."""
+    dev = _chunk_query(q, out)
+    num_pages, hkv, page_size = _kv_pages(k_pages, v_pages, torch.float16, dev)
+    rows, hq = q.shape[0], q.shape[1]
+    B = 1 if cu_seqlens_q is None else _cu_seqlens(cu_seqlens_q, dev)
+    if cu_seqlens_q is None:
+        max_q_len = rows if max_q_len is None else max_q_len
+    _need(max_q_len is not None, "max_q_len is required with cu_seqlens_q")
+    stride = _table(page_table, B, dev)
+    args = PrefillPagedArgs(
+        q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k_pages.data_ptr(), v_pages.data_ptr(),
+        num_pages, page_size, page_table.data_ptr(), stride,
+        None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+        _starts(position_start, B, dev), B, max_q_len)
+    _enqueue(dev, lib().grout_attn_prefill_paged_window, args, window, sinks,
+             make_dims(hq, hkv, stride * page_size if max_seq is None else max_seq, qk_scale=qk_scale))
     return out
 
 

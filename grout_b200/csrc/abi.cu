@@ -87,8 +87,10 @@ float qk_scale(const grout_attn_dims* d) {
   return d->qk_scale > 0.f ? d->qk_scale : 1.0f / std::sqrt((float)d->head_dim);
 }
 
+// elem_bytes 2: f16; 1: bytes (8-bit codes).
 grout_status encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
-                        const uint64_t* strides_elems, const uint32_t* box, const char* what) {
+                        const uint64_t* strides_elems, const uint32_t* box, const char* what,
+                        int elem_bytes = 2) {
   if (!g_encode) return fail(GROUT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   cuuint64_t gd[5];
   cuuint64_t gs[4];
@@ -103,15 +105,16 @@ grout_status encode_map(CUtensorMap* m, const void* base, int rank, const uint64
                   (unsigned long long)dims[i]);
   }
   for (int i = 0; i + 1 < rank; ++i) {
-    gs[i] = strides_elems[i] * 2;
+    gs[i] = strides_elems[i] * (uint64_t)elem_bytes;
     if (gs[i] % 16 != 0 || gs[i] >= (1ull << 40))
       return fail(GROUT_ERR_INVALID_ARG, "%s: stride %d (%llu bytes) must be a multiple of 16",
                   what, i, (unsigned long long)gs[i]);
   }
-  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
-                        const_cast<void*>(base), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUtensorMapDataType type =
+      elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = g_encode(m, type, (cuuint32_t)rank, const_cast<void*>(base), gd, gs, bx, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(GROUT_ERR_CUDA, "%s: cuTensorMapEncodeTiled error %d", what, (int)r);
   return GROUT_OK;
 }
@@ -124,7 +127,7 @@ grout_status encode_map(CUtensorMap* m, const void* base, int rank, const uint64
 // (no workspace, no merge launch).
 int choose_splits(int32_t batch, int32_t max_kv_len, int32_t hkv, int num_sms) {
   const int keys = 64;
-  const int tiles = (max_kv_len + keys - 1) / keys;
+  const int tiles = (int)(((int64_t)max_kv_len + keys - 1) / keys);
   const int64_t units = (int64_t)batch * hkv;
   int64_t nks = (num_sms + units - 1) / units;
   const int64_t hi = std::max(1, tiles / 4);
@@ -180,6 +183,7 @@ grout_status grout_attn_init(int32_t device) {
     g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   }
   CUDA_TRY(decode_set_attributes());
+  CUDA_TRY(decode_window_set_attributes());
   CUDA_TRY(prefill_set_attributes());
   CUDA_TRY(qkv_gemm_set_attributes());
   void* err = nullptr;
@@ -343,7 +347,8 @@ grout_status grout_qk_norm_rope_kv_decode(const void* qkv, const void* q_norm_w,
 static grout_status prefill_common(const grout_prefill_varlen_args* p, int32_t single_len,
                                    int32_t single_pos0, const grout_attn_dims* dims,
                                    grout_stream_t stream, int32_t nsplit = 1,
-                                   void* workspace = nullptr, size_t workspace_bytes = 0) {
+                                   void* workspace = nullptr, size_t workspace_bytes = 0,
+                                   int32_t window = 0, int32_t sinks = 0) {
   grout_status st = check_dims(dims, 0);
   if (st != GROUT_OK) return st;
   if (p->batch == 0 || p->max_q_len == 0) return GROUT_OK;
@@ -405,6 +410,8 @@ static grout_status prefill_common(const grout_prefill_varlen_args* p, int32_t s
   a.scale_log2 = qk_scale(dims) / logf(2.0f);
   a.err = ds->err;
   a.nsplit = nsplit;
+  a.window = window;
+  a.sinks = sinks;
   if (nsplit > 1) {
     const size_t need = grout_attn_prefill_splitk_workspace_bytes(p->batch, p->max_q_len,
                                                                   (int32_t)hq, nsplit);
@@ -699,8 +706,9 @@ static grout_status check_pages(const void* k_pages, const void* v_pages, int32_
   return GROUT_OK;
 }
 
-grout_status grout_attn_prefill_paged(const grout_prefill_paged_args* p,
-                                      const grout_attn_dims* dims, grout_stream_t stream) {
+static grout_status prefill_paged_common(const grout_prefill_paged_args* p, int32_t window,
+                                         int32_t sinks, const grout_attn_dims* dims,
+                                         grout_stream_t stream) {
   if (!p) return fail(GROUT_ERR_INVALID_ARG, "args is null");
   grout_status st = check_dims(dims, 0);
   if (st != GROUT_OK) return st;
@@ -759,8 +767,15 @@ grout_status grout_attn_prefill_paged(const grout_prefill_paged_args* p,
   a.page_size = p->page_size;
   a.num_pages = p->num_pages;
   a.nsplit = 1;
+  a.window = window;
+  a.sinks = sinks;
   CUDA_TRY(launch_prefill(a, tq, tk, tv, reinterpret_cast<cudaStream_t>(stream)));
   return GROUT_OK;
+}
+
+grout_status grout_attn_prefill_paged(const grout_prefill_paged_args* args,
+                                      const grout_attn_dims* dims, grout_stream_t stream) {
+  return prefill_paged_common(args, 0, 0, dims, stream);
 }
 
 grout_status grout_attn_decode_paged(const void* q, const void* k_pages, const void* v_pages,
@@ -927,6 +942,380 @@ grout_status grout_qk_norm_rope_kv_prefill_paged(
   a.num_pages = num_pages;
   CUDA_TRY(launch_qk_norm_rope_kv(a, ds->num_sms, reinterpret_cast<cudaStream_t>(stream)));
   return GROUT_OK;
+}
+
+/* ------------------------------------------------- 8-bit paged KV cache */
+
+static grout_status check_fp8_pages(const grout_fp8_pages* p, const int32_t* page_table,
+                                    int64_t table_stride, const grout_attn_dims* dims) {
+  if (!p) return fail(GROUT_ERR_INVALID_ARG, "pages is null");
+  grout_status st = check_pages(p->k, p->v, p->num_pages, p->page_size, page_table, table_stride, dims);
+  if (st != GROUT_OK) return st;
+  if (!p->k_scales || !p->v_scales) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+  if (!aligned16(p->k_scales) || !aligned16(p->v_scales))
+    return fail(GROUT_ERR_INVALID_ARG, "page scales must be 16-byte aligned");
+  return GROUT_OK;
+}
+
+static Fp8Pages fp8_pages_of(const grout_fp8_pages* p) {
+  return Fp8Pages{static_cast<uint8_t*>(p->k), static_cast<uint8_t*>(p->v), p->k_scales, p->v_scales};
+}
+
+grout_status grout_qk_norm_rope_kv_decode_paged_fp8(
+    const void* qkv, const void* q_norm_w, const void* k_norm_w, const float* rope_table,
+    void* q_out, const grout_fp8_pages* pages, const int32_t* page_table, int32_t table_stride,
+    const uint32_t* d_position, int32_t batch, const grout_attn_dims* dims, grout_stream_t stream) {
+  grout_status st = check_dims(dims, 0);
+  if (st != GROUT_OK) return st;
+  if (batch < 0) return fail(GROUT_ERR_INVALID_ARG, "batch=%d", batch);
+  if (batch == 0) return GROUT_OK;
+  const void* ptrs[] = {qkv, q_norm_w, k_norm_w, rope_table, q_out};
+  for (const void* p : ptrs) {
+    if (!p) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+    if (!aligned16(p)) return fail(GROUT_ERR_INVALID_ARG, "pointer %p is not 16-byte aligned", p);
+  }
+  if (!d_position) return fail(GROUT_ERR_INVALID_ARG, "d_position is null");
+  st = check_fp8_pages(pages, page_table, table_stride, dims);
+  if (st != GROUT_OK) return st;
+  DeviceState* ds;
+  st = current_state(&ds);
+  if (st != GROUT_OK) return st;
+  NormRopeFp8Args a{};
+  a.q = static_cast<const __half*>(qkv);
+  a.q_row_stride = ((int64_t)dims->num_q_heads + 2 * (int64_t)dims->num_kv_heads) * 128;
+  a.q_w = static_cast<const __half*>(q_norm_w);
+  a.k_w = static_cast<const __half*>(k_norm_w);
+  a.table = rope_table;
+  a.q_out = static_cast<__half*>(q_out);
+  a.pages = fp8_pages_of(pages);
+  a.d_position = d_position;
+  a.rows = batch;
+  a.hq = dims->num_q_heads;
+  a.hkv = dims->num_kv_heads;
+  a.max_seq = dims->max_seq;
+  a.eps = dims->rms_eps;
+  a.err = ds->err;
+  a.page_table = page_table;
+  a.table_stride = table_stride;
+  a.page_size = pages->page_size;
+  a.num_pages = pages->num_pages;
+  CUDA_TRY(launch_qk_norm_rope_kv_fp8(a, ds->num_sms, reinterpret_cast<cudaStream_t>(stream)));
+  return GROUT_OK;
+}
+
+grout_status grout_qk_norm_rope_kv_prefill_paged_fp8(
+    const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t kv_row_stride,
+    const void* q_norm_w, const void* k_norm_w, const float* rope_table, void* q_out,
+    const grout_fp8_pages* pages, const int32_t* page_table, int32_t position_start,
+    int32_t seq_len, const grout_attn_dims* dims, grout_stream_t stream) {
+  grout_status st = check_dims(dims, 0);
+  if (st != GROUT_OK) return st;
+  if (seq_len < 0 || position_start < 0)
+    return fail(GROUT_ERR_INVALID_ARG, "seq_len=%d position_start=%d", seq_len, position_start);
+  if ((int64_t)position_start + seq_len > dims->max_seq)
+    return fail(GROUT_ERR_INVALID_ARG, "fused qk/rope/kv range [%d..%lld) exceeds max_seq %d",
+                position_start, (long long)position_start + seq_len, dims->max_seq);
+  if (seq_len == 0) return GROUT_OK;
+  const void* ptrs[] = {q, k, v, q_norm_w, k_norm_w, rope_table, q_out};
+  for (const void* p : ptrs) {
+    if (!p) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+    if (!aligned16(p)) return fail(GROUT_ERR_INVALID_ARG, "pointer %p is not 16-byte aligned", p);
+  }
+  // one table row of ceil(max_seq / page_size) entries
+  st = check_fp8_pages(pages, page_table, INT64_MAX, dims);
+  if (st != GROUT_OK) return st;
+  if (q_row_stride < (int64_t)dims->num_q_heads * 128 || q_row_stride % 8)
+    return fail(GROUT_ERR_INVALID_ARG, "q_row_stride=%lld", (long long)q_row_stride);
+  if (kv_row_stride < (int64_t)dims->num_kv_heads * 128 || kv_row_stride % 8)
+    return fail(GROUT_ERR_INVALID_ARG, "kv_row_stride=%lld", (long long)kv_row_stride);
+  DeviceState* ds;
+  st = current_state(&ds);
+  if (st != GROUT_OK) return st;
+  NormRopeFp8Args a{};
+  a.q = static_cast<const __half*>(q);
+  a.k = static_cast<const __half*>(k);
+  a.v = static_cast<const __half*>(v);
+  a.q_row_stride = q_row_stride;
+  a.kv_row_stride = kv_row_stride;
+  a.q_w = static_cast<const __half*>(q_norm_w);
+  a.k_w = static_cast<const __half*>(k_norm_w);
+  a.table = rope_table;
+  a.q_out = static_cast<__half*>(q_out);
+  a.pages = fp8_pages_of(pages);
+  a.pos0 = position_start;
+  a.rows = seq_len;
+  a.hq = dims->num_q_heads;
+  a.hkv = dims->num_kv_heads;
+  a.max_seq = dims->max_seq;
+  a.eps = dims->rms_eps;
+  a.err = ds->err;
+  a.page_table = page_table;
+  a.page_size = pages->page_size;
+  a.num_pages = pages->num_pages;
+  CUDA_TRY(launch_qk_norm_rope_kv_fp8(a, ds->num_sms, reinterpret_cast<cudaStream_t>(stream)));
+  return GROUT_OK;
+}
+
+grout_status grout_kv_read_paged_fp8(const grout_fp8_pages* pages, const int32_t* page_table,
+                                     int32_t table_stride, const int32_t* cu_seqlens,
+                                     const int32_t* position_start, int32_t batch, int64_t rows,
+                                     void* k_out, void* v_out, int64_t out_row_stride,
+                                     const grout_attn_dims* dims, grout_stream_t stream) {
+  grout_status st = check_dims(dims, 0);
+  if (st != GROUT_OK) return st;
+  if (batch < 0 || rows < 0)
+    return fail(GROUT_ERR_INVALID_ARG, "batch=%d rows=%lld", batch, (long long)rows);
+  if (batch == 0 || rows == 0) return GROUT_OK;
+  if (!cu_seqlens || !k_out || !v_out) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+  if (!aligned16(k_out) || !aligned16(v_out))
+    return fail(GROUT_ERR_INVALID_ARG, "k_out and v_out must be 16-byte aligned");
+  if (out_row_stride < (int64_t)dims->num_kv_heads * 128 || out_row_stride % 8)
+    return fail(GROUT_ERR_INVALID_ARG, "out_row_stride=%lld", (long long)out_row_stride);
+  if (rows > INT32_MAX || rows * dims->num_kv_heads > (int64_t)INT32_MAX * 16)
+    return fail(GROUT_ERR_INVALID_ARG, "rows=%lld is out of range", (long long)rows);
+  st = check_fp8_pages(pages, page_table, table_stride, dims);
+  if (st != GROUT_OK) return st;
+  DeviceState* ds;
+  st = current_state(&ds);
+  if (st != GROUT_OK) return st;
+  KvReadFp8Args a{};
+  a.pages = fp8_pages_of(pages);
+  a.page_table = page_table;
+  a.table_stride = table_stride;
+  a.page_size = pages->page_size;
+  a.num_pages = pages->num_pages;
+  a.cu = cu_seqlens;
+  a.first = position_start;
+  a.batch = batch;
+  a.hkv = dims->num_kv_heads;
+  a.rows = rows;
+  a.max_seq = dims->max_seq;
+  a.k_out = static_cast<__half*>(k_out);
+  a.v_out = static_cast<__half*>(v_out);
+  a.out_row_stride = out_row_stride;
+  a.err = ds->err;
+  CUDA_TRY(launch_kv_read_fp8(a, reinterpret_cast<cudaStream_t>(stream)));
+  return GROUT_OK;
+}
+
+/* --------------------------------- sliding-window attention with sinks */
+
+// Most 64-key tiles that a window decode reads: those of the sinks, and of a
+// window that starts and ends inside tiles.
+static int64_t window_tiles(int32_t max_kv_len, int32_t window, int32_t sinks) {
+  const int64_t all = ((int64_t)max_kv_len + 63) / 64;
+  if (window <= 0) return all;
+  return std::min(all, ((int64_t)sinks + 63) / 64 + ((int64_t)window + 62) / 64 + 1);
+}
+
+int32_t grout_attn_decode_window_splits(int32_t batch, int32_t max_kv_len, int32_t window,
+                                        int32_t sinks, const grout_attn_dims* dims) {
+  if (!dims || batch <= 0 || max_kv_len <= 0 || dims->num_kv_heads <= 0 || window < 0 || sinks < 0)
+    return 1;
+  DeviceState* ds;
+  int sms = 148;
+  if (current_state(&ds) == GROUT_OK) sms = ds->num_sms;
+  const int64_t keys = std::min<int64_t>(window_tiles(max_kv_len, window, sinks) * 64, INT32_MAX);
+  return choose_splits(batch, (int32_t)keys, dims->num_kv_heads, sms);
+}
+
+size_t grout_attn_decode_window_workspace_bytes(int32_t batch, int32_t max_kv_len, int32_t window,
+                                                int32_t sinks, int32_t num_splits,
+                                                const grout_attn_dims* dims) {
+  if (!dims || batch <= 0 || dims->num_q_heads <= 0) return 0;
+  if (num_splits <= 0)
+    num_splits = grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, dims);
+  return decode_ws_bytes(batch, dims->num_q_heads, num_splits);
+}
+
+// The checks and arguments that the window decode entry points share; fills
+// `a` but for the cache fields.
+static grout_status window_decode_args(DecodeWindowArgs* a, const void* q,
+                                       const uint32_t* d_position, void* out, int32_t batch,
+                                       int32_t max_kv_len, int32_t window, int32_t sinks,
+                                       int32_t num_splits, const grout_attn_dims* dims,
+                                       void* workspace, size_t workspace_bytes) {
+  if (!q || !out || !d_position) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+  if (!aligned16(q) || !aligned16(out))
+    return fail(GROUT_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
+  if (batch > 65535 || dims->num_kv_heads > 65535)
+    return fail(GROUT_ERR_UNSUPPORTED, "batch=%d num_kv_heads=%d (at most 65535 each)", batch,
+                dims->num_kv_heads);
+  if (max_kv_len <= 0 || max_kv_len > dims->max_seq)
+    return fail(GROUT_ERR_INVALID_ARG, "max_kv_len=%d must be in [1, max_seq=%d]", max_kv_len,
+                dims->max_seq);
+  if (num_splits == 0)
+    num_splits = grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, dims);
+  if (num_splits < 1 || num_splits > 1024)
+    return fail(GROUT_ERR_INVALID_ARG, "num_splits=%d", num_splits);
+  const size_t need = decode_ws_bytes(batch, dims->num_q_heads, num_splits);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(GROUT_ERR_INVALID_ARG, "workspace of %zu bytes (16-byte aligned) required, got %zu",
+                need, workspace ? workspace_bytes : (size_t)0);
+  DeviceState* ds;
+  grout_status st = current_state(&ds);
+  if (st != GROUT_OK) return st;
+  a->q = static_cast<const __half*>(q);
+  a->out = static_cast<__half*>(out);
+  a->part_o = need ? static_cast<float*>(workspace) : nullptr;
+  a->part_lse = need ? static_cast<float*>(workspace) + (size_t)batch * dims->num_q_heads * num_splits * 128
+                     : nullptr;
+  a->d_position = d_position;
+  a->batch = batch;
+  a->hq = dims->num_q_heads;
+  a->hkv = dims->num_kv_heads;
+  a->nks = num_splits;
+  a->cluster = num_splits > 1 && need == 0;
+  a->max_seq = dims->max_seq;
+  a->window = window;
+  a->sinks = sinks;
+  float scale = qk_scale(dims);
+  if (dims->flags & GROUT_FLAG_DECODE_SCALE_F16) scale = __half2float(__float2half_rn(scale));
+  a->scale_log2 = scale / logf(2.0f);
+  a->err = ds->err;
+  return GROUT_OK;
+}
+
+static grout_status check_window(int32_t window, int32_t sinks) {
+  if (window < 1 || sinks < 0)
+    return fail(GROUT_ERR_INVALID_ARG, "window=%d must be positive and sinks=%d not negative", window,
+                sinks);
+  return GROUT_OK;
+}
+
+grout_status grout_attn_decode_window(const void* q, const void* k_cache, const void* v_cache,
+                                      int64_t cache_batch_stride, int64_t cache_head_stride,
+                                      const uint32_t* d_position, void* out, int32_t batch,
+                                      int32_t max_kv_len, int32_t window, int32_t sinks,
+                                      int32_t num_splits, const grout_attn_dims* dims,
+                                      void* workspace, size_t workspace_bytes,
+                                      grout_stream_t stream) {
+  grout_status st = check_dims(dims, 8);
+  if (st != GROUT_OK) return st;
+  if (batch < 0) return fail(GROUT_ERR_INVALID_ARG, "batch=%d", batch);
+  if ((st = check_window(window, sinks)) != GROUT_OK) return st;
+  if (batch == 0) return GROUT_OK;
+  if (!k_cache || !v_cache) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+  if (!aligned16(k_cache) || !aligned16(v_cache))
+    return fail(GROUT_ERR_INVALID_ARG, "caches must be 16-byte aligned");
+  if (cache_head_stride < (int64_t)dims->max_seq * 128 || cache_head_stride % 8)
+    return fail(GROUT_ERR_INVALID_ARG, "cache_head_stride=%lld", (long long)cache_head_stride);
+  if (batch > 1 &&
+      (cache_batch_stride < cache_head_stride * dims->num_kv_heads || cache_batch_stride % 8))
+    return fail(GROUT_ERR_INVALID_ARG, "cache_batch_stride=%lld", (long long)cache_batch_stride);
+  DecodeWindowArgs a{};
+  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, dims,
+                          workspace, workspace_bytes);
+  if (st != GROUT_OK) return st;
+  CUtensorMap tk, tv;
+  const uint64_t dk[4] = {128, (uint64_t)dims->max_seq, (uint64_t)dims->num_kv_heads,
+                          (uint64_t)batch};
+  const uint64_t sk[3] = {128, (uint64_t)cache_head_stride,
+                          (uint64_t)(batch > 1 ? cache_batch_stride : cache_head_stride * dims->num_kv_heads)};
+  const uint32_t bk[4] = {64, 64, 1, 1};
+  st = encode_map(&tk, k_cache, 4, dk, sk, bk, "k_cache");
+  if (st != GROUT_OK) return st;
+  st = encode_map(&tv, v_cache, 4, dk, sk, bk, "v_cache");
+  if (st != GROUT_OK) return st;
+  CUDA_TRY(launch_decode_window(a, tk, tv, reinterpret_cast<cudaStream_t>(stream)));
+  return GROUT_OK;
+}
+
+grout_status grout_attn_decode_paged_window(const void* q, const void* k_pages,
+                                            const void* v_pages, int32_t num_pages,
+                                            int32_t page_size, const int32_t* page_table,
+                                            int32_t table_stride, const uint32_t* d_position,
+                                            void* out, int32_t batch, int32_t max_kv_len,
+                                            int32_t window, int32_t sinks, int32_t num_splits,
+                                            const grout_attn_dims* dims, void* workspace,
+                                            size_t workspace_bytes, grout_stream_t stream) {
+  grout_status st = check_dims(dims, 8);
+  if (st != GROUT_OK) return st;
+  if (batch < 0) return fail(GROUT_ERR_INVALID_ARG, "batch=%d", batch);
+  if ((st = check_window(window, sinks)) != GROUT_OK) return st;
+  if (batch == 0) return GROUT_OK;
+  st = check_pages(k_pages, v_pages, num_pages, page_size, page_table, table_stride, dims);
+  if (st != GROUT_OK) return st;
+  DecodeWindowArgs a{};
+  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, dims,
+                          workspace, workspace_bytes);
+  if (st != GROUT_OK) return st;
+  a.page_table = page_table;
+  a.table_stride = table_stride;
+  a.page_size = page_size;
+  a.num_pages = num_pages;
+  CUtensorMap tk, tv;
+  const uint64_t dk[4] = {128, (uint64_t)page_size, (uint64_t)dims->num_kv_heads,
+                          (uint64_t)num_pages};
+  const uint64_t sk[3] = {128, (uint64_t)page_size * 128,
+                          (uint64_t)page_size * 128 * (uint64_t)dims->num_kv_heads};
+  const uint32_t bk[4] = {64, 64, 1, 1};
+  st = encode_map(&tk, k_pages, 4, dk, sk, bk, "k_pages");
+  if (st != GROUT_OK) return st;
+  st = encode_map(&tv, v_pages, 4, dk, sk, bk, "v_pages");
+  if (st != GROUT_OK) return st;
+  CUDA_TRY(launch_decode_window(a, tk, tv, reinterpret_cast<cudaStream_t>(stream)));
+  return GROUT_OK;
+}
+
+grout_status grout_attn_decode_paged_fp8(const void* q, const grout_fp8_pages* pages,
+                                         const int32_t* page_table, int32_t table_stride,
+                                         const uint32_t* d_position, void* out, int32_t batch,
+                                         int32_t max_kv_len, int32_t window, int32_t sinks,
+                                         int32_t num_splits, const grout_attn_dims* dims,
+                                         void* workspace, size_t workspace_bytes,
+                                         grout_stream_t stream) {
+  grout_status st = check_dims(dims, 8);
+  if (st != GROUT_OK) return st;
+  if (batch < 0) return fail(GROUT_ERR_INVALID_ARG, "batch=%d", batch);
+  if (!(window == 0 && sinks == 0) && (st = check_window(window, sinks)) != GROUT_OK) return st;
+  if (batch == 0) return GROUT_OK;
+  st = check_fp8_pages(pages, page_table, table_stride, dims);
+  if (st != GROUT_OK) return st;
+  DecodeWindowArgs a{};
+  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, dims,
+                          workspace, workspace_bytes);
+  if (st != GROUT_OK) return st;
+  a.k_scales = pages->k_scales;
+  a.v_scales = pages->v_scales;
+  a.page_table = page_table;
+  a.table_stride = table_stride;
+  a.page_size = pages->page_size;
+  a.num_pages = pages->num_pages;
+  CUtensorMap tk, tv;
+  const uint64_t dk[4] = {128, (uint64_t)pages->page_size, (uint64_t)dims->num_kv_heads,
+                          (uint64_t)pages->num_pages};
+  const uint64_t sk[3] = {128, (uint64_t)pages->page_size * 128,
+                          (uint64_t)pages->page_size * 128 * (uint64_t)dims->num_kv_heads};
+  const uint32_t bk[4] = {128, 64, 1, 1};
+  st = encode_map(&tk, pages->k, 4, dk, sk, bk, "pages->k", 1);
+  if (st != GROUT_OK) return st;
+  st = encode_map(&tv, pages->v, 4, dk, sk, bk, "pages->v", 1);
+  if (st != GROUT_OK) return st;
+  CUDA_TRY(launch_decode_window(a, tk, tv, reinterpret_cast<cudaStream_t>(stream)));
+  return GROUT_OK;
+}
+
+grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* args,
+                                              int32_t window, int32_t sinks,
+                                              const grout_attn_dims* dims, grout_stream_t stream) {
+  if (!args) return fail(GROUT_ERR_INVALID_ARG, "args is null");
+  grout_status st = check_window(window, sinks);
+  if (st != GROUT_OK) return st;
+  if (!args->cu_seqlens_q && args->batch > 1)
+    return fail(GROUT_ERR_INVALID_ARG, "cu_seqlens_q is null with batch=%d", args->batch);
+  if (!args->cu_seqlens_q && args->q_rows < args->max_q_len)
+    return fail(GROUT_ERR_INVALID_ARG, "q_rows=%lld", (long long)args->q_rows);
+  return prefill_common(args, args->cu_seqlens_q ? 0 : args->max_q_len, 0, dims, stream, 1, nullptr,
+                        0, window, sinks);
+}
+
+grout_status grout_attn_prefill_paged_window(const grout_prefill_paged_args* args, int32_t window,
+                                             int32_t sinks, const grout_attn_dims* dims,
+                                             grout_stream_t stream) {
+  grout_status st = check_window(window, sinks);
+  if (st != GROUT_OK) return st;
+  return prefill_paged_common(args, window, sinks, dims, stream);
 }
 
 grout_status grout_qkv_proj_norm_rope_kv_prefill(

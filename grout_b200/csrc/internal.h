@@ -98,6 +98,97 @@ cudaError_t launch_decode(const DecodeArgs& a, const CUtensorMap& tm_k, const CU
                           cudaStream_t s);
 cudaError_t decode_set_attributes();
 
+// 8-bit paged cache: e4m3 codes [num_pages][hkv][page_size][128] and one f32
+// scale per row [num_pages][hkv][page_size] (fp8.cuh).
+struct Fp8Pages {
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scales;
+  float* v_scales;
+};
+
+// The fused norm/RoPE write into the 8-bit paged cache; fields as
+// NormRopeArgs (d_position != null: decode, else prefill of one sequence).
+struct NormRopeFp8Args {
+  const __half* q;
+  const __half* k;
+  const __half* v;
+  int64_t q_row_stride;
+  int64_t kv_row_stride;
+  const __half* q_w;
+  const __half* k_w;
+  const float* table;
+  __half* q_out;
+  Fp8Pages pages;
+  const uint32_t* d_position;
+  int32_t pos0;
+  int32_t rows;
+  int32_t hq;
+  int32_t hkv;
+  int32_t max_seq;
+  float eps;
+  int* err;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t page_size;
+  int32_t num_pages;
+};
+cudaError_t launch_qk_norm_rope_kv_fp8(const NormRopeFp8Args& a, int num_sms, cudaStream_t s);
+
+// Read-back of the 8-bit cache: output row r (of `rows`, stride
+// out_row_stride) of sequence b, cu[b] <= r < cu[b+1], is position
+// first[b] + r - cu[b] (first null: 0).
+struct KvReadFp8Args {
+  Fp8Pages pages;
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t page_size;
+  int32_t num_pages;
+  const int32_t* cu;
+  const int32_t* first;
+  int32_t batch;
+  int32_t hkv;
+  int64_t rows;
+  int32_t max_seq;
+  __half* k_out;
+  __half* v_out;
+  int64_t out_row_stride;
+  int* err;
+};
+cudaError_t launch_kv_read_fp8(const KvReadFp8Args& a, cudaStream_t s);
+
+// Decode attention over a window (window > 0: keys >= kv_len - window, and
+// keys < sinks; 0: all), f16 caches or, with k_scales != null, the 8-bit paged
+// one.  Fields as DecodeArgs.
+struct DecodeWindowArgs {
+  const __half* q;
+  __half* out;
+  float* part_o;
+  float* part_lse;
+  const uint32_t* d_position;
+  int32_t batch;
+  int32_t hq;
+  int32_t hkv;
+  int32_t nks;
+  int32_t cluster;
+  int32_t max_seq;
+  int32_t window;
+  int32_t sinks;
+  float scale_log2;
+  int* err;
+  const float* k_scales;
+  const float* v_scales;
+  const int32_t* page_table;
+  int32_t table_stride;
+  int32_t page_size;
+  int32_t num_pages;
+};
+// tm_k / tm_v: f16 as launch_decode; 8-bit {128, page_size, hkv, num_pages}
+// bytes, box {128, 64, 1, 1}, 128B swizzle.
+cudaError_t launch_decode_window(const DecodeWindowArgs& a, const CUtensorMap& tm_k,
+                                 const CUtensorMap& tm_v, cudaStream_t s);
+cudaError_t decode_window_set_attributes();
+
 struct PrefillArgs {
   __half* out;
   int64_t q_row_stride;
@@ -125,6 +216,10 @@ struct PrefillArgs {
   // part ([item][tile][128 rows][130] f32) and a merge kernel finishes.
   int32_t nsplit;
   float* part;
+  // Sliding window (window > 0, nsplit 1): row p sees keys n <= p with
+  // n > p - window or n < sinks.
+  int32_t window;
+  int32_t sinks;
 };
 
 // tm_q: 3-D {128, hq, q_rows}, box {64, 1, 128}; tm_k / tm_v: 4-D

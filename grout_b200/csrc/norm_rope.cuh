@@ -57,13 +57,13 @@ __device__ __forceinline__ void load_cos_sin(const float* trow, int j, float (&c
 }
 
 // RMSNorm of the octet's row (x = [xl | xh] as lane j's 16-byte chunks),
-// scaled by the norm weight (wl, wh), rotated by (cs, sn) and rounded to f16
-// once.  `mask` is the octet's lane mask for the butterfly.
-__device__ __forceinline__ void octet_norm_rope(const uint4& xl, const uint4& xh,
-                                                const float (&wl)[8], const float (&wh)[8],
-                                                const float (&cs)[8], const float (&sn)[8],
-                                                float eps, unsigned mask, uint4& out_lo,
-                                                uint4& out_hi) {
+// scaled by the norm weight (wl, wh) and rotated by (cs, sn), in f32.  `mask`
+// is the octet's lane mask for the butterfly.
+__device__ __forceinline__ void octet_norm_rope_f32(const uint4& xl, const uint4& xh,
+                                                    const float (&wl)[8], const float (&wh)[8],
+                                                    const float (&cs)[8], const float (&sn)[8],
+                                                    float eps, unsigned mask, float (&ylo)[8],
+                                                    float (&yhi)[8]) {
   float lo[8], hi[8];
   unpack8(xl, lo);
   unpack8(xh, hi);
@@ -77,7 +77,6 @@ __device__ __forceinline__ void octet_norm_rope(const uint4& xl, const uint4& xh
   // ss / 128 is an exact power-of-two scaling; the correctly rounded
   // reciprocal equals the IEEE quotient 1.0f / x.
   const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 0.0078125f), eps)));
-  float ylo[8], yhi[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float nlo = __fmul_rn(__fmul_rn(lo[e], inv), wl[e]);
@@ -85,6 +84,16 @@ __device__ __forceinline__ void octet_norm_rope(const uint4& xl, const uint4& xh
     ylo[e] = __fsub_rn(__fmul_rn(nlo, cs[e]), __fmul_rn(nhi, sn[e]));
     yhi[e] = __fadd_rn(__fmul_rn(nhi, cs[e]), __fmul_rn(nlo, sn[e]));
   }
+}
+
+// The same, rounded to f16 once.
+__device__ __forceinline__ void octet_norm_rope(const uint4& xl, const uint4& xh,
+                                                const float (&wl)[8], const float (&wh)[8],
+                                                const float (&cs)[8], const float (&sn)[8],
+                                                float eps, unsigned mask, uint4& out_lo,
+                                                uint4& out_hi) {
+  float ylo[8], yhi[8];
+  octet_norm_rope_f32(xl, xh, wl, wh, cs, sn, eps, mask, ylo, yhi);
   out_lo = pack8(ylo);
   out_hi = pack8(yhi);
 }

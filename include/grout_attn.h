@@ -426,6 +426,114 @@ grout_status grout_qk_norm_rope_kv_prefill_paged(
     const int32_t* page_table, int32_t position_start, int32_t seq_len,
     const grout_attn_dims* dims, grout_stream_t stream);
 
+/* ------------------------------------------------- 8-bit paged KV cache */
+
+/* No counterpart in the reference (f16 caches); half the cache's bytes and
+ * half of what decode reads.  Pools of e4m3 codes with one f32 scale per row
+ * (one token of one KV head):
+ *   k, v: [num_pages][num_kv_heads][page_size][128] e4m3 (one byte);
+ *   k_scales, v_scales: [num_pages][num_kv_heads][page_size] f32;
+ *   row y is stored as scale = max|y| / 448, code = e4m3(y * (448 / max|y|)),
+ *   nearest even, and stands for code * scale; a row with max|y| <= 2^-25 is
+ *   stored as zeros with scale 0.  A NaN stays a NaN, a row with an infinity
+ *   reads back as NaN.
+ * page_size, page_table and bad table entries as for the f16 paged caches
+ * (below 0 or >= num_pages: device error 0x201, writes skip the row,
+ * attention leaves the tile out, read-back gives zeros). */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scales;
+  float* v_scales;
+  int32_t num_pages;
+  int32_t page_size;
+} grout_fp8_pages;
+
+/* grout_qk_norm_rope_kv_decode_paged / _prefill_paged into the 8-bit cache:
+ * same norm, rotation and q_out bits; K is quantised from its f32 value
+ * (rounded once), V from its f16 value. */
+grout_status grout_qk_norm_rope_kv_decode_paged_fp8(
+    const void* qkv, const void* q_norm_w, const void* k_norm_w, const float* rope_table,
+    void* q_out, const grout_fp8_pages* pages, const int32_t* page_table, int32_t table_stride,
+    const uint32_t* d_position, int32_t batch, const grout_attn_dims* dims, grout_stream_t stream);
+grout_status grout_qk_norm_rope_kv_prefill_paged_fp8(
+    const void* q, const void* k, const void* v, int64_t q_row_stride, int64_t kv_row_stride,
+    const void* q_norm_w, const void* k_norm_w, const float* rope_table, void* q_out,
+    const grout_fp8_pages* pages, const int32_t* page_table, int32_t position_start,
+    int32_t seq_len, const grout_attn_dims* dims, grout_stream_t stream);
+
+/* Read-back of the 8-bit cache to packed f16 rows, f16(code * scale): row r of
+ * sequence b (cu_seqlens[b] <= r < cu_seqlens[b+1], DEVICE int32 [batch+1]) is
+ * position position_start[b] + r - cu_seqlens[b] (DEVICE int32 [batch], NULL =
+ * all 0).  k_out, v_out [rows][num_kv_heads][128], row stride out_row_stride;
+ * rows of no sequence (>= cu_seqlens[batch]) are left as they are; a position
+ * outside [0, max_seq) reads as zeros and records device error 0x200.  The
+ * result is what grout_attn_prefill_varlen and
+ * grout_attn_prefill_varlen_window take with kv_row_stride = out_row_stride,
+ * kv_head_stride = 128 and kv_start = cu_seqlens: attention of a chunk of new
+ * tokens over the 8-bit cache. */
+grout_status grout_kv_read_paged_fp8(const grout_fp8_pages* pages, const int32_t* page_table,
+                                     int32_t table_stride, const int32_t* cu_seqlens,
+                                     const int32_t* position_start, int32_t batch, int64_t rows,
+                                     void* k_out, void* v_out, int64_t out_row_stride,
+                                     const grout_attn_dims* dims, grout_stream_t stream);
+
+/* --------------------------------- sliding-window attention with sinks */
+
+/* No counterpart in the reference.  A query at position p sees key n if
+ * n <= p and (n > p - window or n < sinks): the last `window` keys, its own
+ * among them, and the first `sinks` keys of the sequence.  window >= 1 and
+ * sinks >= 0; a window of p + 1 or more sees every key.  Keys that no query of
+ * a call sees are not read past the 64-key blocks that hold a visible one:
+ * pages that lie wholly outside may be freed (any table entry, -1 for one)
+ * and their rows may hold anything. */
+
+/* Split count of the window decode entry points for num_splits = 0, and the
+ * workspace bytes they need (0 up to 16 splits); window 0 = the whole
+ * context (8-bit caches). */
+int32_t grout_attn_decode_window_splits(int32_t batch, int32_t max_kv_len, int32_t window,
+                                        int32_t sinks, const grout_attn_dims* dims);
+size_t grout_attn_decode_window_workspace_bytes(int32_t batch, int32_t max_kv_len, int32_t window,
+                                                int32_t sinks, int32_t num_splits,
+                                                const grout_attn_dims* dims);
+
+/* Window forms of grout_attn_decode_ex and grout_attn_decode_paged; arguments
+ * as there, num_splits 0 = the automatic count, at most 1024. */
+grout_status grout_attn_decode_window(const void* q, const void* k_cache, const void* v_cache,
+                                      int64_t cache_batch_stride, int64_t cache_head_stride,
+                                      const uint32_t* d_position, void* out, int32_t batch,
+                                      int32_t max_kv_len, int32_t window, int32_t sinks,
+                                      int32_t num_splits, const grout_attn_dims* dims,
+                                      void* workspace, size_t workspace_bytes,
+                                      grout_stream_t stream);
+grout_status grout_attn_decode_paged_window(const void* q, const void* k_pages,
+                                            const void* v_pages, int32_t num_pages,
+                                            int32_t page_size, const int32_t* page_table,
+                                            int32_t table_stride, const uint32_t* d_position,
+                                            void* out, int32_t batch, int32_t max_kv_len,
+                                            int32_t window, int32_t sinks, int32_t num_splits,
+                                            const grout_attn_dims* dims, void* workspace,
+                                            size_t workspace_bytes, grout_stream_t stream);
+/* Window forms of grout_attn_prefill_varlen (cu_seqlens_q may be NULL with
+ * batch 1: one sequence of max_q_len rows) and grout_attn_prefill_paged;
+ * arguments as there.  K/V rows that some row of a 256-row query block sees
+ * must be finite for the block's other rows (a weight of 0 times an infinity
+ * is a NaN); all other rows may hold anything. */
+grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* args,
+                                              int32_t window, int32_t sinks,
+                                              const grout_attn_dims* dims, grout_stream_t stream);
+grout_status grout_attn_prefill_paged_window(const grout_prefill_paged_args* args, int32_t window,
+                                             int32_t sinks, const grout_attn_dims* dims,
+                                             grout_stream_t stream);
+/* Decode over the 8-bit paged cache; window 0 (then sinks 0) = every key. */
+grout_status grout_attn_decode_paged_fp8(const void* q, const grout_fp8_pages* pages,
+                                         const int32_t* page_table, int32_t table_stride,
+                                         const uint32_t* d_position, void* out, int32_t batch,
+                                         int32_t max_kv_len, int32_t window, int32_t sinks,
+                                         int32_t num_splits, const grout_attn_dims* dims,
+                                         void* workspace, size_t workspace_bytes,
+                                         grout_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
