@@ -20,6 +20,7 @@ range problems raise GroutError before any launch, like the reference's
 device is not sm_100 the call raises.
 """
 import ctypes
+import functools
 import math
 import os
 
@@ -697,68 +698,108 @@ def attention_decode_noalloc(q, k_cache, v_cache, position, out, max_kv_len, qk_
 
 
 # ------------------------------------- 8-bit paged cache, sliding windows
+#
+# A decode step's kernel takes a few microseconds, so what these calls do on
+# the host is kept short: one test per tensor (its message is only made when it
+# fails), and structs and sizes that depend on plain numbers alone are kept.
+
+
+# The current stream's handle without a Stream object around it: 0.07 us
+# against 1.25 us for torch.cuda.current_stream(dev).cuda_stream.
+_raw_stream = torch._C._cuda_getCurrentRawStream if torch.cuda._is_compiled() else None
 
 
 def _enqueue(dev, fn, *args):
-    """Calls fn(*args, stream) on the current stream of the tensors' device."""
-    if dev.index == torch.cuda.current_device():
-        _check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    """Calls fn(*args, stream) on the current stream of device dev."""
+    if dev == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            _check(fn(*args, torch.cuda.current_stream().cuda_stream))
+            status = fn(*args, _raw_stream(dev))
+    if status:
+        _check(status)
 
 
-def _cuda(t, name, dtype, dev=None):
-    """t is a contiguous CUDA tensor of the type (and on the device); returns its device."""
+def _refuse_tensor(t, name, dtype, dev):
     _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
     _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
     _need(t.is_contiguous(), f"{name} must be contiguous")
-    _need(dev is None or t.device == dev, f"{name} is on {t.device}, not on {dev}")
-    return t.device
+    raise GroutError(1, f"{name} is on {t.device}, not on cuda:{dev}")
+
+
+def _device_of(t, name, dtype):
+    """The device index of t, a contiguous CUDA tensor of the type."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.is_contiguous()):
+        _refuse_tensor(t, name, dtype, None)
+    return t.get_device()
+
+
+def _cuda(t, name, dtype, dev):
+    """t must be a contiguous CUDA tensor of the type on device dev."""
+    try:
+        if t.get_device() == dev and t.dtype is dtype and t.is_contiguous():
+            return
+    except AttributeError:  # not a tensor
+        pass
+    _refuse_tensor(t, name, dtype, dev)
 
 
 def _positions(t, n, dev):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in (torch.int32, torch.uint32)
-          and t.is_contiguous() and t.numel() >= n and t.device == dev,
-          "position must be a contiguous device int32/uint32 tensor with one entry per sequence")
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == dev and t.numel() >= n
+            and (t.dtype is torch.int32 or t.dtype is torch.uint32) and t.is_contiguous()):
+        raise GroutError(1, "position must be a contiguous device int32/uint32 tensor with one entry "
+                            f"per sequence on cuda:{dev}")
 
 
 def _table(t, batch, dev):
     """[batch, table_stride] page table; returns the stride."""
     _cuda(t, "page_table", torch.int32, dev)
-    _need(t.dim() == 2 and t.shape[0] >= batch, f"page_table must be [batch, table_stride]: {tuple(t.shape)}")
-    return t.shape[1]
+    if t.dim() != 2 or t.size(0) < batch:
+        raise GroutError(1, f"page_table must be [batch, table_stride]: {tuple(t.shape)}")
+    return t.size(1)
 
 
 def _kv_pages(k_pages, v_pages, dtype, dev):
     _cuda(k_pages, "k_pages", dtype, dev)
     _cuda(v_pages, "v_pages", dtype, dev)
-    _need(k_pages.dim() == 4 and k_pages.shape[3] == HEAD_DIM,
-          f"k_pages must be [num_pages, Hkv, page_size, 128]: {tuple(k_pages.shape)}")
-    _need(v_pages.shape == k_pages.shape, "v_pages shape mismatch")
-    return k_pages.shape[:3]
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM:
+        raise GroutError(1, f"k_pages must be [num_pages, Hkv, page_size, 128]: {tuple(shape)}")
+    if v_pages.shape != shape:
+        raise GroutError(1, "v_pages shape mismatch")
+    return shape
 
 
 def _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev):
     """The C struct of an 8-bit page pool, its KV heads and page size."""
-    num_pages, hkv, page_size = _kv_pages(k_pages, v_pages, torch.float8_e4m3fn, dev)
-    for t, n in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-        _cuda(t, n, torch.float32, dev)
-        _need(t.shape == k_pages.shape[:3], f"{n} must be [num_pages, Hkv, page_size]: {tuple(t.shape)}")
+    num_pages, hkv, page_size, _ = shape = _kv_pages(k_pages, v_pages, torch.float8_e4m3fn, dev)
+    _cuda(k_scales, "k_scales", torch.float32, dev)
+    _cuda(v_scales, "v_scales", torch.float32, dev)
+    if k_scales.shape != shape[:3] or v_scales.shape != shape[:3]:
+        raise GroutError(1, "k_scales and v_scales must be [num_pages, Hkv, page_size]: "
+                            f"{tuple(k_scales.shape)}, {tuple(v_scales.shape)}")
     return Fp8Pages(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                     num_pages, page_size), hkv, page_size
 
 
 def _rope(t, max_seq, dev):
     _cuda(t, "rope_table", torch.float32, dev)
-    _need(t.dim() == 2 and t.shape[1] == HEAD_DIM and t.shape[0] >= max_seq,
-          f"rope_table must be [>= max_seq={max_seq}, 128] f32: {tuple(t.shape)}")
+    if t.dim() != 2 or t.size(1) != HEAD_DIM or t.size(0) < max_seq:
+        raise GroutError(1, f"rope_table must be [>= max_seq={max_seq}, 128] f32: {tuple(t.shape)}")
 
 
 def _norm_weights(q_norm_w, k_norm_w, dev):
-    for t, n in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
-        _cuda(t, n, torch.float16, dev)
-        _need(t.numel() == HEAD_DIM, f"{n} must have 128 entries")
+    _cuda(q_norm_w, "q_norm_w", torch.float16, dev)
+    _cuda(k_norm_w, "k_norm_w", torch.float16, dev)
+    if q_norm_w.numel() != HEAD_DIM or k_norm_w.numel() != HEAD_DIM:
+        raise GroutError(1, "q_norm_w and k_norm_w must have 128 entries")
+
+
+@functools.lru_cache(maxsize=1024)
+def _dims(num_q_heads, num_kv_heads, max_seq, rms_eps, qk_scale, flags):
+    """AttnDims of these numbers (read only)."""
+    return AttnDims(num_q_heads, num_kv_heads, HEAD_DIM, max_seq, rms_eps,
+                    float(qk_scale) if qk_scale else 0.0, flags)
 
 
 def qk_norm_rope_kv_decode_paged_fp8(qkv, q_norm_w, k_norm_w, rope_table, q_out, k_pages, v_pages,
@@ -768,15 +809,17 @@ def qk_norm_rope_kv_decode_paged_fp8(qkv, q_norm_w, k_norm_w, rope_table, q_out,
     v_pages [num_pages, Hkv, page_size, 128] float8_e4m3fn with one f32 scale
     per row in k_scales, v_scales [num_pages, Hkv, page_size].  A row y is
     stored as scale = max|y| / 448, code = e4m3(y * (448 / max|y|))."""
-    dev = _cuda(qkv, "qkv", torch.float16)
+    dev = _device_of(qkv, "qkv", torch.float16)
     _cuda(q_out, "q_out", torch.float16, dev)
     _norm_weights(q_norm_w, k_norm_w, dev)
     pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    hq = num_q_heads
-    _need(hkv == num_kv_heads, "k_pages head count mismatch")
-    B = qkv.shape[0] if qkv.dim() == 2 else 1
-    _need(qkv.numel() == B * (hq + 2 * hkv) * HEAD_DIM, f"qkv shape mismatch: {tuple(qkv.shape)}")
-    _need(q_out.numel() == B * hq * HEAD_DIM, f"q_out shape mismatch: {tuple(q_out.shape)}")
+    if hkv != num_kv_heads:
+        raise GroutError(1, f"k_pages has {hkv} KV heads, not {num_kv_heads}")
+    B = qkv.size(0) if qkv.dim() == 2 else 1
+    if qkv.numel() != B * (num_q_heads + 2 * hkv) * HEAD_DIM:
+        raise GroutError(1, f"qkv shape mismatch: {tuple(qkv.shape)}")
+    if q_out.numel() != B * num_q_heads * HEAD_DIM:
+        raise GroutError(1, f"q_out shape mismatch: {tuple(q_out.shape)}")
     _positions(position, B, dev)
     stride = _table(page_table, B, dev)
     if max_seq is None:
@@ -785,7 +828,7 @@ def qk_norm_rope_kv_decode_paged_fp8(qkv, q_norm_w, k_norm_w, rope_table, q_out,
     _enqueue(dev, lib().grout_qk_norm_rope_kv_decode_paged_fp8, qkv.data_ptr(), q_norm_w.data_ptr(),
              k_norm_w.data_ptr(), rope_table.data_ptr(), q_out.data_ptr(), pages,
              page_table.data_ptr(), stride, position.data_ptr(), B,
-             AttnDims(hq, hkv, HEAD_DIM, max_seq, eps, 0.0, 0))
+             _dims(num_q_heads, hkv, max_seq, eps, 0.0, 0))
     return q_out
 
 
@@ -795,31 +838,36 @@ def qk_norm_rope_kv_prefill_paged_fp8(q, k, v, q_norm_w, k_norm_w, rope_table, q
     """qk_norm_rope_kv_prefill_paged into the 8-bit paged cache (see
     qk_norm_rope_kv_decode_paged_fp8): one sequence, page_table_row is its row
     of the page table."""
-    dev = _cuda(q, "q", torch.float16)
+    dev = _device_of(q, "q", torch.float16)
     for t, n in ((k, "k"), (v, "v"), (q_out, "q_out")):
         _cuda(t, n, torch.float16, dev)
     _norm_weights(q_norm_w, k_norm_w, dev)
     pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    _need(q.dim() == 3 and q.shape[2] == HEAD_DIM, f"q shape mismatch: {tuple(q.shape)}")
+    if q.dim() != 3 or q.size(2) != HEAD_DIM:
+        raise GroutError(1, f"q shape mismatch: {tuple(q.shape)}")
     S, hq, _ = q.shape
-    _need(k.shape == (S, hkv, HEAD_DIM) and v.shape == k.shape, "k/v shape mismatch")
-    _need(q_out.shape == q.shape, "q_out shape mismatch")
+    if k.shape != (S, hkv, HEAD_DIM) or v.shape != k.shape:
+        raise GroutError(1, f"k/v shape mismatch: {tuple(k.shape)}, {tuple(v.shape)}")
+    if q_out.shape != q.shape:
+        raise GroutError(1, f"q_out shape mismatch: {tuple(q_out.shape)}")
     _cuda(page_table_row, "page_table_row", torch.int32, dev)
     if max_seq is None:
         max_seq = page_table_row.numel() * page_size
-    _need(page_table_row.numel() * page_size >= max_seq, "page_table_row shorter than max_seq")
+    if page_table_row.numel() * page_size < max_seq:
+        raise GroutError(1, "page_table_row shorter than max_seq")
     _rope(rope_table, max_seq, dev)
     _enqueue(dev, lib().grout_qk_norm_rope_kv_prefill_paged_fp8, q.data_ptr(), k.data_ptr(),
              v.data_ptr(), hq * HEAD_DIM, hkv * HEAD_DIM, q_norm_w.data_ptr(), k_norm_w.data_ptr(),
              rope_table.data_ptr(), q_out.data_ptr(), pages, page_table_row.data_ptr(),
-             int(position_start), S, AttnDims(hq, hkv, HEAD_DIM, max_seq, eps, 0.0, 0))
+             int(position_start), S, _dims(hq, hkv, max_seq, eps, 0.0, 0))
     return q_out
 
 
 def _cu_seqlens(t, dev):
     """Device int32 [batch + 1]; returns the batch."""
     _cuda(t, "cu_seqlens", torch.int32, dev)
-    _need(t.dim() == 1 and t.numel() >= 1, f"cu_seqlens must be [batch + 1]: {tuple(t.shape)}")
+    if t.dim() != 1 or t.numel() < 1:
+        raise GroutError(1, f"cu_seqlens must be [batch + 1]: {tuple(t.shape)}")
     return t.numel() - 1
 
 
@@ -827,7 +875,8 @@ def _starts(t, batch, dev, name="position_start"):
     if t is None:
         return None
     _cuda(t, name, torch.int32, dev)
-    _need(t.numel() >= batch, f"{name} needs one entry per sequence")
+    if t.numel() < batch:
+        raise GroutError(1, f"{name} needs one entry per sequence")
     return t.data_ptr()
 
 
@@ -838,22 +887,23 @@ def kv_read_paged_fp8(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v
     position position_start[b] (default 0) on; cu_seqlens, position_start
     device int32.  Rows behind the last sequence are left as they are.
     attention_prefill_varlen(_window) takes the result with kv_row_stride =
-    Hkv * 128, kv_head_stride = 128, kv_start = cu_seqlens[:-1]: attention of
-    a chunk of new tokens over the 8-bit cache."""
-    dev = _cuda(k_out, "k_out", torch.float16)
+    Hkv * 128, kv_head_stride = 128, kv_start = cu_seqlens: attention of a
+    chunk of new tokens over the 8-bit cache."""
+    dev = _device_of(k_out, "k_out", torch.float16)
     _cuda(v_out, "v_out", torch.float16, dev)
     pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    _need(k_out.dim() == 3 and k_out.shape[1:] == (hkv, HEAD_DIM),
-          f"k_out must be [rows, {hkv}, 128]: {tuple(k_out.shape)}")
-    _need(v_out.shape == k_out.shape, "v_out shape mismatch")
+    shape = k_out.shape
+    if len(shape) != 3 or shape[1] != hkv or shape[2] != HEAD_DIM:
+        raise GroutError(1, f"k_out must be [rows, {hkv}, 128]: {tuple(shape)}")
+    if v_out.shape != shape:
+        raise GroutError(1, "v_out shape mismatch")
     B = _cu_seqlens(cu_seqlens, dev)
     start = _starts(position_start, B, dev)
     stride = _table(page_table, B, dev)
-    if max_seq is None:
-        max_seq = stride * page_size
     _enqueue(dev, lib().grout_kv_read_paged_fp8, pages, page_table.data_ptr(), stride,
-             cu_seqlens.data_ptr(), start, B, k_out.shape[0], k_out.data_ptr(), v_out.data_ptr(),
-             hkv * HEAD_DIM, AttnDims(hkv, hkv, HEAD_DIM, max_seq, 0.0, 0.0, 0))
+             cu_seqlens.data_ptr(), start, B, shape[0], k_out.data_ptr(), v_out.data_ptr(),
+             hkv * HEAD_DIM,
+             _dims(hkv, hkv, stride * page_size if max_seq is None else max_seq, 0.0, 0.0, 0))
     return k_out, v_out
 
 
@@ -871,32 +921,44 @@ def decode_window_workspace_bytes(batch, max_kv_len, window, sinks, num_q_heads,
                                                           num_splits, dims)
 
 
+@functools.lru_cache(maxsize=4096)
+def _window_need(dev, *args):
+    """decode_window_workspace_bytes on device dev (a function of the numbers alone)."""
+    with torch.cuda.device(dev):
+        return decode_window_workspace_bytes(*args)
+
+
 def _decode_window(fn, cache_args, q, out, dev, position, max_kv_len, window, sinks, num_splits,
                    workspace, hkv, max_seq, qk_scale, scale_f16):
     """The tail of the window decode calls: fn(q, *cache_args, position, out, ...)."""
-    B, hq = q.shape[0], q.shape[1]
+    B, hq, _ = q.shape
     _cuda(out, "out", torch.float16, dev)
-    _need(out.shape == q.shape, "out shape mismatch")
+    if out.shape != q.shape:
+        raise GroutError(1, "out shape mismatch")
     _positions(position, B, dev)
-    dims = AttnDims(hq, hkv, HEAD_DIM, max_seq, 0.0, float(qk_scale) if qk_scale else 0.0,
-                    FLAG_DECODE_SCALE_F16 if scale_f16 else 0)
-    num_splits = int(num_splits or 0)
-    need = lib().grout_attn_decode_window_workspace_bytes(B, max_kv_len, window, sinks, num_splits, dims)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    num_splits = num_splits or 0
     ws, ws_bytes = None, 0
     if workspace is not None:
-        _need(workspace.is_cuda and workspace.device == dev and workspace.is_contiguous(),
-              "workspace must be a contiguous tensor on the call's device")
+        if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.is_contiguous()
+                and workspace.get_device() == dev):
+            raise GroutError(1, f"workspace must be a contiguous tensor on cuda:{dev}")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    else:
+        need = _window_need(dev, B, max_kv_len, window, sinks, hq, hkv, max_seq, num_splits)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            ws, ws_bytes = workspace.data_ptr(), need
     _enqueue(dev, fn, q.data_ptr(), *cache_args, position.data_ptr(), out.data_ptr(), B, max_kv_len,
-             window, sinks, num_splits, dims, ws, ws_bytes)
+             window, sinks, num_splits,
+             _dims(hq, hkv, max_seq, 0.0, qk_scale, FLAG_DECODE_SCALE_F16 if scale_f16 else 0),
+             ws, ws_bytes)
     return out
 
 
 def _decode_query(q):
-    dev = _cuda(q, "q", torch.float16)
-    _need(q.dim() == 3 and q.shape[2] == HEAD_DIM, f"q must be [B, Hq, 128]: {tuple(q.shape)}")
+    dev = _device_of(q, "q", torch.float16)
+    if q.dim() != 3 or q.size(2) != HEAD_DIM:
+        raise GroutError(1, f"q must be [B, Hq, 128]: {tuple(q.shape)}")
     return dev
 
 
@@ -909,10 +971,12 @@ def attention_decode_window(q, k_cache, v_cache, position, out, max_kv_len, wind
     dev = _decode_query(q)
     _cuda(k_cache, "k_cache", torch.float16, dev)
     _cuda(v_cache, "v_cache", torch.float16, dev)
-    _need(k_cache.dim() == 4 and k_cache.shape[0] >= q.shape[0] and k_cache.shape[3] == HEAD_DIM,
-          f"k_cache must be [B, Hkv, max_seq, 128]: {tuple(k_cache.shape)}")
-    _need(v_cache.shape == k_cache.shape, "v_cache shape mismatch")
-    hkv, max_seq = k_cache.shape[1], k_cache.shape[2]
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[0] < q.size(0) or shape[3] != HEAD_DIM:
+        raise GroutError(1, f"k_cache must be [B, Hkv, max_seq, 128]: {tuple(shape)}")
+    if v_cache.shape != shape:
+        raise GroutError(1, "v_cache shape mismatch")
+    _, hkv, max_seq, _ = shape
     return _decode_window(lib().grout_attn_decode_window,
                           (k_cache.data_ptr(), v_cache.data_ptr(), hkv * max_seq * HEAD_DIM, max_seq * HEAD_DIM),
                           q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
@@ -926,8 +990,8 @@ def attention_decode_paged_window(q, k_pages, v_pages, page_table, position, out
     attention_decode_window).  Pages that hold no visible key may be freed:
     their table entries are not looked at."""
     dev = _decode_query(q)
-    num_pages, hkv, page_size = _kv_pages(k_pages, v_pages, torch.float16, dev)
-    stride = _table(page_table, q.shape[0], dev)
+    num_pages, hkv, page_size, _ = _kv_pages(k_pages, v_pages, torch.float16, dev)
+    stride = _table(page_table, q.size(0), dev)
     return _decode_window(lib().grout_attn_decode_paged_window,
                           (k_pages.data_ptr(), v_pages.data_ptr(), num_pages, page_size,
                            page_table.data_ptr(), stride),
@@ -943,18 +1007,29 @@ def attention_decode_paged_fp8(q, k_pages, v_pages, k_scales, v_scales, page_tab
     else as attention_decode_paged_window."""
     dev = _decode_query(q)
     pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    stride = _table(page_table, q.shape[0], dev)
+    stride = _table(page_table, q.size(0), dev)
     return _decode_window(lib().grout_attn_decode_paged_fp8, (pages, page_table.data_ptr(), stride),
                           q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
                           stride * page_size if max_seq is None else max_seq, qk_scale, scale_f16)
 
 
 def _chunk_query(q, out):
-    dev = _cuda(q, "q", torch.float16)
-    _need(q.dim() == 3 and q.shape[2] == HEAD_DIM, f"q must be [q_rows, Hq, 128]: {tuple(q.shape)}")
+    dev = _device_of(q, "q", torch.float16)
+    if q.dim() != 3 or q.size(2) != HEAD_DIM:
+        raise GroutError(1, f"q must be [q_rows, Hq, 128]: {tuple(q.shape)}")
     _cuda(out, "out", torch.float16, dev)
-    _need(out.shape == q.shape, "out shape mismatch")
+    if out.shape != q.shape:
+        raise GroutError(1, "out shape mismatch")
     return dev
+
+
+def _chunk_batch(cu_seqlens_q, max_q_len, rows, dev):
+    """(batch, cu_seqlens pointer, max_q_len) of a chunk call."""
+    if cu_seqlens_q is None:
+        return 1, None, rows if max_q_len is None else max_q_len
+    if max_q_len is None:
+        raise GroutError(1, "max_q_len is required with cu_seqlens_q")
+    return _cu_seqlens(cu_seqlens_q, dev), cu_seqlens_q.data_ptr(), max_q_len
 
 
 def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads,
@@ -967,25 +1042,23 @@ def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_k
     dev = _chunk_query(q, out)
     _cuda(k, "k", torch.float16, dev)
     _cuda(v, "v", torch.float16, dev)
-    rows, hq = q.shape[0], q.shape[1]
-    B = 1 if cu_seqlens_q is None else _cu_seqlens(cu_seqlens_q, dev)
-    if cu_seqlens_q is None:
-        max_q_len = rows if max_q_len is None else max_q_len
-    _need(max_q_len is not None, "max_q_len is required with cu_seqlens_q")
-    _need(kv_row_stride > 0 and kv_head_stride > 0 and kv_batch_stride >= 0, "bad kv strides")
+    rows, hq, _ = q.shape
+    B, cu, max_q_len = _chunk_batch(cu_seqlens_q, max_q_len, rows, dev)
+    if kv_row_stride <= 0 or kv_head_stride <= 0 or kv_batch_stride < 0 or num_kv_heads <= 0:
+        raise GroutError(1, "bad kv strides")
     # the furthest element that the strides address lies in k and v
     fixed = max(0, B - 1) * kv_batch_stride + (num_kv_heads - 1) * kv_head_stride + HEAD_DIM
     most = (min(k.numel(), v.numel()) - fixed) // kv_row_stride + 1
     if kv_rows is None:
         kv_rows = most
-    _need(0 < kv_rows <= most, f"kv_rows={kv_rows}: k and v hold {most} rows at these strides")
+    if not 0 < kv_rows <= most:
+        raise GroutError(1, f"kv_rows={kv_rows}: k and v hold {most} rows at these strides")
     args = PrefillVarlenArgs(
         q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k.data_ptr(), v.data_ptr(),
-        kv_batch_stride, kv_row_stride, kv_head_stride, kv_rows,
-        None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+        kv_batch_stride, kv_row_stride, kv_head_stride, kv_rows, cu,
         _starts(position_start, B, dev), _starts(kv_start, B, dev, "kv_start"), B, max_q_len)
     _enqueue(dev, lib().grout_attn_prefill_varlen_window, args, window, sinks,
-             make_dims(hq, num_kv_heads, 1 << 30, qk_scale=qk_scale))
+             _dims(hq, num_kv_heads, 1 << 30, 0.0, qk_scale, 0))
     return out
 
 
@@ -996,20 +1069,16 @@ def attention_prefill_paged_window(q, k_pages, v_pages, page_table, out, window,
     attention_prefill_varlen_window).  Pages that hold no key a row of the
     chunk sees may be freed: their table entries are not looked at."""
     dev = _chunk_query(q, out)
-    num_pages, hkv, page_size = _kv_pages(k_pages, v_pages, torch.float16, dev)
-    rows, hq = q.shape[0], q.shape[1]
-    B = 1 if cu_seqlens_q is None else _cu_seqlens(cu_seqlens_q, dev)
-    if cu_seqlens_q is None:
-        max_q_len = rows if max_q_len is None else max_q_len
-    _need(max_q_len is not None, "max_q_len is required with cu_seqlens_q")
+    num_pages, hkv, page_size, _ = _kv_pages(k_pages, v_pages, torch.float16, dev)
+    rows, hq, _ = q.shape
+    B, cu, max_q_len = _chunk_batch(cu_seqlens_q, max_q_len, rows, dev)
     stride = _table(page_table, B, dev)
     args = PrefillPagedArgs(
         q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k_pages.data_ptr(), v_pages.data_ptr(),
-        num_pages, page_size, page_table.data_ptr(), stride,
-        None if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-        _starts(position_start, B, dev), B, max_q_len)
+        num_pages, page_size, page_table.data_ptr(), stride, cu, _starts(position_start, B, dev), B,
+        max_q_len)
     _enqueue(dev, lib().grout_attn_prefill_paged_window, args, window, sinks,
-             make_dims(hq, hkv, stride * page_size if max_seq is None else max_seq, qk_scale=qk_scale))
+             _dims(hq, hkv, stride * page_size if max_seq is None else max_seq, 0.0, qk_scale, 0))
     return out
 
 
