@@ -184,6 +184,7 @@ grout_status grout_attn_init(int32_t device) {
   }
   CUDA_TRY(decode_set_attributes());
   CUDA_TRY(decode_window_set_attributes());
+  CUDA_TRY(prefill_window_set_attributes());
   CUDA_TRY(prefill_set_attributes());
   CUDA_TRY(qkv_gemm_set_attributes());
   void* err = nullptr;
@@ -347,8 +348,7 @@ grout_status grout_qk_norm_rope_kv_decode(const void* qkv, const void* q_norm_w,
 static grout_status prefill_common(const grout_prefill_varlen_args* p, int32_t single_len,
                                    int32_t single_pos0, const grout_attn_dims* dims,
                                    grout_stream_t stream, int32_t nsplit = 1,
-                                   void* workspace = nullptr, size_t workspace_bytes = 0,
-                                   int32_t window = 0, int32_t sinks = 0) {
+                                   void* workspace = nullptr, size_t workspace_bytes = 0) {
   grout_status st = check_dims(dims, 0);
   if (st != GROUT_OK) return st;
   if (p->batch == 0 || p->max_q_len == 0) return GROUT_OK;
@@ -410,8 +410,6 @@ static grout_status prefill_common(const grout_prefill_varlen_args* p, int32_t s
   a.scale_log2 = qk_scale(dims) / logf(2.0f);
   a.err = ds->err;
   a.nsplit = nsplit;
-  a.window = window;
-  a.sinks = sinks;
   if (nsplit > 1) {
     const size_t need = grout_attn_prefill_splitk_workspace_bytes(p->batch, p->max_q_len,
                                                                   (int32_t)hq, nsplit);
@@ -706,9 +704,8 @@ static grout_status check_pages(const void* k_pages, const void* v_pages, int32_
   return GROUT_OK;
 }
 
-static grout_status prefill_paged_common(const grout_prefill_paged_args* p, int32_t window,
-                                         int32_t sinks, const grout_attn_dims* dims,
-                                         grout_stream_t stream) {
+grout_status grout_attn_prefill_paged(const grout_prefill_paged_args* p,
+                                      const grout_attn_dims* dims, grout_stream_t stream) {
   if (!p) return fail(GROUT_ERR_INVALID_ARG, "args is null");
   grout_status st = check_dims(dims, 0);
   if (st != GROUT_OK) return st;
@@ -767,15 +764,8 @@ static grout_status prefill_paged_common(const grout_prefill_paged_args* p, int3
   a.page_size = p->page_size;
   a.num_pages = p->num_pages;
   a.nsplit = 1;
-  a.window = window;
-  a.sinks = sinks;
   CUDA_TRY(launch_prefill(a, tq, tk, tv, reinterpret_cast<cudaStream_t>(stream)));
   return GROUT_OK;
-}
-
-grout_status grout_attn_prefill_paged(const grout_prefill_paged_args* args,
-                                      const grout_attn_dims* dims, grout_stream_t stream) {
-  return prefill_paged_common(args, 0, 0, dims, stream);
 }
 
 grout_status grout_attn_decode_paged(const void* q, const void* k_pages, const void* v_pages,
@@ -1296,26 +1286,126 @@ grout_status grout_attn_decode_paged_fp8(const void* q, const grout_fp8_pages* p
   return GROUT_OK;
 }
 
-grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* args,
-                                              int32_t window, int32_t sinks,
-                                              const grout_attn_dims* dims, grout_stream_t stream) {
-  if (!args) return fail(GROUT_ERR_INVALID_ARG, "args is null");
-  grout_status st = check_window(window, sinks);
+// The checks and the launch that the window prefill entry points share; `a`
+// comes with the cache fields set (max_keys: positions per sequence), dk and sk
+// are the K/V maps' dims and strides.
+static grout_status window_prefill(PrefillWindowArgs* a, const void* q, void* out,
+                                   int64_t q_row_stride, int64_t q_rows, const void* k,
+                                   const void* v, const uint64_t* dk, const uint64_t* sk,
+                                   const int32_t* cu_seqlens_q, const int32_t* position_start,
+                                   int32_t batch, int32_t max_q_len, int32_t window, int32_t sinks,
+                                   const grout_attn_dims* dims, grout_stream_t stream) {
+  const int64_t hq = dims->num_q_heads, hkv = dims->num_kv_heads;
+  if (!q || !out) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+  if (!aligned16(q) || !aligned16(out))
+    return fail(GROUT_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
+  if (!cu_seqlens_q && batch != 1)
+    return fail(GROUT_ERR_INVALID_ARG, "cu_seqlens_q is null with batch=%d", batch);
+  if (q_row_stride < hq * 128 || q_row_stride % 8)
+    return fail(GROUT_ERR_INVALID_ARG, "q_row_stride=%lld", (long long)q_row_stride);
+  if (q_rows <= 0 || q_rows > INT32_MAX || (!cu_seqlens_q && q_rows < max_q_len))
+    return fail(GROUT_ERR_INVALID_ARG, "q_rows=%lld", (long long)q_rows);
+  DeviceState* ds;
+  grout_status st = current_state(&ds);
   if (st != GROUT_OK) return st;
-  if (!args->cu_seqlens_q && args->batch > 1)
-    return fail(GROUT_ERR_INVALID_ARG, "cu_seqlens_q is null with batch=%d", args->batch);
-  if (!args->cu_seqlens_q && args->q_rows < args->max_q_len)
-    return fail(GROUT_ERR_INVALID_ARG, "q_rows=%lld", (long long)args->q_rows);
-  return prefill_common(args, args->cu_seqlens_q ? 0 : args->max_q_len, 0, dims, stream, 1, nullptr,
-                        0, window, sinks);
+  const int32_t group = (int32_t)(hq / hkv);
+  a->tok = 128 / group;
+  CUtensorMap tq, tk, tv;
+  const uint64_t dq[3] = {128, (uint64_t)hq, (uint64_t)q_rows};
+  const uint64_t sq[2] = {128, (uint64_t)q_row_stride};
+  const uint32_t bq[3] = {64, (uint32_t)group, (uint32_t)a->tok};
+  st = encode_map(&tq, q, 3, dq, sq, bq, "q");
+  if (st != GROUT_OK) return st;
+  const uint32_t bk[4] = {64, 64, 1, 1};
+  st = encode_map(&tk, k, 4, dk, sk, bk, "k");
+  if (st != GROUT_OK) return st;
+  st = encode_map(&tv, v, 4, dk, sk, bk, "v");
+  if (st != GROUT_OK) return st;
+  a->out = static_cast<__half*>(out);
+  a->q_row_stride = q_row_stride;
+  a->q_rows = q_rows;
+  a->cu_q = cu_seqlens_q;
+  a->pos0 = position_start;
+  a->batch = batch;
+  a->single_len = max_q_len;
+  a->hq = (int32_t)hq;
+  a->hkv = (int32_t)hkv;
+  a->scale_log2 = qk_scale(dims) / logf(2.0f);
+  a->window = window;
+  a->sinks = sinks;
+  a->err = ds->err;
+  CUDA_TRY(launch_prefill_window(*a, max_q_len, ds->num_sms, tq, tk, tv,
+                                 reinterpret_cast<cudaStream_t>(stream)));
+  return GROUT_OK;
 }
 
-grout_status grout_attn_prefill_paged_window(const grout_prefill_paged_args* args, int32_t window,
+// Position arithmetic of the window prefill stays in 31 bits.
+constexpr int64_t kMaxKeys = INT32_MAX - 4096;
+
+grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* p, int32_t window,
+                                              int32_t sinks, const grout_attn_dims* dims,
+                                              grout_stream_t stream) {
+  if (!p) return fail(GROUT_ERR_INVALID_ARG, "args is null");
+  grout_status st = check_dims(dims, 128);
+  if (st != GROUT_OK) return st;
+  if ((st = check_window(window, sinks)) != GROUT_OK) return st;
+  if (p->batch < 0 || p->max_q_len < 0)
+    return fail(GROUT_ERR_INVALID_ARG, "batch=%d max_q_len=%d", p->batch, p->max_q_len);
+  if (p->batch == 0 || p->max_q_len == 0) return GROUT_OK;
+  if (!p->k || !p->v) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
+  if (!aligned16(p->k) || !aligned16(p->v))
+    return fail(GROUT_ERR_INVALID_ARG, "k and v must be 16-byte aligned");
+  if (p->kv_row_stride <= 0 || p->kv_head_stride <= 0 || p->kv_batch_stride < 0 ||
+      p->kv_row_stride % 8 || p->kv_head_stride % 8 || p->kv_batch_stride % 8)
+    return fail(GROUT_ERR_INVALID_ARG, "bad kv strides row=%lld head=%lld batch=%lld",
+                (long long)p->kv_row_stride, (long long)p->kv_head_stride,
+                (long long)p->kv_batch_stride);
+  if (p->kv_rows <= 0 || p->kv_rows > kMaxKeys)
+    return fail(GROUT_ERR_INVALID_ARG, "kv_rows=%lld", (long long)p->kv_rows);
+  const bool batched = p->kv_batch_stride > 0 && p->batch > 1;
+  const uint64_t dk[4] = {128, (uint64_t)p->kv_rows, (uint64_t)dims->num_kv_heads,
+                          batched ? (uint64_t)p->batch : 1};
+  const uint64_t sk[3] = {(uint64_t)p->kv_row_stride, (uint64_t)p->kv_head_stride,
+                          batched ? (uint64_t)p->kv_batch_stride : 128};
+  PrefillWindowArgs a{};
+  a.kv_start = p->kv_start;
+  a.kv_rows = (int32_t)p->kv_rows;
+  a.kv_batched = batched ? 1 : 0;
+  a.max_keys = p->kv_rows;
+  return window_prefill(&a, p->q, p->out, p->q_row_stride, p->q_rows, p->k, p->v, dk, sk,
+                        p->cu_seqlens_q, p->position_start, p->batch, p->max_q_len, window, sinks,
+                        dims, stream);
+}
+
+grout_status grout_attn_prefill_paged_window(const grout_prefill_paged_args* p, int32_t window,
                                              int32_t sinks, const grout_attn_dims* dims,
                                              grout_stream_t stream) {
-  grout_status st = check_window(window, sinks);
+  if (!p) return fail(GROUT_ERR_INVALID_ARG, "args is null");
+  grout_status st = check_dims(dims, 128);
   if (st != GROUT_OK) return st;
-  return prefill_paged_common(args, window, sinks, dims, stream);
+  if ((st = check_window(window, sinks)) != GROUT_OK) return st;
+  if (p->batch < 0 || p->max_q_len < 0)
+    return fail(GROUT_ERR_INVALID_ARG, "batch=%d max_q_len=%d", p->batch, p->max_q_len);
+  if (p->batch == 0 || p->max_q_len == 0) return GROUT_OK;
+  st = check_pages(p->k_pages, p->v_pages, p->num_pages, p->page_size, p->page_table,
+                   p->table_stride, dims);
+  if (st != GROUT_OK) return st;
+  if (!p->position_start && !p->cu_seqlens_q && p->max_q_len > dims->max_seq)
+    return fail(GROUT_ERR_INVALID_ARG, "max_q_len=%d exceeds max_seq %d", p->max_q_len,
+                dims->max_seq);
+  const uint64_t dk[4] = {128, (uint64_t)p->page_size, (uint64_t)dims->num_kv_heads,
+                          (uint64_t)p->num_pages};
+  const uint64_t sk[3] = {128, (uint64_t)p->page_size * 128,
+                          (uint64_t)p->page_size * 128 * (uint64_t)dims->num_kv_heads};
+  PrefillWindowArgs a{};
+  a.page_table = p->page_table;
+  a.table_stride = p->table_stride;
+  a.page_size = p->page_size;
+  a.num_pages = p->num_pages;
+  a.max_keys = std::min<int64_t>(dims->max_seq, kMaxKeys);
+  return window_prefill(&a, p->q, p->out, p->q_row_stride, p->q_rows, p->k_pages, p->v_pages, dk, sk,
+                        p->cu_seqlens_q, p->position_start, p->batch, p->max_q_len, window, sinks,
+                        dims, stream);
 }
 
 grout_status grout_qkv_proj_norm_rope_kv_prefill(

@@ -216,10 +216,6 @@ struct PrefillArgs {
   // part ([item][tile][128 rows][130] f32) and a merge kernel finishes.
   int32_t nsplit;
   float* part;
-  // Sliding window (window > 0, nsplit 1): row p sees keys n <= p with
-  // n > p - window or n < sinks.
-  int32_t window;
-  int32_t sinks;
 };
 
 // tm_q: 3-D {128, hq, q_rows}, box {64, 1, 128}; tm_k / tm_v: 4-D
@@ -230,6 +226,40 @@ constexpr int kPrefillPartFloats = 128 * 130;
 cudaError_t launch_prefill(const PrefillArgs& a, const CUtensorMap& tm_q, const CUtensorMap& tm_k,
                            const CUtensorMap& tm_v, cudaStream_t s);
 cudaError_t prefill_set_attributes();
+
+// Sliding-window prefill: row p sees keys n <= p with n > p - window or
+// n < sinks.  Fields as PrefillArgs.
+struct PrefillWindowArgs {
+  __half* out;
+  int64_t q_row_stride;
+  int64_t q_rows;
+  const int32_t* cu_q;
+  const int32_t* pos0;
+  const int32_t* kv_start;
+  int32_t batch;
+  int32_t single_len;   // used when cu_q == null (batch 1)
+  int32_t hq;
+  int32_t hkv;
+  int32_t tok;          // tokens per query tile: 128 / (hq / hkv)
+  int32_t window;
+  int32_t sinks;
+  float scale_log2;
+  int* err;
+  int64_t max_keys;     // kv_start + positions stay below (else error 0x200, rows left)
+  int32_t kv_rows;      // contiguous: rows of the K/V maps
+  int32_t kv_batched;   // contiguous: the maps' last coordinate is the sequence
+  const int32_t* page_table;
+  int32_t table_stride;
+  int32_t page_size;
+  int32_t num_pages;
+};
+// tm_q: 3-D {128, hq, q_rows}, box {64, hq / hkv, tok}; tm_k / tm_v: 4-D
+// {128, kv_rows, hkv, B} or {128, page_size, hkv, num_pages}, box {64, 64, 1,
+// 1}; all 128B swizzle.  max_q_len sizes the grid only.
+cudaError_t launch_prefill_window(const PrefillWindowArgs& a, int32_t max_q_len, int num_sms,
+                                  const CUtensorMap& tm_q, const CUtensorMap& tm_k,
+                                  const CUtensorMap& tm_v, cudaStream_t s);
+cudaError_t prefill_window_set_attributes();
 
 // QKV projection + fused norm/RoPE/KV write (prefill): X [rows][hidden] f16
 // (row stride x_row_stride) times W [(hq+2hkv)*128][hidden] f16; maps are

@@ -21,8 +21,7 @@
 //               SM sub-partition with two busy softmax warps, so each MMA is
 //               kept to a few instructions: descriptors are precomputed low
 //               words advanced by constant adds.
-//   warp 14     idle, or, with a sliding window, clears the V rows no query sees
-//   warp 15     idle (completes the fourth warpgroup)
+//   warps 14-15 idle (they complete the fourth warpgroup)
 // Tensor memory (512 columns, f32): S0 [0,128) S1 [128,256) O0 [256,384)
 // O1 [384,512).  P_t (f16 pairs) overwrites the first 64 columns of S_t and
 // feeds the PV MMA straight from TMEM (A operand in TMEM, V from shared
@@ -37,6 +36,7 @@
 // the half-period offset between the two tiles survives item boundaries and
 // the output of one item overlaps the start of the next.
 #include "internal.h"
+#include "prefill_common.cuh"
 #include "ptx.cuh"
 
 namespace grout {
@@ -45,8 +45,6 @@ namespace {
 constexpr int kBM = 128;          // query rows per tile (= TMEM lanes)
 constexpr int kBN = 128;          // keys per KV tile
 constexpr int kSlots = 4;         // K/V ring slots
-constexpr int kTile = 128 * 128 * 2;  // bytes of one 128x128 f16 tile (two 64-col boxes)
-constexpr int kBox = kTile / 2;
 constexpr int kThreads = 512;     // 4 warpgroups, one persistent CTA per SM
 // Register split (setmaxnreg): launched at 128 per thread (512 x 128 =
 // 65536); the two softmax warpgroups rise to 192, the output and issue
@@ -77,98 +75,9 @@ constexpr int kBarOfull = kBarP + 2;          // + tile: O_t of the item final (
 constexpr int kBarOempty = kBarOfull + 2;     // + tile: O_t read out (4 output warps)
 constexpr int kBarL = kBarOempty + 2;         // + tile: row sums written (4 softmax warps)
 constexpr int kNumBars = kBarL + 2;
-constexpr int kBarVok = kNumBars;             // + slot, windows only: unseen V rows cleared (warp 14)
-constexpr int kNumBarsWin = kBarVok + kSlots;
-
-// ---- packed f32x2 arithmetic (sm_100a): two softmax elements per instruction
-__device__ __forceinline__ uint64_t f2pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2unpack(uint64_t r, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-// 2^x (x <= 0) for a pair, on the FMA/ALU pipes, used for a share of the
-// softmax exponentials so the MUFU unit is not the only path.  Range
-// reduction x = n + f, n = round(x) via the 1.5*2^23 magic constant,
-// f in [-1/2, 1/2]; 2^f by a degree-3 polynomial fitted for minimum relative
-// error (max 7.6e-5, below the f16 rounding P gets next); 2^n added into the
-// exponent field.  Inputs below -125 clamp to ~2^-125 (P rounds to 0 in
-// f16); the clamp keeps n + exponent(p) >= 1, so the sum never reaches the
-// sign bit (p can be slightly below 1 when f < 0).
-__device__ __forceinline__ void ex2_poly2(uint64_t x2, float& r0, float& r1) {
-  float x0, x1;
-  f2unpack(x2, x0, x1);
-  x2 = f2pack(fmaxf(x0, -125.0f), fmaxf(x1, -125.0f));
-  const uint64_t t2 = fadd2(x2, f2pack(12582912.0f, 12582912.0f));
-  const uint64_t n2 = fadd2(t2, f2pack(-12582912.0f, -12582912.0f));
-  const uint64_t f2 = ffma2(n2, f2pack(-1.0f, -1.0f), x2);
-  uint64_t p2 = ffma2(f2pack(0.05517090484f, 0.05517090484f), f2,
-                      f2pack(0.24260953069f, 0.24260953069f));
-  p2 = ffma2(p2, f2, f2pack(0.69326096773f, 0.69326096773f));
-  p2 = ffma2(p2, f2, f2pack(0.99992817640f, 0.99992817640f));
-  float p0, p1, t0, t1;
-  f2unpack(p2, p0, p1);
-  f2unpack(t2, t0, t1);
-  r0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  r1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
-}
-
-// Element pairs (of the 16 per 32-column chunk) whose exponentials run on
-// ex2_poly2: one in four, so MUFU carries 3/4 of the exponentials.
-__device__ __forceinline__ constexpr bool poly_pair(int i) { return (i & 3) == 3; }
-
-// Online-softmax rescaling threshold (log2 units): the reference max a row
-// exponentiates against moves only when the row max grows by more than this,
-// so P stays <= 2^8 and O is rescaled rarely.
-constexpr float kRescaleThreshold = 8.0f;
 
 __device__ __forceinline__ int ring_slot(int i) { return i % kSlots; }
 __device__ __forceinline__ uint32_t ring_parity(int i) { return (uint32_t)((i / kSlots) & 1); }
-
-// Low/high words of the SW128 shared-memory descriptor (matches
-// smem_desc_sw128): low = start address >> 4 | LBO >> 4 << 16;
-// high = SBO (1024) >> 4 | version 1 << 14 | layout SW128 (2) << 29.
-constexpr uint32_t kDescLboK = (16u >> 4) << 16;
-constexpr uint32_t kDescLboV = ((uint32_t)kBox >> 4) << 16;
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-static_assert(((uint64_t)kDescHi << 32) == ((uint64_t)(1024u >> 4) << 32 | 1ull << 46 | 2ull << 61),
-              "descriptor high word");
-__device__ __forceinline__ void mma_ss_lo(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc,
-                                          uint32_t acc) {
-  asm volatile(
-      "{ .reg .pred p; .reg .b64 da, db; setp.ne.u32 p, %4, 0;"
-      " mov.b64 da, {%1, %5}; mov.b64 db, {%2, %5};"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p; }" ::"r"(d),
-      "r"(alo), "r"(blo), "r"(idesc), "r"(acc), "n"(kDescHi)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t blo, uint32_t idesc,
-                                          uint32_t acc) {
-  asm volatile(
-      "{ .reg .pred p; .reg .b64 db; setp.ne.u32 p, %4, 0;"
-      " mov.b64 db, {%2, %5};"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p; }" ::"r"(d),
-      "r"(a_tmem), "r"(blo), "r"(idesc), "r"(acc), "n"(kDescHi)
-      : "memory");
-}
 
 // One work item = two 128-row query tiles of one (sequence, head); items are
 // numbered longest-first (query-tile pair descending, then head, then
@@ -181,17 +90,8 @@ struct Item {
   int h, b, q0, S, P, ks, q_start, n_kv, n_kv0;
   int lo;   // first KV tile of this item (split-K: its range starts here)
   int nch;  // split-K: number of non-empty splits of this (pair, head, sequence)
-  // window: first key after the sinks that some row of the item sees, one past
-  // the last one, and the item's KV tiles: 0 .. sink_tiles-1, then from
-  // sink_tiles + skip on
-  int wlo, vis_end, sink_tiles, skip;
 };
-template <bool kWin>
-__device__ __forceinline__ int kv_tile(const Item& it, int j) {
-  if (kWin) return j < it.sink_tiles ? j : j + it.skip;
-  return it.lo + j;
-}
-template <bool kSplit, bool kWin>
+template <bool kSplit>
 __device__ __forceinline__ bool decode_item(const PrefillArgs& a, int idx, int n_pairs, Item& it) {
   int split = 0;
   if (kSplit) {
@@ -220,15 +120,6 @@ __device__ __forceinline__ bool decode_item(const PrefillArgs& a, int idx, int n
   it.n_kv0 = (it.P + min(it.q0 + kBM, it.S) + kBN - 1) / kBN;
   it.lo = 0;
   it.nch = 1;
-  if (kWin) {
-    it.vis_end = it.P + rows_hi;
-    it.wlo = max(0, it.P + it.q0 - a.window + 1);
-    const int first = it.wlo / kBN;
-    it.sink_tiles = min(first, (int)(((int64_t)a.sinks + kBN - 1) / kBN));
-    it.skip = first - it.sink_tiles;
-    it.n_kv -= it.skip;
-    it.n_kv0 -= it.skip;
-  }
   if (kSplit) {
     // Split [0, n_kv0) into chunks of tps tiles; the last chunk also takes
     // tile 1's extra tile, so both tiles have work in every chunk.
@@ -298,18 +189,9 @@ __device__ __forceinline__ int build_schedule(const PrefillArgs& a, int n_pairs,
 }
 
 // kPaged: K/V from a page pool; kSplit: split-K partial output; kCompact: a
-// ragged batch scheduled over its non-empty items; kWin: sliding window with
-// sinks.  The plain instantiation carries none of them.
-//
-// kWin: row p sees key n if n <= p and (n > p - window or n < sinks).  An item
-// streams only the KV tiles that hold a key one of its rows sees (the sinks'
-// tiles, then from the first row's window on).  Rows that no row of the item
-// sees may hold anything (freed pages, unwritten rows, NaN): K needs no care,
-// their scores are replaced, but 0 * NaN in the PV product is NaN, so 64-key
-// blocks without a seen key are not read at all (paged: an out-of-range page
-// coordinate, which TMA fills with zeros) and warp 14 clears the unseen rows
-// of every V tile in shared memory before the MMA warp may use it.
-template <bool kPaged, bool kSplit, bool kCompact, bool kWin>
+// ragged batch scheduled over its non-empty items.  The plain instantiation
+// carries none of them.
+template <bool kPaged, bool kSplit, bool kCompact>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const PrefillArgs a) {
@@ -317,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + (kWin ? kNumBarsWin : kNumBars));
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   float* lbuf = reinterpret_cast<float*>(smem + kOffL);
 
@@ -344,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < (kWin ? kNumBarsWin : kNumBars); ++i) {
+    for (int i = 0; i < kNumBars; ++i) {
       uint32_t cnt = 1;
       if ((i >= kBarP && i < kBarP + 2) || (i >= kBarOempty && i < kBarOempty + 2) ||
           (i >= kBarL && i < kBarL + 2))
@@ -376,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int r = 0, idx; ok && (idx = item_of(r)) < n_items; ++r) {
         Item it;
-        if (!decode_item<kSplit, kWin>(a, idx, n_pairs, it)) continue;
+        if (!decode_item<kSplit>(a, idx, n_pairs, it)) continue;
         const int kh = it.h / (a.hq / a.hkv);
         const int kvb = a.kv_batched ? it.b : 0;
         // Q_0, K_0, Q_1, then the rest: each tile's query buffer is refilled
@@ -410,29 +292,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(full, kTile);
           const CUtensorMap* map = (i & 1) ? &tm_v : &tm_k;
           const uint32_t dst = smem_base + kOffKV + slot * kTile;
-          const int tile = kv_tile<kWin>(it, i >> 1);
-          const int row = it.ks + tile * kBN;
-          if (kPaged && kWin) {
-            // two 64-key halves as below; one that no row of the item sees,
-            // or whose page is outside the pool, is filled with zeros
-            const int32_t* trow = a.page_table + (int64_t)it.b * a.table_stride;
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const int key = tile * kBN + hh * 64;
-              int page = a.num_pages, r = 0;
-              if (key < it.vis_end && (key + 64 > it.wlo || key < a.sinks)) {
-                const int pg = key / a.page_size;
-                if (pg < a.table_stride) page = __ldg(trow + pg);
-                r = key - pg * a.page_size;
-                if (page < 0 || page >= a.num_pages) {
-                  if (a.err) atomicCAS(a.err, 0, DEV_ERR_PAGE);
-                  page = a.num_pages;
-                }
-              }
-              tma_load_4d(dst + hh * (kBox / 2), map, full, 0, r, kh, page);
-              tma_load_4d(dst + kBox + hh * (kBox / 2), map, full, 64, r, kh, page);
-            }
-          } else if (kPaged) {
+          const int row = it.ks + (it.lo + (i >> 1)) * kBN;
+          if (kPaged) {
             // two 64-key halves, each inside one page (page_size % 64 == 0);
             // a half past the sequence's last key reads page 0 (masked) and
             // leaves the table untouched
@@ -440,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int kv_len = it.P + it.S;
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-              const int key = tile * kBN + hh * 64;
+              const int key = (it.lo + (i >> 1)) * kBN + hh * 64;
               int page = 0, r = 0;
               if (key < kv_len) {
                 const int pg = key / a.page_size;
@@ -495,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // half-period offset across item boundaries.
     auto next_valid = [&](int& rr, Item& itm) -> bool {
       for (int idx; (idx = item_of(rr)) < n_items; ++rr)
-        if (decode_item<kSplit, kWin>(a, idx, n_pairs, itm)) return true;
+        if (decode_item<kSplit>(a, idx, n_pairs, itm)) return true;
       return false;
     };
     int ring = 0, nq = 0, pc0 = 0, pc1 = 0;
@@ -531,8 +392,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int iv = ring + 2 * j + 1, ik = ring + 2 * j + 2;
         const bool next = j + 1 < n_kv;
         ok = mbar_wait(smem_u32(&bars[kBarFull + ring_slot(iv)]), ring_parity(iv), a.err, 22, abort_flag);
-        if (kWin && ok)
-          ok = mbar_wait(smem_u32(&bars[kBarVok + ring_slot(iv)]), ring_parity(iv), a.err, 29, abort_flag);
         // K(j+1) only needs the slot K(j-1) released, so it is awaited
         // here, before P0(j), keeping the wait off the PV0 -> QK0 path.
         if (ok && next)
@@ -597,36 +456,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       rr = rn;
       has = hn;
     }
-  } else if (kWin && warp == 14) {
-    // ---------------------------------------- clear the unseen rows of V tiles
-    // A V tile is two boxes of 128 rows x 128 bytes; the swizzle moves bytes
-    // within a row only, so whole rows are cleared in place.
-    int ring = 0;
-    bool ok = true;
-    for (int r = 0, idx; ok && (idx = item_of(r)) < n_items; ++r) {
-      Item it;
-      if (!decode_item<kSplit, kWin>(a, idx, n_pairs, it)) continue;
-      for (int j = 0; j < it.n_kv; ++j, ring += 2) {
-        const int iv = ring + 1;
-        ok = mbar_wait(smem_u32(&bars[kBarFull + ring_slot(iv)]), ring_parity(iv), a.err, 50, abort_flag);
-        if (!ok) break;
-        const int base = kv_tile<kWin>(it, j) * kBN;
-        const int lo0 = max(0, a.sinks - base), hi0 = min(kBN, it.wlo - base);  // before the window
-        const int lo1 = max(0, it.vis_end - base);                              // after the last key
-        if (lo0 < hi0 || lo1 < kBN) {
-          uint8_t* v = smem + kOffKV + ring_slot(iv) * kTile;
-          for (int row = lane >> 3; row < kBN; row += 4) {
-            if ((row >= lo0 && row < hi0) || row >= lo1) {
-              *reinterpret_cast<uint4*>(v + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-              *reinterpret_cast<uint4*>(v + kBox + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bars[kBarVok + ring_slot(iv)]));
-      }
-    }
   } else if (warp < 12) {
     // ------------------------------------------------------------ output
     // Warp 8 + q reads TMEM lanes 32q.. (query rows) of O_t once the MMA
@@ -639,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int r = 0, idx; ok && (idx = item_of(r)) < n_items; ++r) {
       Item it;
-      if (!decode_item<kSplit, kWin>(a, idx, n_pairs, it)) continue;
+      if (!decode_item<kSplit>(a, idx, n_pairs, it)) continue;
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
         ok = mbar_wait(smem_u32(&bars[kBarOfull + t]), nq & 1, a.err, 40 + t, abort_flag);
@@ -704,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int r = 0, idx; ok && (idx = item_of(r)) < n_items; ++r) {
       Item it;
-      if (!decode_item<kSplit, kWin>(a, idx, n_pairs, it)) continue;
+      if (!decode_item<kSplit>(a, idx, n_pairs, it)) continue;
       const int row_q = it.q0 + t * kBM + row;
       const int kv_len = it.P + it.S;
       const int key_lim = min(it.P + row_q, kv_len - 1);  // last visible key
@@ -724,21 +553,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(r[c][i]);
-        const int base = kv_tile<kWin>(it, j) * kBN;
-        const int lim = key_lim - base;
+        const int lim = key_lim - (it.lo + j) * kBN;
         if (lim < kBN - 1) {
 #pragma unroll
           for (int c = 0; c < 128; ++c)
             if (c > lim) s[c] = -INFINITY;
-        }
-        if (kWin) {
-          const int low = it.P + row_q - a.window + 1 - base;  // first column of the window
-          const int sk = a.sinks - base;
-          if (low > 0 && sk < min(low, kBN)) {
-#pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (c < low && c >= sk) s[c] = -INFINITY;
-          }
         }
         float mx0 = fmaxf(s[0], s[1]), mx1 = fmaxf(s[2], s[3]);
         float mx2 = fmaxf(s[4], s[5]), mx3 = fmaxf(s[6], s[7]);
@@ -849,7 +668,7 @@ __global__ void __launch_bounds__(1024) prefill_merge_kernel(const PrefillArgs a
     const int n_pairs = (a.max_q_len + 2 * kBM - 1) / (2 * kBM);
     Item it;
     int nch = 0;
-    if (decode_item<true, false>(a, base * a.nsplit, n_pairs, it)) {
+    if (decode_item<true>(a, base * a.nsplit, n_pairs, it)) {
       nch = it.nch;
       s_rows = min(kBM, it.S - (it.q0 + t * kBM));
       s_out_row = it.q_start + it.q0 + t * kBM;
@@ -906,12 +725,10 @@ __global__ void __launch_bounds__(1024) prefill_merge_kernel(const PrefillArgs a
 }  // namespace
 
 cudaError_t prefill_set_attributes() {
-  for (auto k : {prefill_kernel<false, false, false, false>, prefill_kernel<true, false, false, false>,
-                 prefill_kernel<false, true, false, false>, prefill_kernel<true, true, false, false>,
-                 prefill_kernel<false, false, true, false>, prefill_kernel<true, false, true, false>,
-                 prefill_kernel<false, true, true, false>, prefill_kernel<true, true, true, false>,
-                 prefill_kernel<false, false, false, true>, prefill_kernel<true, false, false, true>,
-                 prefill_kernel<false, false, true, true>, prefill_kernel<true, false, true, true>}) {
+  for (auto k : {prefill_kernel<false, false, false>, prefill_kernel<true, false, false>,
+                 prefill_kernel<false, true, false>, prefill_kernel<true, true, false>,
+                 prefill_kernel<false, false, true>, prefill_kernel<true, false, true>,
+                 prefill_kernel<false, true, true>, prefill_kernel<true, true, true>}) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return e;
   }
@@ -942,24 +759,18 @@ cudaError_t launch_prefill(const PrefillArgs& a, const CUtensorMap& tm_q, const 
   const bool compact = a.cu_q != nullptr && a.batch > 1 && a.batch <= kSchedMaxBatch &&
                        n_pairs <= kSchedMaxPairs && (n_items + grid - 1) / grid <= kSchedMaxRounds &&
                        a.hq * a.batch < 2 * grid;
-  if (a.window > 0 && split) return cudaErrorInvalidValue;
-#define GROUT_PREFILL_LAUNCH(P, SP, C, W) \
-  prefill_kernel<P, SP, C, W><<<grid, kThreads, kSmemBytes, s>>>(tm_q, tm_k, tm_v, a)
-  if (a.window > 0) {
-    if (paged && compact) GROUT_PREFILL_LAUNCH(true, false, true, true);
-    else if (paged) GROUT_PREFILL_LAUNCH(true, false, false, true);
-    else if (compact) GROUT_PREFILL_LAUNCH(false, false, true, true);
-    else GROUT_PREFILL_LAUNCH(false, false, false, true);
-  } else if (compact) {
-    if (paged && split) GROUT_PREFILL_LAUNCH(true, true, true, false);
-    else if (paged) GROUT_PREFILL_LAUNCH(true, false, true, false);
-    else if (split) GROUT_PREFILL_LAUNCH(false, true, true, false);
-    else GROUT_PREFILL_LAUNCH(false, false, true, false);
+#define GROUT_PREFILL_LAUNCH(P, SP, C) \
+  prefill_kernel<P, SP, C><<<grid, kThreads, kSmemBytes, s>>>(tm_q, tm_k, tm_v, a)
+  if (compact) {
+    if (paged && split) GROUT_PREFILL_LAUNCH(true, true, true);
+    else if (paged) GROUT_PREFILL_LAUNCH(true, false, true);
+    else if (split) GROUT_PREFILL_LAUNCH(false, true, true);
+    else GROUT_PREFILL_LAUNCH(false, false, true);
   } else {
-    if (paged && split) GROUT_PREFILL_LAUNCH(true, true, false, false);
-    else if (paged) GROUT_PREFILL_LAUNCH(true, false, false, false);
-    else if (split) GROUT_PREFILL_LAUNCH(false, true, false, false);
-    else GROUT_PREFILL_LAUNCH(false, false, false, false);
+    if (paged && split) GROUT_PREFILL_LAUNCH(true, true, false);
+    else if (paged) GROUT_PREFILL_LAUNCH(true, false, false);
+    else if (split) GROUT_PREFILL_LAUNCH(false, true, false);
+    else GROUT_PREFILL_LAUNCH(false, false, false);
   }
 #undef GROUT_PREFILL_LAUNCH
   cudaError_t e = cudaGetLastError();

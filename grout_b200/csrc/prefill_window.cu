@@ -1,0 +1,635 @@
+// Sliding-window causal GQA prefill with sinks on the 5th-generation tensor
+// cores: row p of a sequence sees key n if n <= p and (n > p - window or
+// n < sinks).  O = softmax(scale Q K^T + mask) V, f16 in, f32 accumulate, P
+// rounded to f16 before the PV product, f16 out.  No counterpart in the
+// reference (its prefill attends to every earlier key, src/kernels.rs:
+// 2570-2725).
+//
+// The pipeline is prefill.cu's (persistent CTAs, 512 threads: two softmax
+// warpgroups, one output warpgroup, a TMA warp, an MMA warp; S and P in TMEM,
+// P feeds the PV MMA from there; one-pass softmax with a lazily moved
+// reference maximum).  What a window changes:
+//
+// Rows.  A 128-row query tile holds floor(128 / G) tokens with all G query
+// heads of one KV head (row = token * G + head).  All of a tile's rows so
+// need nearly the same keys: a tile of 128 tokens of one head touches
+// window + 127 keys, one of 16 tokens x 8 heads window + 15, and a chunk of
+// a few tokens fills one tile with every head instead of one tile per head.
+// An item is two such tiles of one (sequence, KV head), or one, when
+// the sequence ends in the first.
+//
+// Keys.  An item streams the 64-key blocks that hold a key one of its rows
+// sees (the sinks' blocks, then from the first row's window on), two blocks
+// to a 128-key tile whether they are neighbours or not.  TMA loads
+// each block by itself (64-row boxes), from its page or its cache row.
+//
+// Unseen rows.  Rows that no row of the item sees may hold anything (freed
+// pages, unwritten rows, NaN).  Their scores are replaced, but 0 * NaN in the
+// PV product is a NaN, so blocks without a seen key are not read (TMA fills
+// an out-of-range coordinate with zeros), and warp 14 clears the unseen
+// rows of the at most three partial blocks of an item in shared memory before
+// the MMA warp may use their V tile.
+#include "internal.h"
+#include "prefill_common.cuh"
+#include "ptx.cuh"
+
+namespace grout {
+namespace {
+
+constexpr int kBM = 128;       // query rows per tile (= TMEM lanes)
+constexpr int kBlk = 64;       // keys per block, two blocks per KV tile
+constexpr int kSlots = 4;      // K/V ring slots (even ring entries K, odd ones V)
+constexpr int kThreads = 512;  // 4 warpgroups, one persistent CTA per SM
+// Register split (setmaxnreg): launched at 128 per thread (512 x 128 =
+// 65536); 2 x 128 x 192 + 2 x 128 x 64 = 65536.
+constexpr int kRegsOther = 64;
+constexpr int kRegsSoftmax = 192;
+constexpr int kOffQ = 0;          // 2 query tiles
+constexpr int kOffKV = 2 * kTile; // ring
+constexpr int kOffBar = kOffKV + kSlots * kTile;
+constexpr int kOffL = kOffBar + 512;  // row sums [item parity][tile][row]
+constexpr int kSmemBytes = kOffL + 2 * 2 * 128 * 4 + 1024;
+
+// barrier indices (phases run on across the work items of a CTA; those of
+// tile 1 skip the items that have one tile)
+constexpr int kBarQ = 0;                      // + tile: Q_t landed (TMA)
+constexpr int kBarQfree = 2;                  // + tile: last QK_t of the item done (commit)
+constexpr int kBarFull = 4;                   // + slot
+constexpr int kBarEmpty = kBarFull + kSlots;  // + slot
+constexpr int kBarS = kBarEmpty + kSlots;     // + tile (commit)
+constexpr int kBarP = kBarS + 2;              // + tile (4 softmax warps)
+constexpr int kBarOfull = kBarP + 2;          // + tile: O_t of the item final (commit)
+constexpr int kBarOempty = kBarOfull + 2;     // + tile: O_t read out (4 output warps)
+constexpr int kBarL = kBarOempty + 2;         // + tile: row sums written (4 softmax warps)
+constexpr int kBarClr = kBarL + 2;            // + V slot (ring slot / 2): unseen rows cleared (warp 14)
+constexpr int kBarDrain = kBarClr + 2;        // MMAs in flight when a wait gave up
+constexpr int kNumBars = kBarDrain + 1;
+
+__device__ __forceinline__ int ring_slot(int i) { return i % kSlots; }
+__device__ __forceinline__ uint32_t ring_parity(int i) { return (uint32_t)((i / kSlots) & 1); }
+
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+struct Item {
+  int b, kh, q0, S, P, ks, q_start;
+  int n0, n_kv;     // KV tiles of query tile 0, of the item (tile 1 takes all)
+  bool two;         // the item has a second query tile
+  int nblk, sink_blk, skip;  // 64-key blocks; entry i is block i or, past the sinks, i + skip
+  int wlo, vis_end; // keys some row sees: n < sinks, and wlo <= n < vis_end
+  // first key of block entry i
+  __device__ __forceinline__ int key0(int i) const { return (i < sink_blk ? i : i + skip) * kBlk; }
+  // whether block entry i holds a key that no row of the item sees
+  __device__ __forceinline__ bool partial(int i, int sinks) const {
+    const int k = key0(i);
+    return k + kBlk > vis_end || (k < wlo && k + kBlk > sinks);
+  }
+};
+
+// Walks this CTA's items: entry r * grid + c of the list (r * grid + grid - 1
+// - c in odd rounds, so that the longer items at the front even out), which
+// numbers, sequence by sequence, token blocks in descending order, KV heads
+// fastest.  A sequence whose lengths or positions fit neither the query rows
+// nor the cache has no items (device error 0x200).
+struct Walk {
+  int r = 0, b = -1;
+  int64_t base = 0;
+  int cnt = 0, S = 0, P = 0, ks = 0, q_start = 0;
+
+  __device__ __forceinline__ void enter(const PrefillWindowArgs& a) {
+    if (a.cu_q) {
+      q_start = a.cu_q[b];
+      S = a.cu_q[b + 1] - q_start;
+    } else {
+      q_start = 0;
+      S = a.single_len;
+    }
+    P = a.pos0 ? a.pos0[b] : 0;
+    ks = a.kv_start ? a.kv_start[b] : 0;
+    cnt = 0;
+    if (S <= 0) return;
+    if (q_start < 0 || (int64_t)q_start + S > a.q_rows || P < 0 || ks < 0 ||
+        (int64_t)ks + P + S > a.max_keys) {
+      if (a.err) atomicCAS(a.err, 0, DEV_ERR_POSITION);
+      return;
+    }
+    cnt = (S + 2 * a.tok - 1) / (2 * a.tok) * a.hkv;
+  }
+
+  __device__ __forceinline__ bool next(const PrefillWindowArgs& a, Item& it) {
+    const int64_t G = gridDim.x, c = blockIdx.x;
+    const int64_t k = r * G + ((r & 1) ? G - 1 - c : c);
+    ++r;
+    while (k >= base + cnt) {
+      if (b >= a.batch - 1) return false;
+      base += cnt;
+      ++b;
+      enter(a);
+    }
+    const int local = (int)(k - base);
+    const int pair = cnt / a.hkv - 1 - local / a.hkv;
+    it.b = b;
+    it.kh = local % a.hkv;
+    it.S = S;
+    it.P = P;
+    it.ks = ks;
+    it.q_start = q_start;
+    it.q0 = pair * 2 * a.tok;
+    it.two = S > it.q0 + a.tok;
+    const int end0 = P + min(it.q0 + a.tok, S);
+    it.vis_end = P + min(it.q0 + 2 * a.tok, S);
+    it.wlo = max(0, P + it.q0 - a.window + 1);
+    const int first = it.wlo / kBlk;
+    it.sink_blk = min(first, (int)(((int64_t)a.sinks + kBlk - 1) / kBlk));
+    it.skip = first - it.sink_blk;
+    it.nblk = (it.vis_end + kBlk - 1) / kBlk - it.skip;
+    it.n_kv = (it.nblk + 1) / 2;
+    it.n0 = ((end0 + kBlk - 1) / kBlk - it.skip + 1) / 2;
+    return true;
+  }
+};
+
+template <bool kPaged>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefill_window_kernel(const __grid_constant__ CUtensorMap tm_q,
+                          const __grid_constant__ CUtensorMap tm_k,
+                          const __grid_constant__ CUtensorMap tm_v, const PrefillWindowArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float* lbuf = reinterpret_cast<float*>(smem + kOffL);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  auto bar = [&](int i) -> uint32_t { return smem_u32(&bars[i]); };
+  auto wait = [&](int i, uint32_t parity, int site) -> bool {
+    return mbar_wait(bar(i), parity & 1u, a.err, site, abort_flag);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kNumBars; ++i) {
+      // P, Oempty, L: one arrival per warp of a warpgroup
+      const bool four = (i >= kBarP && i < kBarP + 2) || (i >= kBarOempty && i < kBarOempty + 2) ||
+                        (i >= kBarL && i < kBarL + 2);
+      mbar_init(bar(i), four ? 4 : 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 13) {
+    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  const uint32_t smem_base = smem_u32(smem);
+
+  Walk walk;
+  Item it;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == 12) {
+      // ---------------------------------------------------------- producer
+      if (lane == 0) {
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        int ring = 0;
+        int nq[2] = {0, 0};
+        bool ok = true;
+        while (ok && walk.next(a, it)) {
+          // Q_0, K_0, Q_1, then the rest: each tile's query buffer is refilled
+          // as soon as that tile's last QK of the previous item has run.
+          auto load_q = [&](int t) -> bool {
+            if (nq[t] > 0 && !wait(kBarQfree + t, nq[t] - 1, 11 + t)) return false;
+            ++nq[t];
+            mbar_arrive_expect_tx(bar(kBarQ + t), a.tok * (a.hq / a.hkv) * 256);
+            const uint32_t dst = smem_base + kOffQ + t * kTile;
+            const int row = it.q_start + it.q0 + t * a.tok, head = it.kh * (a.hq / a.hkv);
+            tma_load_3d(dst, &tm_q, bar(kBarQ + t), 0, head, row);
+            tma_load_3d(dst + kBox, &tm_q, bar(kBarQ + t), 64, head, row);
+            return true;
+          };
+          if (!load_q(0)) break;
+          for (int i = 0; i < 2 * it.n_kv; ++i) {
+            if (i == 1 && it.two && !load_q(1)) {
+              ok = false;
+              break;
+            }
+            const int slot = ring_slot(ring);
+            if (ring >= kSlots && !wait(kBarEmpty + slot, ring_parity(ring) ^ 1u, 10)) {
+              ok = false;
+              break;
+            }
+            int row[2], outer[2];
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              const int e = (i >> 1) * 2 + hh;
+              // past the last block: an out-of-range coordinate, filled with zeros
+              row[hh] = kPaged ? 0 : a.kv_rows;
+              outer[hh] = kPaged ? a.num_pages : (a.kv_batched ? it.b : 0);
+              if (e < it.nblk) {
+                const int key = it.key0(e);
+                if (kPaged) {
+                  const int pg = key / a.page_size;
+                  const int page = __ldg(a.page_table + (int64_t)it.b * a.table_stride + pg);
+                  row[hh] = key - pg * a.page_size;
+                  if (page >= 0 && page < a.num_pages) outer[hh] = page;
+                  else if (a.err) atomicCAS(a.err, 0, DEV_ERR_PAGE);
+                } else {
+                  row[hh] = it.ks + key;
+                }
+              }
+            }
+            const uint32_t full = bar(kBarFull + slot);
+            mbar_arrive_expect_tx(full, kTile);
+            const CUtensorMap* map = (i & 1) ? &tm_v : &tm_k;
+            const uint32_t dst = smem_base + kOffKV + slot * kTile;
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              tma_load_4d(dst + hh * (kBox / 2), map, full, 0, row[hh], it.kh, outer[hh]);
+              tma_load_4d(dst + kBox + hh * (kBox / 2), map, full, 64, row[hh], it.kh, outer[hh]);
+            }
+            ++ring;
+          }
+        }
+        // a wait gave up: let the loads in flight land before the CTA leaves
+        if (*abort_flag) {
+          for (int i = max(0, ring - kSlots); i < ring; ++i)
+            for (int n = 0; n < (1 << 20); ++n)
+              if (mbar_try_wait(bar(kBarFull + ring_slot(i)), ring_parity(i))) break;
+          for (int t = 0; t < 2; ++t)
+            for (int n = 0; nq[t] > 0 && n < (1 << 20); ++n)
+              if (mbar_try_wait(bar(kBarQ + t), (nq[t] - 1) & 1)) break;
+        }
+      }
+    } else if (warp == 13) {
+      // ------------------------------------------------------------ MMA issue
+      // The whole warp runs the issue loop (warp-uniform descriptors); one
+      // elected lane issues every MMA and commit.  Per KV tile j of an item:
+      // PV0(j), QK0(j+1), PV1(j), QK1(j+1); the first QKs of the next item
+      // follow the last PVs of this one, and its first PV_t waits until the
+      // output warps have read O_t of the item before out of TMEM.
+      const bool leader = elect_one();
+      constexpr uint32_t idesc_qk = idesc_f16_f32(kBM, 128, 0, 0);
+      constexpr uint32_t idesc_pv = idesc_f16_f32(kBM, 128, 0, 1);
+      const uint32_t base16 = smem_base >> 4;
+      auto commit = [&](int i) {
+        if (leader) tc_commit(bar(i));
+      };
+      auto qk = [&](int t, int slot) {
+        const uint32_t qlo = base16 + (kOffQ + t * kTile) / 16 + kDescLboK;
+        const uint32_t klo = base16 + (kOffKV + slot * kTile) / 16 + kDescLboK;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) / 16;
+          if (leader) mma_ss_lo(tmem + t * 128, qlo + off, klo + off, idesc_qk, kk > 0 ? 1u : 0u);
+        }
+      };
+      auto pv = [&](int t, int slot, bool acc) {
+        const uint32_t vlo = base16 + (kOffKV + slot * kTile) / 16 + kDescLboV;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          if (leader)
+            mma_ts_lo(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, vlo + kk * (2048 / 16), idesc_pv,
+                      (acc || kk > 0) ? 1u : 0u);
+        }
+      };
+      int nst[2] = {0, 0};  // items started per tile (QK_t(0) issued)
+      int npv[2] = {0, 0};  // items per tile whose first PV_t has been issued
+      int pc[2] = {0, 0};   // P_t tiles taken
+      auto start = [&](int t, const Item& x, int iring) -> bool {
+        if (!wait(kBarQ + t, nst[t], 20 + t) || !wait(kBarFull + ring_slot(iring), ring_parity(iring), 22))
+          return false;
+        ++nst[t];
+        tc_fence_after();
+        qk(t, ring_slot(iring));
+        commit(kBarS + t);
+        if (t == 1 || !x.two) commit(kBarEmpty + ring_slot(iring));
+        if ((t == 0 ? x.n0 : x.n_kv) == 1) commit(kBarQfree + t);
+        return true;
+      };
+      auto take_p = [&](int t, bool first) -> bool {
+        if (!wait(kBarP + t, pc[t], 24 + t)) return false;
+        ++pc[t];
+        if (first) {
+          if (npv[t] > 0 && !wait(kBarOempty + t, npv[t] - 1, 26 + t)) return false;
+          ++npv[t];
+        }
+        tc_fence_after();
+        return true;
+      };
+      int ring = 0;
+      Item cur = {}, nx = {};
+      bool has = walk.next(a, cur);
+      bool ok = !has || (start(0, cur, ring) && (!cur.two || start(1, cur, ring)));
+      while (has && ok) {
+        const bool hn = walk.next(a, nx);
+        const int n_kv = cur.n_kv, n0 = cur.n0;
+        const int nring = ring + 2 * n_kv;  // K_0 of the next item
+        for (int j = 0; j < n_kv; ++j) {
+          const int iv = ring + 2 * j + 1, ik = ring + 2 * j + 2;
+          const bool next = j + 1 < n_kv;
+          ok = wait(kBarFull + ring_slot(iv), ring_parity(iv), 23) &&
+               wait(kBarClr + (ring_slot(iv) >> 1), ring_parity(iv), 29);
+          // K(j+1) only needs the slot K(j-1) released, so it is awaited
+          // here, before P0(j), keeping the wait off the PV0 -> QK0 path.
+          if (ok && next) ok = wait(kBarFull + ring_slot(ik), ring_parity(ik), 22);
+          if (!ok) break;
+          if (j < n0) {
+            if (!(ok = take_p(0, j == 0))) break;
+            pv(0, ring_slot(iv), j > 0);
+            if (!cur.two) commit(kBarEmpty + ring_slot(iv));
+            if (j == n0 - 1) commit(kBarOfull + 0);
+          }
+          if (j + 1 < n0) {
+            qk(0, ring_slot(ik));
+            commit(kBarS + 0);
+            if (!cur.two) commit(kBarEmpty + ring_slot(ik));
+            if (j + 1 == n0 - 1) commit(kBarQfree + 0);
+          } else if (j + 1 == n0 && hn) {
+            // tile 0 is done with this item: start the next one
+            if (!(ok = start(0, nx, nring))) break;
+          }
+          if (cur.two) {
+            if (!(ok = take_p(1, j == 0))) break;
+            pv(1, ring_slot(iv), j > 0);
+            commit(kBarEmpty + ring_slot(iv));
+            if (!next) commit(kBarOfull + 1);
+            if (next) {
+              qk(1, ring_slot(ik));
+              commit(kBarS + 1);
+              commit(kBarEmpty + ring_slot(ik));
+              if (j + 1 == n_kv - 1) commit(kBarQfree + 1);
+            }
+          }
+          if (!next && hn && nx.two && !(ok = start(1, nx, nring))) break;
+        }
+        if (!ok) break;
+        ring = nring;
+        cur = nx;
+        has = hn;
+      }
+      if (!ok) {  // let the MMAs in flight finish before their memory is given back
+        commit(kBarDrain);
+        for (int n = 0; n < (1 << 20); ++n)
+          if (mbar_try_wait(bar(kBarDrain), 0)) break;
+      }
+    } else if (warp == 14) {
+      // ------------------------------------- clear the unseen rows of V tiles
+      // A V tile is two boxes of 128 rows x 128 bytes; the swizzle moves bytes
+      // within a row only, so whole rows are cleared in place.
+      int ring = 0;
+      bool ok = true;
+      while (ok && walk.next(a, it)) {
+        for (int j = 0; j < it.n_kv; ++j, ring += 2) {
+          const int iv = ring + 1;
+          ok = wait(kBarFull + ring_slot(iv), ring_parity(iv), 50);
+          if (!ok) break;
+          bool wrote = false;
+          for (int e = 2 * j; e < min(2 * j + 2, it.nblk); ++e) {
+            if (!it.partial(e, a.sinks)) continue;
+            const int key = it.key0(e);
+            const int lo0 = max(0, a.sinks - key), hi0 = min(kBlk, it.wlo - key);  // before the window
+            const int lo1 = max(0, it.vis_end - key);                             // past the last key
+            uint8_t* v = smem + kOffKV + ring_slot(iv) * kTile + (e & 1) * (kBox / 2);
+            for (int row = lane >> 3; row < kBlk; row += 4) {
+              if ((row >= lo0 && row < hi0) || row >= lo1) {
+                uint8_t* p = v + row * 128 + (lane & 7) * 16;
+                *reinterpret_cast<uint4*>(p) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(p + kBox) = make_uint4(0, 0, 0, 0);
+              }
+            }
+            wrote = true;
+          }
+          if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kBarClr + (ring_slot(iv) >> 1)));
+        }
+      }
+    } else if (warp < 12) {
+      // ------------------------------------------------------------ output
+      // Warp 8 + q reads TMEM lanes 32q.. (query rows) of O_t once the MMA
+      // warp reports it final, frees O_t for the next item, and writes the
+      // normalised rows.
+      const int quad = warp & 3;
+      const int row = quad * 32 + lane;
+      const int G = a.hq / a.hkv;
+      const int tok = row / G, head = row - tok * G;
+      const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+      int nq[2] = {0, 0};
+      bool ok = true;
+      while (ok && walk.next(a, it)) {
+#pragma unroll 1
+        for (int t = 0; t < (it.two ? 2 : 1); ++t) {
+          const int n = t ? nq[1]++ : nq[0]++;
+          ok = wait(kBarOfull + t, n, 40 + t) && wait(kBarL + t, n, 42 + t);
+          if (!ok) break;
+          tc_fence_after();
+          const float l_row = lbuf[((n & 1) * 2 + t) * 128 + row];
+          const float inv_l = l_row != 0.f ? 1.0f / l_row : 0.f;
+          const int row_q = it.q0 + t * a.tok + tok;
+          const bool valid = tok < a.tok && row_q < it.S;
+          __half* orow = a.out + (int64_t)(it.q_start + row_q) * a.q_row_stride +
+                         (int64_t)(it.kh * G + head) * 128;
+          const uint32_t tO = tmem + 256 + t * 128 + lane_off;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t r[32];
+            tmem_ld32(tO + c * 32, r);
+            tc_wait_ld();
+            if (c == 3) {  // all of O_t is in registers now: release it
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(kBarOempty + t));
+            }
+            if (valid) {
+              uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint4 u;
+                u.x = pack_half2(__uint_as_float(r[8 * v + 0]) * inv_l, __uint_as_float(r[8 * v + 1]) * inv_l);
+                u.y = pack_half2(__uint_as_float(r[8 * v + 2]) * inv_l, __uint_as_float(r[8 * v + 3]) * inv_l);
+                u.z = pack_half2(__uint_as_float(r[8 * v + 4]) * inv_l, __uint_as_float(r[8 * v + 5]) * inv_l);
+                u.w = pack_half2(__uint_as_float(r[8 * v + 6]) * inv_l, __uint_as_float(r[8 * v + 7]) * inv_l);
+                dst[v] = u;
+              }
+            }
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // --------------------------------------------------------------- softmax
+    const int t = warp >> 2;            // query tile
+    const int row = threadIdx.x & 127;  // TMEM lane == query row within the tile
+    const int tok = row / (a.hq / a.hkv);
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + t * 128 + lane_off;
+    const uint32_t tO = tmem + 256 + t * 128 + lane_off;
+    const float sl2 = a.scale_log2;
+    int sc = 0, nq = 0;
+    bool ok = true;
+    while (ok && walk.next(a, it)) {
+      if (t == 1 && !it.two) continue;
+      const int row_q = it.q0 + t * a.tok + tok;
+      const int key_lim = min(it.P + row_q, it.vis_end - 1);  // last visible key
+      const int key_low = it.P + row_q - a.window + 1;        // first key of the window
+      const int n_t = t == 0 ? it.n0 : it.n_kv;
+      float m_run = -INFINITY, l = 0.f;  // m_run: the max P is exponentiated against
+      for (int j = 0; j < n_t; ++j) {
+        ok = wait(kBarS + t, sc, 30 + t);
+        if (!ok) break;
+        ++sc;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
+        tc_wait_ld();
+        float s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(r[c][i]);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int e = 2 * j + hh;
+          const int base = it.key0(e);
+          const int lim = e < it.nblk ? key_lim - base : -1;
+          if (lim < kBlk - 1) {
+#pragma unroll
+            for (int c = 0; c < kBlk; ++c)
+              if (c > lim) s[hh * kBlk + c] = -INFINITY;
+          }
+          const int low = key_low - base, sk = a.sinks - base;
+          if (low > 0 && sk < min(low, kBlk)) {
+#pragma unroll
+            for (int c = 0; c < kBlk; ++c)
+              if (c < low && c >= sk) s[hh * kBlk + c] = -INFINITY;
+          }
+        }
+        float mx0 = fmax3_nan(s[0], s[1], s[0]), mx1 = fmax3_nan(s[2], s[3], s[2]);
+        float mx2 = fmax3_nan(s[4], s[5], s[4]), mx3 = fmax3_nan(s[6], s[7], s[6]);
+#pragma unroll
+        for (int c = 8; c < 128; c += 8) {
+          mx0 = fmax3_nan(mx0, s[c], s[c + 1]);
+          mx1 = fmax3_nan(mx1, s[c + 2], s[c + 3]);
+          mx2 = fmax3_nan(mx2, s[c + 4], s[c + 5]);
+          mx3 = fmax3_nan(mx3, s[c + 6], s[c + 7]);
+        }
+        const float mx_s = fmax3_nan(fmax3_nan(mx0, mx1, mx2), mx3, mx3) * sl2;
+        float alpha = 1.0f;
+        float m_new = m_run;
+        if (mx_s > m_run + kRescaleThreshold) {
+          m_new = mx_s;
+          alpha = ex2(m_run - m_new);
+        }
+        const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
+        const uint64_t sl2x2 = f2pack(sl2, sl2);
+        const uint64_t negm2 = f2pack(-m_use, -m_use);
+        uint64_t rsum = f2pack(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t x2 = ffma2(f2pack(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), sl2x2, negm2);
+            float p0, p1;
+            if (poly_pair(i)) {
+              ex2_poly2(x2, p0, p1);
+            } else {
+              float x0, x1;
+              f2unpack(x2, x0, x1);
+              p0 = ex2(x0);
+              p1 = ex2(x1);
+            }
+            rsum = fadd2(rsum, f2pack(p0, p1));
+            pk[i] = pack_half2(p0, p1);
+          }
+          asm volatile(
+              "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, "
+              "%10, %11, %12, %13, %14, %15, %16};" ::"r"(tS + c * 16),
+              "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]),
+              "r"(pk[7]), "r"(pk[8]), "r"(pk[9]), "r"(pk[10]), "r"(pk[11]), "r"(pk[12]),
+              "r"(pk[13]), "r"(pk[14]), "r"(pk[15])
+              : "memory");
+        }
+        float rs0, rs1;
+        f2unpack(rsum, rs0, rs1);
+        l = l * alpha + (rs0 + rs1);
+        // a NaN or an infinite score of a visible key makes the row NaN (the
+        // clamp of ex2_poly2 would lose it)
+        if (!(mx_s < INFINITY)) l = NAN;
+        // Rescale O_t only when some row of the warp moved its reference max
+        // (PV_t(j-1) has completed: it was issued before the QK that produced
+        // this S).
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(tO + c * 32, o);
+          }
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kBarP + t));
+        m_run = m_new;
+      }
+      if (!ok) break;
+      // Row sums for the output warps.  The output warps must have taken
+      // the previous item's sums (O_t of that item read out) first, so the
+      // row-sum barrier never runs two phases ahead of its reader.
+      if (nq > 0 && !(ok = wait(kBarOempty + t, nq - 1, 32 + t))) break;
+      lbuf[((nq & 1) * 2 + t) * 128 + row] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kBarL + t));
+      ++nq;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 13) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+cudaError_t prefill_window_set_attributes() {
+  for (auto k : {prefill_window_kernel<false>, prefill_window_kernel<true>}) {
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+cudaError_t launch_prefill_window(const PrefillWindowArgs& a, int32_t max_q_len, int num_sms,
+                                  const CUtensorMap& tm_q, const CUtensorMap& tm_k,
+                                  const CUtensorMap& tm_v, cudaStream_t s) {
+  const int64_t items = (int64_t)((max_q_len + 2 * (int64_t)a.tok - 1) / (2 * a.tok)) * a.hkv * a.batch;
+  if (items == 0) return cudaSuccess;
+  const int grid = (int)(items < num_sms ? items : num_sms);
+  if (a.page_table)
+    prefill_window_kernel<true><<<grid, kThreads, kSmemBytes, s>>>(tm_q, tm_k, tm_v, a);
+  else
+    prefill_window_kernel<false><<<grid, kThreads, kSmemBytes, s>>>(tm_q, tm_k, tm_v, a);
+  return cudaGetLastError();
+}
+
+}  // namespace grout

@@ -516,9 +516,13 @@ grout_status grout_attn_decode_paged_window(const void* q, const void* k_pages,
                                             size_t workspace_bytes, grout_stream_t stream);
 /* Window forms of grout_attn_prefill_varlen (cu_seqlens_q may be NULL with
  * batch 1: one sequence of max_q_len rows) and grout_attn_prefill_paged;
- * arguments as there.  K/V rows that some row of a 256-row query block sees
- * must be finite for the block's other rows (a weight of 0 times an infinity
- * is a NaN); all other rows may hold anything. */
+ * arguments as there; a group of up to 128 query heads per KV head.  Keys
+ * stay below kv_rows (varlen: kv_start + position) or dims->max_seq (paged),
+ * query rows below q_rows: a sequence that does not is left out, with device
+ * error 0x200.  Query rows are worked on in blocks of 2 * floor(128 / group)
+ * neighbours: a V row that one of them sees must be finite for the others (a
+ * weight of 0 times an infinity is a NaN); all other rows may hold anything.
+ * A page outside the pool that holds a visible key reads as zeros (0x201). */
 grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* args,
                                               int32_t window, int32_t sinks,
                                               const grout_attn_dims* dims, grout_stream_t stream);
