@@ -1309,6 +1309,7 @@ static grout_status window_prefill(PrefillWindowArgs* a, const void* q, void* ou
   grout_status st = current_state(&ds);
   if (st != GROUT_OK) return st;
   const int32_t group = (int32_t)(hq / hkv);
+  a->group = group;
   a->tok = 128 / group;
   CUtensorMap tq, tk, tv;
   const uint64_t dq[3] = {128, (uint64_t)hq, (uint64_t)q_rows};

@@ -240,7 +240,8 @@ struct PrefillWindowArgs {
   int32_t single_len;   // used when cu_q == null (batch 1)
   int32_t hq;
   int32_t hkv;
-  int32_t tok;          // tokens per query tile: 128 / (hq / hkv)
+  int32_t group;        // hq / hkv
+  int32_t tok;          // tokens per query tile: 128 / group
   int32_t window;
   int32_t sinks;
   float scale_log2;

@@ -41,14 +41,18 @@ constexpr int kBlk = 64;       // keys per block, two blocks per KV tile
 constexpr int kSlots = 4;      // K/V ring slots (even ring entries K, odd ones V)
 constexpr int kThreads = 512;  // 4 warpgroups, one persistent CTA per SM
 // Register split (setmaxnreg): launched at 128 per thread (512 x 128 =
-// 65536); 2 x 128 x 192 + 2 x 128 x 64 = 65536.
-constexpr int kRegsOther = 64;
-constexpr int kRegsSoftmax = 192;
+// 65536); 2 x 128 x 152 + 2 x 128 x 104 = 65536.
+constexpr int kRegsOther = 104;
+constexpr int kRegsSoftmax = 152;
 constexpr int kOffQ = 0;          // 2 query tiles
 constexpr int kOffKV = 2 * kTile; // ring
 constexpr int kOffBar = kOffKV + kSlots * kTile;
 constexpr int kOffL = kOffBar + 512;  // row sums [item parity][tile][row]
-constexpr int kSmemBytes = kOffL + 2 * 2 * 128 * 4 + 1024;
+constexpr int kOffAbort = kOffBar + 448;
+constexpr int kOffTmem = kOffBar + 452;
+constexpr int kOffWalk = kOffL + 2 * 2 * 128 * 4;  // each warp's place in the item list
+constexpr int kOffMask = kOffWalk + 16 * 32;       // softmax warps: what masks the tiles of their item
+constexpr int kSmemBytes = kOffMask + 8 * 32 + 1024;
 
 // barrier indices (phases run on across the work items of a CTA; those of
 // tile 1 skip the items that have one tile)
@@ -61,12 +65,52 @@ constexpr int kBarP = kBarS + 2;              // + tile (4 softmax warps)
 constexpr int kBarOfull = kBarP + 2;          // + tile: O_t of the item final (commit)
 constexpr int kBarOempty = kBarOfull + 2;     // + tile: O_t read out (4 output warps)
 constexpr int kBarL = kBarOempty + 2;         // + tile: row sums written (4 softmax warps)
-constexpr int kBarClr = kBarL + 2;            // + V slot (ring slot / 2): unseen rows cleared (warp 14)
+constexpr int kBarClr = kBarL + 2;            // + V slot (ring slot / 2): V tile with unseen rows cleared
 constexpr int kBarDrain = kBarClr + 2;        // MMAs in flight when a wait gave up
 constexpr int kNumBars = kBarDrain + 1;
+static_assert(kNumBars * 8 <= 448, "barriers overlap the abort flag");
 
 __device__ __forceinline__ int ring_slot(int i) { return i % kSlots; }
 __device__ __forceinline__ uint32_t ring_parity(int i) { return (uint32_t)((i / kSlots) & 1); }
+
+// Shared memory by 32-bit addresses: generic pointers would hold two registers
+// each through the softmax loop, which has none to spare.
+__device__ __forceinline__ int ld_shared(uint32_t addr) {
+  int v;
+  asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ int4 ld_shared4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.volatile.shared.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared(uint32_t addr, int v) {
+  asm volatile("st.volatile.shared.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_shared4(uint32_t addr, int x, int y, int z, int w) {
+  asm volatile("st.volatile.shared.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x), "r"(y),
+               "r"(z), "r"(w)
+               : "memory");
+}
+// mbar_wait with the abort flag by its shared address.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* err, int site,
+                                         uint32_t abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 0) {
+      if (ld_shared(abort_flag)) return false;
+      if (globaltimer() - t0 > kWaitTimeoutNs) {
+        st_shared(abort_flag, 1);
+        if (err) atomicCAS(err, 0, DEV_ERR_TIMEOUT_BASE + site);
+        return false;
+      }
+    }
+  }
+}
 
 __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
   float d;
@@ -74,8 +118,13 @@ __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
   return d;
 }
 
+// The lowest n of 32 bits (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t bits_below(int n) {
+  return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1u;
+}
+
 struct Item {
-  int b, kh, q0, S, P, ks, q_start;
+  int b, kh, q0, S, P, q_start;
   int n0, n_kv;     // KV tiles of query tile 0, of the item (tile 1 takes all)
   bool two;         // the item has a second query tile
   int nblk, sink_blk, skip;  // 64-key blocks; entry i is block i or, past the sinks, i + skip
@@ -87,6 +136,11 @@ struct Item {
     const int k = key0(i);
     return k + kBlk > vis_end || (k < wlo && k + kBlk > sinks);
   }
+  // whether V tile j may have rows to clear: it holds the sinks' last block, the
+  // window's first one or the item's last one
+  __device__ __forceinline__ bool clears(int j) const {
+    return j == (sink_blk - 1) >> 1 || j == sink_blk >> 1 || j == n_kv - 1;
+  }
 };
 
 // Walks this CTA's items: entry r * grid + c of the list (r * grid + grid - 1
@@ -95,9 +149,8 @@ struct Item {
 // fastest.  A sequence whose lengths or positions fit neither the query rows
 // nor the cache has no items (device error 0x200).
 struct Walk {
-  int r = 0, b = -1;
-  int64_t base = 0;
-  int cnt = 0, S = 0, P = 0, ks = 0, q_start = 0;
+  int r = 0, b = -1, base = 0, cnt = 0;
+  int S = 0, P = 0, pairs = 0, q_start = 0;
 
   __device__ __forceinline__ void enter(const PrefillWindowArgs& a) {
     if (a.cu_q) {
@@ -108,7 +161,7 @@ struct Walk {
       S = a.single_len;
     }
     P = a.pos0 ? a.pos0[b] : 0;
-    ks = a.kv_start ? a.kv_start[b] : 0;
+    const int ks = a.kv_start ? a.kv_start[b] : 0;
     cnt = 0;
     if (S <= 0) return;
     if (q_start < 0 || (int64_t)q_start + S > a.q_rows || P < 0 || ks < 0 ||
@@ -116,12 +169,13 @@ struct Walk {
       if (a.err) atomicCAS(a.err, 0, DEV_ERR_POSITION);
       return;
     }
-    cnt = (S + 2 * a.tok - 1) / (2 * a.tok) * a.hkv;
+    pairs = (S + 2 * a.tok - 1) / (2 * a.tok);
+    cnt = pairs * a.hkv;
   }
 
   __device__ __forceinline__ bool next(const PrefillWindowArgs& a, Item& it) {
-    const int64_t G = gridDim.x, c = blockIdx.x;
-    const int64_t k = r * G + ((r & 1) ? G - 1 - c : c);
+    const int G = gridDim.x, c = blockIdx.x;
+    const int k = r * G + ((r & 1) ? G - 1 - c : c);
     ++r;
     while (k >= base + cnt) {
       if (b >= a.batch - 1) return false;
@@ -129,13 +183,13 @@ struct Walk {
       ++b;
       enter(a);
     }
-    const int local = (int)(k - base);
-    const int pair = cnt / a.hkv - 1 - local / a.hkv;
+    const int local = k - base;
+    const int back = local / a.hkv;  // pairs behind this one
+    const int pair = pairs - 1 - back;
     it.b = b;
-    it.kh = local % a.hkv;
+    it.kh = local - back * a.hkv;
     it.S = S;
     it.P = P;
-    it.ks = ks;
     it.q_start = q_start;
     it.q0 = pair * 2 * a.tok;
     it.two = S > it.q0 + a.tok;
@@ -158,18 +212,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                           const __grid_constant__ CUtensorMap tm_k,
                           const __grid_constant__ CUtensorMap tm_v, const PrefillWindowArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + kNumBars);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  float* lbuf = reinterpret_cast<float*>(smem + kOffL);
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023) & ~1023u;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  auto bar = [&](int i) -> uint32_t { return smem_u32(&bars[i]); };
+  auto bar = [&](int i) -> uint32_t { return smem_base + kOffBar + 8 * i; };
   auto wait = [&](int i, uint32_t parity, int site) -> bool {
-    return mbar_wait(bar(i), parity & 1u, a.err, site, abort_flag);
+    return bar_wait(bar(i), parity & 1u, a.err, site, smem_base + kOffAbort);
   };
 
   if (threadIdx.x == 0) {
@@ -177,22 +226,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       // P, Oempty, L: one arrival per warp of a warpgroup
       const bool four = (i >= kBarP && i < kBarP + 2) || (i >= kBarOempty && i < kBarOempty + 2) ||
                         (i >= kBarL && i < kBarL + 2);
-      mbar_init(bar(i), four ? 4 : 1);
+      // a V slot is empty once the MMA warp and warp 14 are through with it
+      const bool v_empty = i == kBarEmpty + 1 || i == kBarEmpty + 3;
+      mbar_init(bar(i), four ? 4 : (v_empty ? 2 : 1));
     }
-    *abort_flag = 0;
+    st_shared(smem_base + kOffAbort, 0);
     fence_mbar_init();
   }
   if (warp == 13) {
-    tmem_alloc(smem_u32(tmem_holder), 512);
+    tmem_alloc(smem_base + kOffTmem, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
-  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t tmem = (uint32_t)ld_shared(smem_base + kOffTmem);
 
-  Walk walk;
+  // The next item of a whole warp.  Its place in the list waits in shared
+  // memory between items: no role has eight registers to spare for it.
+  const uint32_t place = smem_base + kOffWalk + warp * 32;
+  if (lane == 0) {
+    st_shared4(place, 0, -1, 0, 0);
+    st_shared4(place + 16, 0, 0, 0, 0);
+  }
+  __syncwarp();
+  auto next_item = [&](Item& x) -> bool {
+    const int4 p0 = ld_shared4(place), p1 = ld_shared4(place + 16);
+    Walk w;
+    w.r = p0.x, w.b = p0.y, w.base = p0.z, w.cnt = p0.w;
+    w.S = p1.x, w.P = p1.y, w.pairs = p1.z, w.q_start = p1.w;
+    const bool has = w.next(a, x);
+    __syncwarp();
+    if (lane == 0) {
+      st_shared4(place, w.r, w.b, w.base, w.cnt);
+      st_shared4(place + 16, w.S, w.P, w.pairs, w.q_start);
+    }
+    __syncwarp();
+    return has;
+  };
   Item it;
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
@@ -205,24 +276,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         int ring = 0;
         int nq[2] = {0, 0};
         bool ok = true;
-        while (ok && walk.next(a, it)) {
+        Walk walk;
+        Item nx = {};
+        bool has = walk.next(a, nx);
+        while (ok && has) {
+          it = nx;
+          const int ks = a.kv_start ? a.kv_start[it.b] : 0;
           // Q_0, K_0, Q_1, then the rest: each tile's query buffer is refilled
           // as soon as that tile's last QK of the previous item has run.
           auto load_q = [&](int t) -> bool {
             if (nq[t] > 0 && !wait(kBarQfree + t, nq[t] - 1, 11 + t)) return false;
             ++nq[t];
-            mbar_arrive_expect_tx(bar(kBarQ + t), a.tok * (a.hq / a.hkv) * 256);
+            mbar_arrive_expect_tx(bar(kBarQ + t), a.tok * a.group * 256);
             const uint32_t dst = smem_base + kOffQ + t * kTile;
-            const int row = it.q_start + it.q0 + t * a.tok, head = it.kh * (a.hq / a.hkv);
+            const int row = it.q_start + it.q0 + t * a.tok, head = it.kh * a.group;
             tma_load_3d(dst, &tm_q, bar(kBarQ + t), 0, head, row);
             tma_load_3d(dst + kBox, &tm_q, bar(kBarQ + t), 64, head, row);
             return true;
           };
           if (!load_q(0)) break;
           for (int i = 0; i < 2 * it.n_kv; ++i) {
-            if (i == 1 && it.two && !load_q(1)) {
-              ok = false;
-              break;
+            if (i == 1) {
+              if (it.two && !load_q(1)) {
+                ok = false;
+                break;
+              }
+              has = walk.next(a, nx);  // off the path between two items' loads
             }
             const int slot = ring_slot(ring);
             if (ring >= kSlots && !wait(kBarEmpty + slot, ring_parity(ring) ^ 1u, 10)) {
@@ -245,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   if (page >= 0 && page < a.num_pages) outer[hh] = page;
                   else if (a.err) atomicCAS(a.err, 0, DEV_ERR_PAGE);
                 } else {
-                  row[hh] = it.ks + key;
+                  row[hh] = ks + key;
                 }
               }
             }
@@ -262,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // a wait gave up: let the loads in flight land before the CTA leaves
-        if (*abort_flag) {
+        if (ld_shared(smem_base + kOffAbort)) {
           for (int i = max(0, ring - kSlots); i < ring; ++i)
             for (int n = 0; n < (1 << 20); ++n)
               if (mbar_try_wait(bar(kBarFull + ring_slot(i)), ring_parity(i))) break;
@@ -306,6 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int nst[2] = {0, 0};  // items started per tile (QK_t(0) issued)
       int npv[2] = {0, 0};  // items per tile whose first PV_t has been issued
       int pc[2] = {0, 0};   // P_t tiles taken
+      int nclr[2] = {0, 0}; // cleared V tiles taken, per V slot
       auto start = [&](int t, const Item& x, int iring) -> bool {
         if (!wait(kBarQ + t, nst[t], 20 + t) || !wait(kBarFull + ring_slot(iring), ring_parity(iring), 22))
           return false;
@@ -329,17 +409,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int ring = 0;
       Item cur = {}, nx = {};
-      bool has = walk.next(a, cur);
+      bool has = next_item(cur);
       bool ok = !has || (start(0, cur, ring) && (!cur.two || start(1, cur, ring)));
       while (has && ok) {
-        const bool hn = walk.next(a, nx);
+        const bool hn = next_item(nx);
         const int n_kv = cur.n_kv, n0 = cur.n0;
         const int nring = ring + 2 * n_kv;  // K_0 of the next item
         for (int j = 0; j < n_kv; ++j) {
           const int iv = ring + 2 * j + 1, ik = ring + 2 * j + 2;
           const bool next = j + 1 < n_kv;
-          ok = wait(kBarFull + ring_slot(iv), ring_parity(iv), 23) &&
-               wait(kBarClr + (ring_slot(iv) >> 1), ring_parity(iv), 29);
+          ok = wait(kBarFull + ring_slot(iv), ring_parity(iv), 23);
+          if (ok && cur.clears(j)) {
+            const int vs = ring_slot(iv) >> 1;
+            ok = wait(kBarClr + vs, nclr[vs], 29);
+            ++nclr[vs];
+          }
           // K(j+1) only needs the slot K(j-1) released, so it is awaited
           // here, before P0(j), keeping the wait off the PV0 -> QK0 path.
           if (ok && next) ok = wait(kBarFull + ring_slot(ik), ring_parity(ik), 22);
@@ -389,30 +473,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       // within a row only, so whole rows are cleared in place.
       int ring = 0;
       bool ok = true;
-      while (ok && walk.next(a, it)) {
+      while (ok && next_item(it)) {
         for (int j = 0; j < it.n_kv; ++j, ring += 2) {
           const int iv = ring + 1;
           ok = wait(kBarFull + ring_slot(iv), ring_parity(iv), 50);
           if (!ok) break;
-          bool wrote = false;
           for (int e = 2 * j; e < min(2 * j + 2, it.nblk); ++e) {
-            if (!it.partial(e, a.sinks)) continue;
+            if (!it.partial(e, a.sinks)) continue;  // (a second block past the last is TMA's zeros)
             const int key = it.key0(e);
             const int lo0 = max(0, a.sinks - key), hi0 = min(kBlk, it.wlo - key);  // before the window
             const int lo1 = max(0, it.vis_end - key);                             // past the last key
-            uint8_t* v = smem + kOffKV + ring_slot(iv) * kTile + (e & 1) * (kBox / 2);
+            const uint32_t v = smem_base + kOffKV + ring_slot(iv) * kTile + (e & 1) * (kBox / 2);
             for (int row = lane >> 3; row < kBlk; row += 4) {
               if ((row >= lo0 && row < hi0) || row >= lo1) {
-                uint8_t* p = v + row * 128 + (lane & 7) * 16;
-                *reinterpret_cast<uint4*>(p) = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(p + kBox) = make_uint4(0, 0, 0, 0);
+                st_shared4(v + row * 128 + (lane & 7) * 16, 0, 0, 0, 0);
+                st_shared4(v + kBox + row * 128 + (lane & 7) * 16, 0, 0, 0, 0);
               }
             }
-            wrote = true;
           }
-          if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          const bool cleared = it.clears(j);
+          if (cleared) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(kBarClr + (ring_slot(iv) >> 1)));
+          if (lane == 0) {
+            if (cleared) mbar_arrive(bar(kBarClr + (ring_slot(iv) >> 1)));
+            mbar_arrive(bar(kBarEmpty + ring_slot(iv)));
+          }
         }
       }
     } else if (warp < 12) {
@@ -422,19 +507,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       // normalised rows.
       const int quad = warp & 3;
       const int row = quad * 32 + lane;
-      const int G = a.hq / a.hkv;
+      const int G = a.group;
       const int tok = row / G, head = row - tok * G;
       const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
       int nq[2] = {0, 0};
       bool ok = true;
-      while (ok && walk.next(a, it)) {
+      while (ok && next_item(it)) {
 #pragma unroll 1
         for (int t = 0; t < (it.two ? 2 : 1); ++t) {
           const int n = t ? nq[1]++ : nq[0]++;
           ok = wait(kBarOfull + t, n, 40 + t) && wait(kBarL + t, n, 42 + t);
           if (!ok) break;
           tc_fence_after();
-          const float l_row = lbuf[((n & 1) * 2 + t) * 128 + row];
+          const float l_row = __int_as_float(ld_shared(smem_base + kOffL + (((n & 1) * 2 + t) * 128 + row) * 4));
           const float inv_l = l_row != 0.f ? 1.0f / l_row : 0.f;
           const int row_q = it.q0 + t * a.tok + tok;
           const bool valid = tok < a.tok && row_q < it.S;
@@ -472,60 +557,87 @@ __global__ void __launch_bounds__(kThreads, 1)
     // --------------------------------------------------------------- softmax
     const int t = warp >> 2;            // query tile
     const int row = threadIdx.x & 127;  // TMEM lane == query row within the tile
-    const int tok = row / (a.hq / a.hkv);
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off;
     const uint32_t tO = tmem + 256 + t * 128 + lane_off;
     const float sl2 = a.scale_log2;
+    // What masked tiles need waits in shared memory (two records: the next
+    // item's is written while this one is worked on).  Tiles j_lo <= j < j_hi
+    // hold only keys that every row of the tile sees.
+    const int tok = row / a.group;
+    uint32_t rec = 0, rec_next = smem_base + kOffMask + warp * 32;
+    int n_next = 0, lo_next = 0, hi_next = 0;
+    auto next_tile = [&]() -> bool {
+      Item x = {};
+      do {
+        if (!next_item(x)) return false;
+      } while (t == 1 && !x.two);
+      const int first = x.P + x.q0 + t * a.tok;  // position of the tile's first row
+      if (lane == 0) st_shared4(rec_next, first, x.sink_blk, x.skip, x.vis_end);
+      __syncwarp();
+      n_next = t == 0 ? x.n0 : x.n_kv;
+      // blocks from low_all on lie in every row's window, those before
+      // first + 1 past no row's position
+      const int low_all = max(0, first + a.tok - a.window);
+      lo_next = max(0, (low_all + kBlk - 1) / kBlk - x.skip + 1) / 2;
+      hi_next = max(0, (first + 1) / kBlk - x.skip) / 2;
+      return true;
+    };
     int sc = 0, nq = 0;
     bool ok = true;
-    while (ok && walk.next(a, it)) {
-      if (t == 1 && !it.two) continue;
-      const int row_q = it.q0 + t * a.tok + tok;
-      const int key_lim = min(it.P + row_q, it.vis_end - 1);  // last visible key
-      const int key_low = it.P + row_q - a.window + 1;        // first key of the window
-      const int n_t = t == 0 ? it.n0 : it.n_kv;
+    bool has = next_tile();
+    while (ok && has) {
+      const int n_t = n_next, j_lo = lo_next, j_hi = hi_next;
+      rec = rec_next;
+      rec_next ^= 16;
       float m_run = -INFINITY, l = 0.f;  // m_run: the max P is exponentiated against
       for (int j = 0; j < n_t; ++j) {
+        if (j == n_t - 1) has = next_tile();  // while S is computed
         ok = wait(kBarS + t, sc, 30 + t);
         if (!ok) break;
         ++sc;
         tc_fence_after();
-        uint32_t r[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, r[c]);
-        tc_wait_ld();
-        float s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s[c * 32 + i] = __uint_as_float(r[c][i]);
-#pragma unroll
+        // Two passes over S, a 64-key block at a time (rolled: code that is
+        // unrolled over all 128 columns does not stay in the instruction
+        // cache beside the other roles' code, and leaves no registers).
+        // Pass 1: the row maximum; masked scores go back to S.
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+        const bool masked = j < j_lo || j >= j_hi;
+#pragma unroll 1
         for (int hh = 0; hh < 2; ++hh) {
-          const int e = 2 * j + hh;
-          const int base = it.key0(e);
-          const int lim = e < it.nblk ? key_lim - base : -1;
-          if (lim < kBlk - 1) {
+          uint32_t r[2][32];
+          tmem_ld32(tS + hh * kBlk, r[0]);
+          tmem_ld32(tS + hh * kBlk + 32, r[1]);
+          tc_wait_ld();
+          if (masked) {  // (a block past the last one starts past every row)
+            const int4 m = ld_shared4(rec);
+            const int pos = m.x + tok;  // this row's position
+            const int e = 2 * j + hh;
+            const int base = (e < m.y ? e : e + m.z) * kBlk;
+            const int end = min(pos + 1, m.w) - base, low = pos - a.window + 1 - base, sk = a.sinks - base;
 #pragma unroll
-            for (int c = 0; c < kBlk; ++c)
-              if (c > lim) s[hh * kBlk + c] = -INFINITY;
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t keep = bits_below(end - 32 * w) & (~bits_below(low - 32 * w) | bits_below(sk - 32 * w));
+              // a warp's rows are a few neighbouring tokens: most words are the same for all
+              if (__all_sync(0xffffffffu, keep == 0xFFFFFFFFu)) continue;
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (!(keep & (1u << c))) r[w][c] = 0xFF800000u;  // -inf
+              tmem_st32(tS + hh * kBlk + w * 32, r[w]);
+            }
           }
-          const int low = key_low - base, sk = a.sinks - base;
-          if (low > 0 && sk < min(low, kBlk)) {
 #pragma unroll
-            for (int c = 0; c < kBlk; ++c)
-              if (c < low && c >= sk) s[hh * kBlk + c] = -INFINITY;
-          }
-        }
-        float mx0 = fmax3_nan(s[0], s[1], s[0]), mx1 = fmax3_nan(s[2], s[3], s[2]);
-        float mx2 = fmax3_nan(s[4], s[5], s[4]), mx3 = fmax3_nan(s[6], s[7], s[6]);
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int c = 8; c < 128; c += 8) {
-          mx0 = fmax3_nan(mx0, s[c], s[c + 1]);
-          mx1 = fmax3_nan(mx1, s[c + 2], s[c + 3]);
-          mx2 = fmax3_nan(mx2, s[c + 4], s[c + 5]);
-          mx3 = fmax3_nan(mx3, s[c + 6], s[c + 7]);
+            for (int c = 0; c < 32; c += 8) {
+              const auto f = [&](int i) { return __uint_as_float(r[w][c + i]); };
+              mx0 = fmax3_nan(mx0, f(0), f(1));
+              mx1 = fmax3_nan(mx1, f(2), f(3));
+              mx2 = fmax3_nan(mx2, f(4), f(5));
+              mx3 = fmax3_nan(mx3, f(6), f(7));
+            }
         }
+        if (masked) tc_wait_st();
         const float mx_s = fmax3_nan(fmax3_nan(mx0, mx1, mx2), mx3, mx3) * sl2;
         float alpha = 1.0f;
         float m_new = m_run;
@@ -537,31 +649,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t sl2x2 = f2pack(sl2, sl2);
         const uint64_t negm2 = f2pack(-m_use, -m_use);
         uint64_t rsum = f2pack(0.f, 0.f);
+        // Pass 2: P.  Block hh's P lands on columns that its own S (hh = 0) or
+        // block 0's S (hh = 1) no longer needs.
+#pragma unroll 1
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t r[2][32];
+          tmem_ld32(tS + hh * kBlk, r[0]);
+          tmem_ld32(tS + hh * kBlk + 32, r[1]);
+          tc_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+          for (int w = 0; w < 2; ++w) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint64_t x2 = ffma2(f2pack(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), sl2x2, negm2);
-            float p0, p1;
-            if (poly_pair(i)) {
-              ex2_poly2(x2, p0, p1);
-            } else {
-              float x0, x1;
-              f2unpack(x2, x0, x1);
-              p0 = ex2(x0);
-              p1 = ex2(x1);
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t x2 = ffma2(f2pack(__uint_as_float(r[w][2 * i]), __uint_as_float(r[w][2 * i + 1])), sl2x2, negm2);
+              float p0, p1;
+              if (poly_pair(i)) {
+                ex2_poly2(x2, p0, p1);
+              } else {
+                float x0, x1;
+                f2unpack(x2, x0, x1);
+                p0 = ex2(x0);
+                p1 = ex2(x1);
+              }
+              rsum = fadd2(rsum, f2pack(p0, p1));
+              pk[i] = pack_half2(p0, p1);
             }
-            rsum = fadd2(rsum, f2pack(p0, p1));
-            pk[i] = pack_half2(p0, p1);
+            asm volatile(
+                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, "
+                "%10, %11, %12, %13, %14, %15, %16};" ::"r"(tS + hh * 32 + w * 16),
+                "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]),
+                "r"(pk[7]), "r"(pk[8]), "r"(pk[9]), "r"(pk[10]), "r"(pk[11]), "r"(pk[12]),
+                "r"(pk[13]), "r"(pk[14]), "r"(pk[15])
+                : "memory");
           }
-          asm volatile(
-              "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, "
-              "%10, %11, %12, %13, %14, %15, %16};" ::"r"(tS + c * 16),
-              "r"(pk[0]), "r"(pk[1]), "r"(pk[2]), "r"(pk[3]), "r"(pk[4]), "r"(pk[5]), "r"(pk[6]),
-              "r"(pk[7]), "r"(pk[8]), "r"(pk[9]), "r"(pk[10]), "r"(pk[11]), "r"(pk[12]),
-              "r"(pk[13]), "r"(pk[14]), "r"(pk[15])
-              : "memory");
         }
         float rs0, rs1;
         f2unpack(rsum, rs0, rs1);
@@ -594,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the previous item's sums (O_t of that item read out) first, so the
       // row-sum barrier never runs two phases ahead of its reader.
       if (nq > 0 && !(ok = wait(kBarOempty + t, nq - 1, 32 + t))) break;
-      lbuf[((nq & 1) * 2 + t) * 128 + row] = l;
+      st_shared(smem_base + kOffL + (((nq & 1) * 2 + t) * 128 + row) * 4, __float_as_int(l));
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kBarL + t));
       ++nq;
