@@ -1198,14 +1198,15 @@ grout_status grout_attn_decode_window(const void* q, const void* k_cache, const 
                           workspace, workspace_bytes);
   if (st != GROUT_OK) return st;
   CUtensorMap tk, tv;
-  const uint64_t dk[4] = {128, (uint64_t)dims->max_seq, (uint64_t)dims->num_kv_heads,
+  // a row's two 64-dim halves as a dimension of their own: one load per tile
+  const uint64_t dk[5] = {64, (uint64_t)dims->max_seq, 2, (uint64_t)dims->num_kv_heads,
                           (uint64_t)batch};
-  const uint64_t sk[3] = {128, (uint64_t)cache_head_stride,
+  const uint64_t sk[4] = {128, 64, (uint64_t)cache_head_stride,
                           (uint64_t)(batch > 1 ? cache_batch_stride : cache_head_stride * dims->num_kv_heads)};
-  const uint32_t bk[4] = {64, 64, 1, 1};
-  st = encode_map(&tk, k_cache, 4, dk, sk, bk, "k_cache");
+  const uint32_t bk[5] = {64, 64, 2, 1, 1};
+  st = encode_map(&tk, k_cache, 5, dk, sk, bk, "k_cache");
   if (st != GROUT_OK) return st;
-  st = encode_map(&tv, v_cache, 4, dk, sk, bk, "v_cache");
+  st = encode_map(&tv, v_cache, 5, dk, sk, bk, "v_cache");
   if (st != GROUT_OK) return st;
   CUDA_TRY(launch_decode_window(a, tk, tv, reinterpret_cast<cudaStream_t>(stream)));
   return GROUT_OK;
@@ -1235,14 +1236,14 @@ grout_status grout_attn_decode_paged_window(const void* q, const void* k_pages,
   a.page_size = page_size;
   a.num_pages = num_pages;
   CUtensorMap tk, tv;
-  const uint64_t dk[4] = {128, (uint64_t)page_size, (uint64_t)dims->num_kv_heads,
+  const uint64_t dk[5] = {64, (uint64_t)page_size, 2, (uint64_t)dims->num_kv_heads,
                           (uint64_t)num_pages};
-  const uint64_t sk[3] = {128, (uint64_t)page_size * 128,
+  const uint64_t sk[4] = {128, 64, (uint64_t)page_size * 128,
                           (uint64_t)page_size * 128 * (uint64_t)dims->num_kv_heads};
-  const uint32_t bk[4] = {64, 64, 1, 1};
-  st = encode_map(&tk, k_pages, 4, dk, sk, bk, "k_pages");
+  const uint32_t bk[5] = {64, 64, 2, 1, 1};
+  st = encode_map(&tk, k_pages, 5, dk, sk, bk, "k_pages");
   if (st != GROUT_OK) return st;
-  st = encode_map(&tv, v_pages, 4, dk, sk, bk, "v_pages");
+  st = encode_map(&tv, v_pages, 5, dk, sk, bk, "v_pages");
   if (st != GROUT_OK) return st;
   CUDA_TRY(launch_decode_window(a, tk, tv, reinterpret_cast<cudaStream_t>(stream)));
   return GROUT_OK;

@@ -17,12 +17,17 @@
 // the f16 weights of the PV product use f16's range whatever the scales are,
 // and l sums w / vs = 2^(s - m) in f32.  Codes become f16 exactly.
 //
-// Structure as decode.cu (HBM-bound; one CTA per split, KV head and sequence;
-// a producer warp fills a TMA ring, four consumer warps run mma.sync with the
-// GQA group on the 8-wide N side, up to 16 splits merge in a thread-block
-// cluster).  A stage of the ring holds 32 KB: 64 f16 keys or 128 8-bit keys
-// (two 64-key tiles, which need not be neighbours: the sinks' last tile and
-// the window's first one share a stage).
+// HBM-bound; one CTA per split, KV head and sequence.  A producer warp fills a
+// 96 KB TMA ring of three stages, each 64 f16 keys or 128 8-bit ones (two
+// 64-key tiles, which need not be neighbours); every consumer warp takes 16
+// keys of each stage, four warps for f16 and eight for 8-bit keys, whose
+// conversion makes the chain through a stage longer than its share of the
+// memory time.  S^T = K Q^T and O^T += V^T P^T run on mma.sync m16n8k16 with
+// the GQA group on the 8-wide N side, as in decode.cu.
+// The warps merge through shared memory.  Up to 16 splits form a thread-block
+// cluster: each CTA pushes its heads' results into the shared memory of the
+// CTA that owns the head (no round trip, one barrier), which writes the row;
+// more splits go through the caller's workspace and a merge kernel.
 //
 // Keys that are not seen get no weight and their V rows are zeroed before the
 // product, so that whatever they hold (an unwritten page, a NaN) stays out.
@@ -37,45 +42,48 @@
 namespace grout {
 namespace {
 
-constexpr int kKeys = 64;  // keys per tile (one TMA box per 128 bytes of a row)
+constexpr int kKeys = 64;  // keys per tile
 constexpr int kStages = 3;
-constexpr int kStageBytes = 32768;  // K and V of one f16 tile, or of two 8-bit tiles
-constexpr int kThreads = 160;
+constexpr int kStageBytes = 32768;  // K and V of one f16 tile, or of two 8-bit ones
 constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kScaleFloats = 4 * kKeys;  // per stage: K scales of both tiles, V scales of both
-constexpr int kCtlBytes = 128;           // full/empty barriers, abort flag, per-stage tile masks
-constexpr int kSmemF16 = kRingBytes + 1024 + kCtlBytes;
+// Consumer warps; one more produces.
+__host__ __device__ constexpr int consumers(bool fp8) { return fp8 ? 8 : 4; }
+__host__ __device__ constexpr int threads(bool fp8) { return 32 * (consumers(fp8) + 1); }
+constexpr int kCtlBytes = 256;     // full/empty barriers, abort flag, per-stage tile masks
+// Split results pushed by the CTAs of a cluster: for each head that this CTA
+// owns (head % splits == rank), [split] rows of 128 values, then [split] lse.
+// At most ceil(8 / n) * n rows for n splits: 16.
+constexpr int kRecvRows = 16;
+constexpr int kRecvBytes = kRecvRows * (128 + 1) * 4;
+constexpr int kOffCtl = kRingBytes;
+constexpr int kOffRecv = kOffCtl + kCtlBytes;
+constexpr int kOffScales = kOffRecv + kRecvBytes;  // 8-bit: [stage][K0 K1 V0 V1][64]
+constexpr int kSmemF16 = kOffScales + 1024;
 constexpr int kSmemFp8 = kSmemF16 + kStages * kScaleFloats * 4;
 
 struct RedSmem {
-  float o[4][128][9];  // padded: the per-dimension merge reads are conflict-free
-  float m[4][8];
-  float l[4][8];
+  float o[8][128][9];  // [warp]; padded: the per-dimension merge reads are conflict-free
+  float m[8][8];
+  float l[8][8];
 };
-// A CTA's final split result, read by the other CTAs of its cluster.
-struct FinSmem {
-  float o[8][128];
-  float lse[8];
-};
-constexpr int kFinOffset = 20480;
-static_assert(sizeof(RedSmem) <= kFinOffset, "reduction area overlaps the split result");
-static_assert(kFinOffset + sizeof(FinSmem) <= kRingBytes, "merge areas must fit in the ring");
+static_assert(sizeof(RedSmem) <= kRingBytes, "the merge area must fit in the ring");
 
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float ld_dsmem_f32(const float* local, uint32_t rank) {
+__device__ __forceinline__ void st_dsmem_f32(float* local, uint32_t rank, float v) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
 // w_s = 2^(lse_s - max) / sum, out = sum_s w_s * O_s, rounded to f16.  Splits
@@ -125,19 +133,23 @@ struct TileList {
 };
 
 template <bool kFp8, bool kPaged, bool kCluster>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(threads(kFp8), 2)
     decode_window_kernel(const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const DecodeWindowArgs a) {
-  constexpr int kTiles = kFp8 ? 2 : 1;                   // 64-key tiles per stage
+  constexpr int kTiles = kFp8 ? 2 : 1;  // 64-key tiles per stage
   constexpr int kTileBytes = kKeys * 128 * (kFp8 ? 1 : 2);
-  constexpr int kVOff = kTiles * kTileBytes;             // V tiles follow the K tiles
+  constexpr int kVOff = kTiles * kTileBytes;  // V tiles follow the K tiles
+  constexpr int kWarps = consumers(kFp8);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kRingBytes);  // full[3], empty[3]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffCtl);  // full[kStages], empty[kStages]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * kStages);
   volatile int* bad_tile = abort_flag + 1;  // [kStages][2]: a page outside the pool
-  float* scales = reinterpret_cast<float*>(smem + kRingBytes + kCtlBytes);  // [kStages][K0 K1 V0 V1][64]
+  float* recv = reinterpret_cast<float*>(smem + kOffRecv);
+  float* scales = reinterpret_cast<float*>(smem + kOffScales);
+
+  if (kCluster) cluster_arrive();  // "this CTA runs": awaited before its peers' memory is written
 
   const int split = blockIdx.x;
   const int kh = blockIdx.y;
@@ -147,6 +159,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int lane = threadIdx.x & 31;
 
   const uint32_t pos = a.d_position[b];
+  if (threadIdx.x == 32 * kWarps) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&bars[i]), 1);
+      mbar_init(smem_u32(&bars[kStages + i]), kWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
   const bool pos_ok = pos < (uint32_t)a.max_seq;
   if (!pos_ok && split == 0 && kh == 0 && threadIdx.x == 0 && a.err)
     atomicCAS(a.err, 0, DEV_ERR_POSITION);
@@ -156,15 +178,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int nt = min(tps, list.n - t0);
   const int n_stages = (nt + kTiles - 1) / kTiles;
   const int64_t head0 = (int64_t)b * a.hq + (int64_t)kh * G;
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(smem_u32(&bars[i]), 1);
-      mbar_init(smem_u32(&bars[kStages + i]), 4);
-    }
-    *abort_flag = 0;
-    fence_mbar_init();
-  }
   __syncthreads();
 
   // Consumer state lives at function scope so it survives the CTA barrier
@@ -176,66 +189,76 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
   for (int mt = 0; mt < 8; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
 
-  if (warp == 4) {
+  if (warp == kWarps) {
     // ------------------------------------------------------------ producer
-    if (lane == 0 && nt > 0) {
-      prefetch_tmap(&tm_k);
-      prefetch_tmap(&tm_v);
-      int issued = 0;
-      for (int it = 0; it < n_stages; ++it) {
-        const int st = it % kStages;
-        const int r = it / kStages;
-        if (r > 0 && !mbar_wait(smem_u32(&bars[kStages + st]), (r - 1) & 1, a.err, 1, abort_flag))
-          break;
-        const int live = min(kTiles, nt - it * kTiles);
-        const uint32_t full = smem_u32(&bars[st]);
-        const uint32_t kb = smem_u32(smem + st * kStageBytes);
-        int row[kTiles], outer[kTiles];
-#pragma unroll
-        for (int x = 0; x < kTiles; ++x) {
-          if (x >= live) break;
-          row[x] = list.key0(t0 + it * kTiles + x);
-          outer[x] = b;  // sequence (contiguous caches) or page (paged pool)
-          int bad = 0;
+    // The warp looks 32 tiles up at once (a lane each), so that the loop over
+    // stages holds no division and no table load: issuing one stage must not
+    // take longer than consuming it.
+    int row_l = 0, outer_l = 0, bad_l = 0;  // of tile (it & ~31) + lane of the split
+    int it = 0, issued = 0;
+    for (int s = 0; s < n_stages; ++s) {
+      const int st = s % kStages;
+      if ((it & 31) == 0) {
+        bad_l = 0;
+        outer_l = b;  // sequence (contiguous caches) or page (paged pool)
+        if (it + lane < nt) {
+          row_l = list.key0(t0 + it + lane);
           if (kPaged) {
             // a 64-key tile never straddles a page (page_size % 64 == 0)
-            const int pg = row[x] / a.page_size;
-            outer[x] = __ldg(a.page_table + (int64_t)b * a.table_stride + pg);
-            row[x] -= pg * a.page_size;
-            if (outer[x] < 0 || outer[x] >= a.num_pages) {
+            const int pg = row_l / a.page_size;
+            outer_l = __ldg(a.page_table + (int64_t)b * a.table_stride + pg);
+            row_l -= pg * a.page_size;
+            if (outer_l < 0 || outer_l >= a.num_pages) {
               // load page 0 instead and leave the tile out of the softmax
               if (a.err) atomicCAS(a.err, 0, DEV_ERR_PAGE);
-              outer[x] = 0;
-              bad = 1;
+              outer_l = 0;
+              bad_l = 1;
             }
           }
-          bad_tile[st * 2 + x] = bad;
         }
+      }
+      const int live = min(kTiles, nt - it);
+      if (s >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars[kStages + st]),
+                                                             (s / kStages - 1) & 1, a.err, 1, abort_flag)))
+        break;
+      const uint32_t full = smem_u32(&bars[st]);
+      int row[kTiles], outer[kTiles];
+#pragma unroll
+      for (int x = 0; x < kTiles; ++x) {
+        row[x] = __shfl_sync(0xffffffffu, row_l, (it + x) & 31);
+        outer[x] = __shfl_sync(0xffffffffu, outer_l, (it + x) & 31);
+        const int bad = __shfl_sync(0xffffffffu, bad_l, (it + x) & 31);
+        if (lane == 0) bad_tile[st * 2 + x] = bad;
+      }
+      if (lane == 0)
         mbar_arrive_expect_tx(full, live * (2 * kTileBytes + (kFp8 ? 2 * kKeys * 4 : 0)));
+      __syncwarp();
+      // lane 0 loads K, lane 1 V, and each its tiles' 64 scales (256-byte
+      // aligned: row % 64 == 0)
+      if (lane < 2) {
+        const CUtensorMap* map = lane == 0 ? &tm_k : &tm_v;
+        const uint32_t dst = smem_u32(smem + st * kStageBytes + lane * kVOff);
 #pragma unroll
         for (int x = 0; x < kTiles; ++x) {
           if (x >= live) break;
-          const uint32_t kx = kb + x * kTileBytes, vx = kx + kVOff;
-          tma_load_4d(kx, &tm_k, full, 0, row[x], kh, outer[x]);
-          if (!kFp8) tma_load_4d(kx + kTileBytes / 2, &tm_k, full, 64, row[x], kh, outer[x]);
-          tma_load_4d(vx, &tm_v, full, 0, row[x], kh, outer[x]);
-          if (!kFp8) tma_load_4d(vx + kTileBytes / 2, &tm_v, full, 64, row[x], kh, outer[x]);
           if (kFp8) {
-            // 64 scales of a page row range: 256-byte aligned (row % 64 == 0)
             const int64_t off = ((int64_t)outer[x] * a.hkv + kh) * a.page_size + row[x];
-            const uint32_t sb = smem_u32(scales + st * kScaleFloats + x * kKeys);
-            bulk_load(sb, a.k_scales + off, kKeys * 4, full);
-            bulk_load(sb + 2 * kKeys * 4, a.v_scales + off, kKeys * 4, full);
+            bulk_load(smem_u32(scales + st * kScaleFloats + (2 * lane + x) * kKeys),
+                      (lane == 0 ? a.k_scales : a.v_scales) + off, kKeys * 4, full);
+            tma_load_4d(dst + x * kTileBytes, map, full, 0, row[x], kh, outer[x]);
+          } else {
+            tma_load_5d(dst, map, full, 0, row[x], 0, kh, outer[x]);
           }
         }
-        issued = it + 1;
       }
-      // a wait gave up: let the copies in flight land before the CTA leaves
-      if (*abort_flag)
-        for (int it = max(0, issued - kStages); it < issued; ++it)
-          for (int i = 0; i < (1 << 20); ++i)
-            if (mbar_try_wait(smem_u32(&bars[it % kStages]), (it / kStages) & 1)) break;
+      it += live;
+      issued = s + 1;
     }
+    // a wait gave up: let the copies in flight land before the CTA leaves
+    if (*abort_flag)
+      for (int s = max(0, issued - kStages); s < issued; ++s)
+        for (int n = 0; n < (1 << 20); ++n)
+          if (mbar_try_wait(smem_u32(&bars[s % kStages]), (s / kStages) & 1)) break;
   } else {
     // ----------------------------------------------------------- consumers
     // B operand of the QK product: an 8-bit row delivers 4 neighbouring dims
@@ -253,166 +276,138 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     const float sl2 = a.scale_log2;
-    const int a_row = 16 * warp + (lane & 7) + ((lane >> 3) & 1) * 8;
+    const int x = warp >> 2;          // this warp's tile of a stage (0 for f16)
+    const int k16 = 16 * (warp & 3);  // its keys of that tile
+    const int a_row = k16 + (lane & 7) + ((lane >> 3) & 1) * 8;
     const int a_chs = lane >> 4;
-    const int v_row = 16 * warp + (lane & 7) + ((lane >> 4) & 1) * 8;
+    const int v_row = k16 + (lane & 7) + ((lane >> 4) & 1) * 8;
     const int v_chs = (lane >> 3) & 1;
 
-    for (int it = 0; it < n_stages; ++it) {
-      const int st = it % kStages;
-      if (!mbar_wait(smem_u32(&bars[st]), (it / kStages) & 1, a.err, 2, abort_flag)) break;
-      const uint32_t kb = smem_u32(smem + st * kStageBytes);
+    for (int s = 0; s < n_stages; ++s) {
+      const int st = s % kStages;
+      if (!mbar_wait(smem_u32(&bars[st]), (s / kStages) & 1, a.err, 2, abort_flag)) break;
+      const int it = s * kTiles + x;
+      if (it >= nt) break;  // the last stage holds one tile
+      const uint32_t kb = smem_u32(smem + st * kStageBytes) + x * kTileBytes;
       const uint32_t vb = kb + kVOff;
-      const float* sc_st = scales + st * kScaleFloats;
 
-      // Scores of this warp's 16 keys of each tile: x = tile; [0],[1] key g
-      // (heads 2t, 2t+1); [2],[3] key g+8.
-      float s[kTiles][4], inv_vs[kTiles][2];
-      bool masked = false;
-      uint32_t keep[kTiles][2];  // V halves to keep: keys 2t, 2t+1 / 2t+8, 2t+9
+      // Scores: [0],[1] key g (heads 2t, 2t+1); [2],[3] key g+8.  Two chains of
+      // four products each.
+      float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
+      if (kFp8) {
 #pragma unroll
-      for (int x = 0; x < kTiles; ++x) {
-        float sc[4] = {0.f, 0.f, 0.f, 0.f};
-        if (kFp8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = 2 * i + a_chs;
-            const uint32_t addr = kb + x * kTileBytes + a_row * 128 + ((c ^ (a_row & 7)) << 4);
-            uint32_t r0, r1, r2, r3;
-            ldsm_x4(addr, r0, r1, r2, r3);
-            mma16816(sc, f16x2_of_e4m3x2(r0), f16x2_of_e4m3x2(r1), f16x2_of_e4m3x2(r0 >> 16),
-                     f16x2_of_e4m3x2(r1 >> 16), qb[2 * i][0], qb[2 * i][1]);
-            mma16816(sc, f16x2_of_e4m3x2(r2), f16x2_of_e4m3x2(r3), f16x2_of_e4m3x2(r2 >> 16),
-                     f16x2_of_e4m3x2(r3 >> 16), qb[2 * i + 1][0], qb[2 * i + 1][1]);
-          }
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const int c = 2 * kk + a_chs;
-            const uint32_t addr =
-                kb + (c >> 3) * (kTileBytes / 2) + a_row * 128 + (((c & 7) ^ (a_row & 7)) << 4);
-            uint32_t a0, a1, a2, a3;
-            ldsm_x4(addr, a0, a1, a2, a3);
-            mma16816(sc, a0, a1, a2, a3, qb[kk][0], qb[kk][1]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int c = 2 * i + a_chs;
+          const uint32_t addr = kb + a_row * 128 + ((c ^ (a_row & 7)) << 4);
+          uint32_t r0, r1, r2, r3;
+          ldsm_x4(addr, r0, r1, r2, r3);
+          mma16816(sc, f16x2_of_e4m3x2(r0), f16x2_of_e4m3x2(r1), f16x2_of_e4m3x2(r0 >> 16),
+                   f16x2_of_e4m3x2(r1 >> 16), qb[2 * i][0], qb[2 * i][1]);
+          mma16816(sd, f16x2_of_e4m3x2(r2), f16x2_of_e4m3x2(r3), f16x2_of_e4m3x2(r2 >> 16),
+                   f16x2_of_e4m3x2(r3 >> 16), qb[2 * i + 1][0], qb[2 * i + 1][1]);
         }
-        const bool there = it * kTiles + x < nt;
-        const int kbase = there ? list.key0(t0 + it * kTiles + x) + 16 * warp : 0;
-        const bool none = !there || (kPaged && bad_tile[st * 2 + x]);
-        const bool part = none || list.partial(kbase);
-        masked |= part;
-        float f0 = sl2, f1 = sl2, lv0 = 0.f, lv1 = 0.f;
-        inv_vs[x][0] = inv_vs[x][1] = 1.f;
-        if (kFp8) {
-          const int i0 = x * kKeys + 16 * warp + g;
-          f0 *= sc_st[i0];
-          f1 *= sc_st[i0 + 8];
-          // a zero row (scale 0) has zero codes: any positive scale serves
-          const float v0 = fmaxf(sc_st[2 * kKeys + i0], 0x1p-60f);
-          const float v1 = fmaxf(sc_st[2 * kKeys + i0 + 8], 0x1p-60f);
-          lv0 = __log2f(v0);
-          lv1 = __log2f(v1);
-          inv_vs[x][0] = __fdividef(1.f, v0);
-          inv_vs[x][1] = __fdividef(1.f, v1);
-        }
-        s[x][0] = fmaf(sc[0], f0, lv0);
-        s[x][1] = fmaf(sc[1], f0, lv0);
-        s[x][2] = fmaf(sc[2], f1, lv1);
-        s[x][3] = fmaf(sc[3], f1, lv1);
-        if (part) {
-          const bool k0 = !none && list.sees(kbase + g), k1 = !none && list.sees(kbase + g + 8);
-          if (!k0) {
-            s[x][0] = s[x][1] = -INFINITY;
-            inv_vs[x][0] = 1.f;
-          }
-          if (!k1) {
-            s[x][2] = s[x][3] = -INFINITY;
-            inv_vs[x][1] = 1.f;
-          }
-          const int q = kbase + 2 * t;
-          keep[x][0] = none ? 0u : (list.sees(q) ? 0xFFFFu : 0u) | (list.sees(q + 1) ? 0xFFFF0000u : 0u);
-          keep[x][1] = none ? 0u : (list.sees(q + 8) ? 0xFFFFu : 0u) | (list.sees(q + 9) ? 0xFFFF0000u : 0u);
-        } else {
-          keep[x][0] = keep[x][1] = 0xFFFFFFFFu;
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const int c = 2 * kk + a_chs;
+          const uint32_t addr =
+              kb + (c >> 3) * (kTileBytes / 2) + a_row * 128 + (((c & 7) ^ (a_row & 7)) << 4);
+          uint32_t a0, a1, a2, a3;
+          ldsm_x4(addr, a0, a1, a2, a3);
+          mma16816(kk & 1 ? sd : sc, a0, a1, a2, a3, qb[kk][0], qb[kk][1]);
         }
       }
-      float mx0 = fmaxf(s[0][0], s[0][2]), mx1 = fmaxf(s[0][1], s[0][3]);
-      if (kTiles == 2) {
-        mx0 = fmaxf(mx0, fmaxf(s[kTiles - 1][0], s[kTiles - 1][2]));
-        mx1 = fmaxf(mx1, fmaxf(s[kTiles - 1][1], s[kTiles - 1][3]));
+      const int kbase = list.key0(t0 + it) + k16;
+      const bool none = kPaged && bad_tile[st * 2 + x];
+      const bool part = none || list.partial(kbase);
+      float f0 = sl2, f1 = sl2, lv0 = 0.f, lv1 = 0.f, iv0 = 1.f, iv1 = 1.f;
+      if (kFp8) {
+        const float* sp = scales + st * kScaleFloats + x * kKeys + k16 + g;
+        f0 *= sp[0];
+        f1 *= sp[8];
+        // a zero row (scale 0) has zero codes: any positive scale serves
+        const float v0 = fmaxf(sp[2 * kKeys], 0x1p-60f), v1 = fmaxf(sp[2 * kKeys + 8], 0x1p-60f);
+        lv0 = __log2f(v0);
+        lv1 = __log2f(v1);
+        iv0 = __fdividef(1.f, v0);
+        iv1 = __fdividef(1.f, v1);
       }
+      float s0 = fmaf(sc[0] + sd[0], f0, lv0), s1 = fmaf(sc[1] + sd[1], f0, lv0);
+      float s2 = fmaf(sc[2] + sd[2], f1, lv1), s3 = fmaf(sc[3] + sd[3], f1, lv1);
+      uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;  // V halves: keys 2t, 2t+1 / 2t+8, 2t+9
+      if (part) {
+        if (none || !list.sees(kbase + g)) s0 = s1 = -INFINITY, iv0 = 1.f;
+        if (none || !list.sees(kbase + g + 8)) s2 = s3 = -INFINITY, iv1 = 1.f;
+        const int q = kbase + 2 * t;
+        keep0 = none ? 0u : (list.sees(q) ? 0xFFFFu : 0u) | (list.sees(q + 1) ? 0xFFFF0000u : 0u);
+        keep1 = none ? 0u : (list.sees(q + 8) ? 0xFFFFu : 0u) | (list.sees(q + 9) ? 0xFFFF0000u : 0u);
+      }
+      float mx0 = fmaxf(s0, s2), mx1 = fmaxf(s1, s3);
 #pragma unroll
       for (int off = 4; off <= 16; off <<= 1) {
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
       }
-      const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-      const float al0 = ex2(m0 - mn0), al1 = ex2(m1 - mn1);
-      l0 *= al0;
-      l1 *= al1;
-      m0 = mn0;
-      m1 = mn1;
+      if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
+        const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+        const float al0 = ex2(m0 - mn0), al1 = ex2(m1 - mn1);
+        l0 *= al0;
+        l1 *= al1;
+        m0 = mn0;
+        m1 = mn1;
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        o[mt][0] *= al0;
-        o[mt][1] *= al1;
-        o[mt][2] *= al0;
-        o[mt][3] *= al1;
-      }
-#pragma unroll
-      for (int x = 0; x < kTiles; ++x) {
-        const float p0 = ex2(s[x][0] - mn0), p1 = ex2(s[x][1] - mn1);
-        const float p2 = ex2(s[x][2] - mn0), p3 = ex2(s[x][3] - mn1);
-        if (kFp8) {
-          l0 += p0 * inv_vs[x][0] + p2 * inv_vs[x][1];
-          l1 += p1 * inv_vs[x][0] + p3 * inv_vs[x][1];
-        } else {
-          l0 += p0 + p2;
-          l1 += p1 + p3;
+        for (int mt = 0; mt < 8; ++mt) {
+          o[mt][0] *= al0;
+          o[mt][1] *= al1;
+          o[mt][2] *= al0;
+          o[mt][3] *= al1;
         }
-        const uint32_t pb0 = movm_t(pack_half2(p0, p1));
-        const uint32_t pb1 = movm_t(pack_half2(p2, p3));
-        const uint32_t z0 = keep[x][0], z1 = keep[x][1];
-        if (kFp8) {
-          // A byte pair of the transposed load is (dim 2g, dim 2g+1) of keys
-          // 2t and 2t+1: MMA rows g and g+8 stand for dims 2g and 2g+1.
+      }
+      const float p0 = ex2(s0 - m0), p1 = ex2(s1 - m1);
+      const float p2 = ex2(s2 - m0), p3 = ex2(s3 - m1);
+      l0 += kFp8 ? p0 * iv0 + p2 * iv1 : p0 + p2;
+      l1 += kFp8 ? p1 * iv0 + p3 * iv1 : p1 + p3;
+      const uint32_t pb0 = movm_t(pack_half2(p0, p1));
+      const uint32_t pb1 = movm_t(pack_half2(p2, p3));
+      if (kFp8) {
+        // A byte pair of the transposed load is (dim 2g, dim 2g+1) of keys 2t
+        // and 2t+1: MMA rows g and g+8 stand for dims 2g and 2g+1.
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = 2 * i + a_chs;
-            const uint32_t addr = vb + x * kTileBytes + a_row * 128 + ((c ^ (a_row & 7)) << 4);
-            uint32_t r[4];
-            ldsm_x4_t(addr, r[0], r[1], r[2], r[3]);
+        for (int i = 0; i < 4; ++i) {
+          const int c = 2 * i + a_chs;
+          const uint32_t addr = vb + a_row * 128 + ((c ^ (a_row & 7)) << 4);
+          uint32_t r[4];
+          ldsm_x4_t(addr, r[0], r[1], r[2], r[3]);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) r[q] = __byte_perm(r[q], 0u, 0x3120);
+          for (int q = 0; q < 4; ++q) r[q] = __byte_perm(r[q], 0u, 0x3120);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t a0 = f16x2_of_e4m3x2(r[2 * h]), a1 = f16x2_of_e4m3x2(r[2 * h] >> 16);
-              uint32_t a2 = f16x2_of_e4m3x2(r[2 * h + 1]), a3 = f16x2_of_e4m3x2(r[2 * h + 1] >> 16);
-              if (masked) {
-                a0 &= z0;
-                a1 &= z0;
-                a2 &= z1;
-                a3 &= z1;
-              }
-              mma16816(o[2 * i + h], a0, a1, a2, a3, pb0, pb1);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t a0 = f16x2_of_e4m3x2(r[2 * h]), a1 = f16x2_of_e4m3x2(r[2 * h] >> 16);
+            uint32_t a2 = f16x2_of_e4m3x2(r[2 * h + 1]), a3 = f16x2_of_e4m3x2(r[2 * h + 1] >> 16);
+            if (part) {
+              a0 &= keep0;
+              a1 &= keep0;
+              a2 &= keep1;
+              a3 &= keep1;
             }
+            mma16816(o[2 * i + h], a0, a1, a2, a3, pb0, pb1);
           }
-        } else {
+        }
+      } else {
 #pragma unroll
-          for (int mt = 0; mt < 8; ++mt) {
-            const int c = 2 * mt + v_chs;
-            const uint32_t addr =
-                vb + (c >> 3) * (kTileBytes / 2) + v_row * 128 + (((c & 7) ^ (v_row & 7)) << 4);
-            uint32_t a0, a1, a2, a3;
-            ldsm_x4_t(addr, a0, a1, a2, a3);
-            if (masked) {
-              a0 &= z0;
-              a1 &= z0;
-              a2 &= z1;
-              a3 &= z1;
-            }
-            mma16816(o[mt], a0, a1, a2, a3, pb0, pb1);
+        for (int mt = 0; mt < 8; ++mt) {
+          const int c = 2 * mt + v_chs;
+          const uint32_t addr =
+              vb + (c >> 3) * (kTileBytes / 2) + v_row * 128 + (((c & 7) ^ (v_row & 7)) << 4);
+          uint32_t a0, a1, a2, a3;
+          ldsm_x4_t(addr, a0, a1, a2, a3);
+          if (part) {
+            a0 &= keep0;
+            a1 &= keep0;
+            a2 &= keep1;
+            a3 &= keep1;
           }
+          mma16816(o[mt], a0, a1, a2, a3, pb0, pb1);
         }
       }
       __syncwarp();
@@ -430,8 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool valid = nt > 0 && !*abort_flag;
 
   RedSmem* red = reinterpret_cast<RedSmem*>(smem);
-  FinSmem* fin = reinterpret_cast<FinSmem*>(smem + kFinOffset);
-  if (valid && warp < 4) {
+  if (valid && warp < kWarps) {
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
       const int d0 = 16 * mt + (kFp8 ? 2 * g : g), d1 = d0 + (kFp8 ? 1 : 8);
@@ -447,18 +441,19 @@ __global__ void __launch_bounds__(kThreads, 2)
       red->l[warp][2 * t + 1] = l1;
     }
   }
+  if (kCluster) cluster_wait();  // every CTA of the cluster runs
   __syncthreads();
-  if (threadIdx.x < 128) {
-    const int d = threadIdx.x;
-    for (int hd = 0; hd < G; ++hd) {
+  if (warp < kWarps) {
+    const int d = threadIdx.x & 127;
+    for (int hd = threadIdx.x >> 7; hd < G; hd += kWarps / 4) {
       float res = 0.f, lse = -INFINITY;
       if (valid) {
         float M = red->m[0][hd];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) M = fmaxf(M, red->m[w][hd]);
+        for (int w = 1; w < kWarps; ++w) M = fmaxf(M, red->m[w][hd]);
         float L = 0.f, O = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
           const float sc = ex2(red->m[w][hd] - M);
           L += red->l[w][hd] * sc;
           O += red->o[w][d][hd] * sc;
@@ -471,30 +466,31 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (a.nks == 1) {
         if (valid || !pos_ok) a.out[(head0 + hd) * 128 + d] = __float2half_rn(res);
       } else if (kCluster) {
-        fin->o[hd][d] = res;
-        if (d == 0) fin->lse[hd] = lse;
+        const int row = hd / a.nks * a.nks + split;
+        const uint32_t owner = hd % a.nks;
+        st_dsmem_f32(recv + row * 128 + d, owner, res);
+        if (d == 0) st_dsmem_f32(recv + kRecvRows * 128 + row, owner, lse);
       } else {
         a.part_o[((head0 + hd) * a.nks + split) * 128 + d] = res;
         if (d == 0) a.part_lse[(head0 + hd) * a.nks + split] = lse;
       }
     }
   }
-  if (kCluster && a.nks > 1) {
-    // Every CTA of the cluster reaches both barriers (no early exit above),
-    // so the cluster cannot deadlock; the second keeps each CTA's shared
-    // memory alive until the others have read it.
-    cluster_sync_all();
-    const uint32_t me = cluster_ctarank();
+  if (kCluster) {
+    // Every CTA of the cluster reaches both barriers (no early exit above);
+    // after this one nobody touches a peer's memory.
+    cluster_arrive();
+    cluster_wait();
     if (threadIdx.x < 128) {
       const int d = threadIdx.x;
-      for (int hd = (int)me; hd < G; hd += a.nks) {
+      for (int hd = (int)cluster_ctarank(); hd < G; hd += a.nks) {
+        const float* po = recv + hd / a.nks * a.nks * 128 + d;
+        const float* lse = recv + kRecvRows * 128 + hd / a.nks * a.nks;
         a.out[(head0 + hd) * 128 + d] = merge_splits(a.nks, [&](int s, bool want_lse) {
-          return want_lse ? ld_dsmem_f32(&fin->lse[hd], (uint32_t)s)
-                          : ld_dsmem_f32(&fin->o[hd][d], (uint32_t)s);
+          return want_lse ? lse[s] : po[s * 128];
         });
       }
     }
-    cluster_sync_all();
   }
 }
 
@@ -524,7 +520,7 @@ cudaError_t launch_split(const DecodeWindowArgs& a, const CUtensorMap& tm_k,
                          const CUtensorMap& tm_v, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.nks, a.hkv, a.batch);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(threads(kFp8), 1, 1);
   cfg.dynamicSmemBytes = kFp8 ? kSmemFp8 : kSmemF16;
   cfg.stream = s;
   cudaLaunchAttribute at[1];

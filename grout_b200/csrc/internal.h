@@ -183,8 +183,9 @@ struct DecodeWindowArgs {
   int32_t page_size;
   int32_t num_pages;
 };
-// tm_k / tm_v: f16 as launch_decode; 8-bit {128, page_size, hkv, num_pages}
-// bytes, box {128, 64, 1, 1}, 128B swizzle.
+// tm_k / tm_v: f16 {64, rows, 2, hkv, batch or pages} (the third dimension a
+// row's two halves), box {64, 64, 2, 1, 1}; 8-bit {128, page_size, hkv,
+// num_pages} bytes, box {128, 64, 1, 1}; 128B swizzle.
 cudaError_t launch_decode_window(const DecodeWindowArgs& a, const CUtensorMap& tm_k,
                                  const CUtensorMap& tm_v, cudaStream_t s);
 cudaError_t decode_window_set_attributes();

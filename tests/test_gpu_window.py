@@ -70,8 +70,9 @@ def test_decode_paged(grout, page_size, window, sinks, splits):
         check(out[b:b + 1], ref, bound)
 
 
-def test_decode_of_a_full_window_is_close_to_plain_decode(grout):
-    """A window at least as long as the context sees every key."""
+def test_decode_of_a_full_window_agrees_with_plain_decode(grout):
+    """A window at least as long as the context sees every key: both kernels
+    (which sum in different orders) are within the bound of the same result."""
     B, hq, hkv, n = 3, 32, 8, 900
     q = normal(7, B, hq, D).half()
     k, v = _caches(B, hkv, n, 30)
@@ -79,7 +80,12 @@ def test_decode_of_a_full_window_is_close_to_plain_decode(grout):
     a, b = torch.empty_like(q), torch.empty_like(q)
     grout.attention_decode(q, k, v, pos, a, n, num_splits=2)
     grout.attention_decode_window(q, k, v, pos, b, n, 900, 0, num_splits=2)
-    assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    for i in range(B):
+        ref, bound = attention64(q[i:i + 1], k[i].transpose(0, 1), v[i].transpose(0, 1), pos[i:i + 1].long(), 0, 0, SCALE_F16)
+        check(a[i:i + 1], ref, bound)
+        check(b[i:i + 1], ref, bound)
 
 
 def test_decode_errors_on_the_device(grout):
