@@ -18,12 +18,14 @@
 // and l sums w / vs = 2^(s - m) in f32.  Codes become f16 exactly.
 //
 // HBM-bound; one CTA per split, KV head and sequence.  A producer warp fills a
-// 96 KB TMA ring of three stages, each 64 f16 keys or 128 8-bit ones (two
-// 64-key tiles, which need not be neighbours); every consumer warp takes 16
-// keys of each stage, four warps for f16 and eight for 8-bit keys, whose
-// conversion makes the chain through a stage longer than its share of the
-// memory time.  S^T = K Q^T and O^T += V^T P^T run on mma.sync m16n8k16 with
-// the GQA group on the 8-wide N side, as in decode.cu.
+// 96 KB TMA ring with 64-key tiles, three of f16 or six of 8-bit keys; a
+// group of four consumer warps takes a tile, each warp 16 of its keys.  f16
+// tiles have one group; 8-bit tiles, which take as long to consume and half as
+// long to load, have two that take turns.  (A stage of the ring always belongs
+// to the same group: a group that skipped phases of a stage's barrier could
+// take an older phase of the same parity for its own.)  S^T = K Q^T and
+// O^T += V^T P^T run on mma.sync m16n8k16 with the GQA group on the 8-wide N
+// side, as in decode.cu.
 // The warps merge through shared memory.  Up to 16 splits form a thread-block
 // cluster: each CTA pushes its heads' results into the shared memory of the
 // CTA that owns the head (no round trip, one barrier), which writes the row;
@@ -43,10 +45,8 @@ namespace grout {
 namespace {
 
 constexpr int kKeys = 64;  // keys per tile
-constexpr int kStages = 3;
-constexpr int kStageBytes = 32768;  // K and V of one f16 tile, or of two 8-bit ones
-constexpr int kRingBytes = kStages * kStageBytes;
-constexpr int kScaleFloats = 4 * kKeys;  // per stage: K scales of both tiles, V scales of both
+constexpr int kRingBytes = 98304;
+constexpr int kMaxStages = 6;
 // Consumer warps; one more produces.
 __host__ __device__ constexpr int consumers(bool fp8) { return fp8 ? 8 : 4; }
 __host__ __device__ constexpr int threads(bool fp8) { return 32 * (consumers(fp8) + 1); }
@@ -58,9 +58,9 @@ constexpr int kRecvRows = 16;
 constexpr int kRecvBytes = kRecvRows * (128 + 1) * 4;
 constexpr int kOffCtl = kRingBytes;
 constexpr int kOffRecv = kOffCtl + kCtlBytes;
-constexpr int kOffScales = kOffRecv + kRecvBytes;  // 8-bit: [stage][K0 K1 V0 V1][64]
+constexpr int kOffScales = kOffRecv + kRecvBytes;  // 8-bit: [stage][K, V][64]
 constexpr int kSmemF16 = kOffScales + 1024;
-constexpr int kSmemFp8 = kSmemF16 + kStages * kScaleFloats * 4;
+constexpr int kSmemFp8 = kSmemF16 + kMaxStages * 2 * kKeys * 4;
 
 struct RedSmem {
   float o[8][128][9];  // [warp]; padded: the per-dimension merge reads are conflict-free
@@ -136,16 +136,18 @@ template <bool kFp8, bool kPaged, bool kCluster>
 __global__ void __launch_bounds__(threads(kFp8), 2)
     decode_window_kernel(const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const DecodeWindowArgs a) {
-  constexpr int kTiles = kFp8 ? 2 : 1;  // 64-key tiles per stage
-  constexpr int kTileBytes = kKeys * 128 * (kFp8 ? 1 : 2);
-  constexpr int kVOff = kTiles * kTileBytes;  // V tiles follow the K tiles
+  constexpr int kTileBytes = kKeys * 128 * (kFp8 ? 1 : 2);  // of K; as much of V follows
+  constexpr int kStageBytes = 2 * kTileBytes;
+  constexpr int kStages = kRingBytes / kStageBytes;
   constexpr int kWarps = consumers(kFp8);
+  constexpr int kGroups = kWarps / 4;
+  static_assert(kStages % kGroups == 0, "a stage belongs to one group");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffCtl);  // full[kStages], empty[kStages]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * kStages);
-  volatile int* bad_tile = abort_flag + 1;  // [kStages][2]: a page outside the pool
+  volatile int* bad_tile = abort_flag + 1;  // [kStages]: a page outside the pool
   float* recv = reinterpret_cast<float*>(smem + kOffRecv);
   float* scales = reinterpret_cast<float*>(smem + kOffScales);
 
@@ -164,7 +166,7 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
     prefetch_tmap(&tm_v);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&bars[i]), 1);
-      mbar_init(smem_u32(&bars[kStages + i]), kWarps);
+      mbar_init(smem_u32(&bars[kStages + i]), 4);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -176,7 +178,6 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
   const int tps = (list.n + a.nks - 1) / a.nks;
   const int t0 = min(split * tps, list.n);
   const int nt = min(tps, list.n - t0);
-  const int n_stages = (nt + kTiles - 1) / kTiles;
   const int64_t head0 = (int64_t)b * a.hq + (int64_t)kh * G;
   __syncthreads();
 
@@ -195,9 +196,9 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
     // stages holds no division and no table load: issuing one stage must not
     // take longer than consuming it.
     int row_l = 0, outer_l = 0, bad_l = 0;  // of tile (it & ~31) + lane of the split
-    int it = 0, issued = 0;
-    for (int s = 0; s < n_stages; ++s) {
-      const int st = s % kStages;
+    int it = 0;
+    for (; it < nt; ++it) {
+      const int st = it % kStages;
       if ((it & 31) == 0) {
         bad_l = 0;
         outer_l = b;  // sequence (contiguous caches) or page (paged pool)
@@ -217,48 +218,38 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
           }
         }
       }
-      const int live = min(kTiles, nt - it);
-      if (s >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars[kStages + st]),
-                                                             (s / kStages - 1) & 1, a.err, 1, abort_flag)))
+      const int row = __shfl_sync(0xffffffffu, row_l, it & 31);
+      const int outer = __shfl_sync(0xffffffffu, outer_l, it & 31);
+      const int bad = __shfl_sync(0xffffffffu, bad_l, it & 31);
+      if (it >= kStages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars[kStages + st]),
+                                                              (it / kStages - 1) & 1, a.err, 1, abort_flag)))
         break;
       const uint32_t full = smem_u32(&bars[st]);
-      int row[kTiles], outer[kTiles];
-#pragma unroll
-      for (int x = 0; x < kTiles; ++x) {
-        row[x] = __shfl_sync(0xffffffffu, row_l, (it + x) & 31);
-        outer[x] = __shfl_sync(0xffffffffu, outer_l, (it + x) & 31);
-        const int bad = __shfl_sync(0xffffffffu, bad_l, (it + x) & 31);
-        if (lane == 0) bad_tile[st * 2 + x] = bad;
+      if (lane == 0) {
+        bad_tile[st] = bad;
+        mbar_arrive_expect_tx(full, kStageBytes + (kFp8 ? 2 * kKeys * 4 : 0));
       }
-      if (lane == 0)
-        mbar_arrive_expect_tx(full, live * (2 * kTileBytes + (kFp8 ? 2 * kKeys * 4 : 0)));
       __syncwarp();
-      // lane 0 loads K, lane 1 V, and each its tiles' 64 scales (256-byte
+      // lane 0 loads K, lane 1 V, and each its tile's 64 scales (256-byte
       // aligned: row % 64 == 0)
       if (lane < 2) {
         const CUtensorMap* map = lane == 0 ? &tm_k : &tm_v;
-        const uint32_t dst = smem_u32(smem + st * kStageBytes + lane * kVOff);
-#pragma unroll
-        for (int x = 0; x < kTiles; ++x) {
-          if (x >= live) break;
-          if (kFp8) {
-            const int64_t off = ((int64_t)outer[x] * a.hkv + kh) * a.page_size + row[x];
-            bulk_load(smem_u32(scales + st * kScaleFloats + (2 * lane + x) * kKeys),
-                      (lane == 0 ? a.k_scales : a.v_scales) + off, kKeys * 4, full);
-            tma_load_4d(dst + x * kTileBytes, map, full, 0, row[x], kh, outer[x]);
-          } else {
-            tma_load_5d(dst, map, full, 0, row[x], 0, kh, outer[x]);
-          }
+        const uint32_t dst = smem_u32(smem + st * kStageBytes + lane * kTileBytes);
+        if (kFp8) {
+          const int64_t off = ((int64_t)outer * a.hkv + kh) * a.page_size + row;
+          bulk_load(smem_u32(scales + (2 * st + lane) * kKeys),
+                    (lane == 0 ? a.k_scales : a.v_scales) + off, kKeys * 4, full);
+          tma_load_4d(dst, map, full, 0, row, kh, outer);
+        } else {
+          tma_load_5d(dst, map, full, 0, row, 0, kh, outer);
         }
       }
-      it += live;
-      issued = s + 1;
     }
     // a wait gave up: let the copies in flight land before the CTA leaves
     if (*abort_flag)
-      for (int s = max(0, issued - kStages); s < issued; ++s)
+      for (int i = max(0, it - kStages); i < it; ++i)
         for (int n = 0; n < (1 << 20); ++n)
-          if (mbar_try_wait(smem_u32(&bars[s % kStages]), (s / kStages) & 1)) break;
+          if (mbar_try_wait(smem_u32(&bars[i % kStages]), (i / kStages) & 1)) break;
   } else {
     // ----------------------------------------------------------- consumers
     // B operand of the QK product: an 8-bit row delivers 4 neighbouring dims
@@ -276,57 +267,66 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
       }
     }
     const float sl2 = a.scale_log2;
-    const int x = warp >> 2;          // this warp's tile of a stage (0 for f16)
-    const int k16 = 16 * (warp & 3);  // its keys of that tile
+    const int k16 = 16 * (warp & 3);  // this warp's keys of a tile
     const int a_row = k16 + (lane & 7) + ((lane >> 3) & 1) * 8;
     const int a_chs = lane >> 4;
     const int v_row = k16 + (lane & 7) + ((lane >> 4) & 1) * 8;
     const int v_chs = (lane >> 3) & 1;
 
-    for (int s = 0; s < n_stages; ++s) {
-      const int st = s % kStages;
-      if (!mbar_wait(smem_u32(&bars[st]), (s / kStages) & 1, a.err, 2, abort_flag)) break;
-      const int it = s * kTiles + x;
-      if (it >= nt) break;  // the last stage holds one tile
-      const uint32_t kb = smem_u32(smem + st * kStageBytes) + x * kTileBytes;
-      const uint32_t vb = kb + kVOff;
+    for (int it = warp >> 2; it < nt; it += kGroups) {
+      const int st = it % kStages;
+      if (!mbar_wait(smem_u32(&bars[st]), (it / kStages) & 1, a.err, 2, abort_flag)) break;
+      const uint32_t kb = smem_u32(smem + st * kStageBytes);
+      const uint32_t vb = kb + kTileBytes;
 
-      // Scores: [0],[1] key g (heads 2t, 2t+1); [2],[3] key g+8.  Two chains of
-      // four products each.
-      float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
+      // Every load of the tile first: each waited for where it is used would
+      // put its latency into the chain (K, then V while the scores are made).
+      float f0 = sl2, f1 = sl2, v0 = 1.f, v1 = 1.f;
       if (kFp8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = 2 * i + a_chs;
-          const uint32_t addr = kb + a_row * 128 + ((c ^ (a_row & 7)) << 4);
-          uint32_t r0, r1, r2, r3;
-          ldsm_x4(addr, r0, r1, r2, r3);
-          mma16816(sc, f16x2_of_e4m3x2(r0), f16x2_of_e4m3x2(r1), f16x2_of_e4m3x2(r0 >> 16),
-                   f16x2_of_e4m3x2(r1 >> 16), qb[2 * i][0], qb[2 * i][1]);
-          mma16816(sd, f16x2_of_e4m3x2(r2), f16x2_of_e4m3x2(r3), f16x2_of_e4m3x2(r2 >> 16),
-                   f16x2_of_e4m3x2(r3 >> 16), qb[2 * i + 1][0], qb[2 * i + 1][1]);
-        }
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const int c = 2 * kk + a_chs;
-          const uint32_t addr =
-              kb + (c >> 3) * (kTileBytes / 2) + a_row * 128 + (((c & 7) ^ (a_row & 7)) << 4);
-          uint32_t a0, a1, a2, a3;
-          ldsm_x4(addr, a0, a1, a2, a3);
-          mma16816(kk & 1 ? sd : sc, a0, a1, a2, a3, qb[kk][0], qb[kk][1]);
-        }
-      }
-      const int kbase = list.key0(t0 + it) + k16;
-      const bool none = kPaged && bad_tile[st * 2 + x];
-      const bool part = none || list.partial(kbase);
-      float f0 = sl2, f1 = sl2, lv0 = 0.f, lv1 = 0.f, iv0 = 1.f, iv1 = 1.f;
-      if (kFp8) {
-        const float* sp = scales + st * kScaleFloats + x * kKeys + k16 + g;
+        const float* sp = scales + 2 * st * kKeys + k16 + g;
         f0 *= sp[0];
         f1 *= sp[8];
         // a zero row (scale 0) has zero codes: any positive scale serves
-        const float v0 = fmaxf(sp[2 * kKeys], 0x1p-60f), v1 = fmaxf(sp[2 * kKeys + 8], 0x1p-60f);
+        v0 = fmaxf(sp[kKeys], 0x1p-60f);
+        v1 = fmaxf(sp[kKeys + 8], 0x1p-60f);
+      }
+      constexpr int kFrag = kFp8 ? 4 : 8;
+      uint32_t kf[kFrag][4], vf[kFrag][4];
+#pragma unroll
+      for (int i = 0; i < kFrag; ++i) {
+        const int c = 2 * i + a_chs;
+        const uint32_t addr = kb + (kFp8 ? 0 : (c >> 3) * (kTileBytes / 2)) + a_row * 128 + (((c & 7) ^ (a_row & 7)) << 4);
+        ldsm_x4(addr, kf[i][0], kf[i][1], kf[i][2], kf[i][3]);
+      }
+#pragma unroll
+      for (int i = 0; i < kFrag; ++i) {
+        // f16: the transposed tile's keys on the MMA's k side; 8-bit: as K
+        const int row = kFp8 ? a_row : v_row, c = 2 * i + (kFp8 ? a_chs : v_chs);
+        const uint32_t addr = vb + (kFp8 ? 0 : (c >> 3) * (kTileBytes / 2)) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        ldsm_x4_t(addr, vf[i][0], vf[i][1], vf[i][2], vf[i][3]);
+      }
+      const bool none = kPaged && bad_tile[st];
+      __syncwarp();  // the tile is in registers: its stage can be filled again
+      if (lane == 0) mbar_arrive(smem_u32(&bars[kStages + st]));
+      // Scores: [0],[1] key g (heads 2t, 2t+1); [2],[3] key g+8.  Two chains of
+      // four products each.
+      float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kFrag; ++i) {
+        const uint32_t(&r)[4] = kf[i];
+        if (kFp8) {
+          mma16816(sc, f16x2_of_e4m3x2(r[0]), f16x2_of_e4m3x2(r[1]), f16x2_of_e4m3x2(r[0] >> 16),
+                   f16x2_of_e4m3x2(r[1] >> 16), qb[2 * i][0], qb[2 * i][1]);
+          mma16816(sd, f16x2_of_e4m3x2(r[2]), f16x2_of_e4m3x2(r[3]), f16x2_of_e4m3x2(r[2] >> 16),
+                   f16x2_of_e4m3x2(r[3] >> 16), qb[2 * i + 1][0], qb[2 * i + 1][1]);
+        } else {
+          mma16816(i & 1 ? sd : sc, r[0], r[1], r[2], r[3], qb[i][0], qb[i][1]);
+        }
+      }
+      const int kbase = list.key0(t0 + it) + k16;
+      const bool part = none || list.partial(kbase);
+      float lv0 = 0.f, lv1 = 0.f, iv0 = 1.f, iv1 = 1.f;
+      if (kFp8) {
         lv0 = __log2f(v0);
         lv1 = __log2f(v1);
         iv0 = __fdividef(1.f, v0);
@@ -369,49 +369,30 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
       l1 += kFp8 ? p1 * iv0 + p3 * iv1 : p1 + p3;
       const uint32_t pb0 = movm_t(pack_half2(p0, p1));
       const uint32_t pb1 = movm_t(pack_half2(p2, p3));
-      if (kFp8) {
-        // A byte pair of the transposed load is (dim 2g, dim 2g+1) of keys 2t
-        // and 2t+1: MMA rows g and g+8 stand for dims 2g and 2g+1.
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = 2 * i + a_chs;
-          const uint32_t addr = vb + a_row * 128 + ((c ^ (a_row & 7)) << 4);
-          uint32_t r[4];
-          ldsm_x4_t(addr, r[0], r[1], r[2], r[3]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) r[q] = __byte_perm(r[q], 0u, 0x3120);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t a0 = f16x2_of_e4m3x2(r[2 * h]), a1 = f16x2_of_e4m3x2(r[2 * h] >> 16);
-            uint32_t a2 = f16x2_of_e4m3x2(r[2 * h + 1]), a3 = f16x2_of_e4m3x2(r[2 * h + 1] >> 16);
-            if (part) {
-              a0 &= keep0;
-              a1 &= keep0;
-              a2 &= keep1;
-              a3 &= keep1;
-            }
-            mma16816(o[2 * i + h], a0, a1, a2, a3, pb0, pb1);
-          }
+      for (int mt = 0; mt < 8; ++mt) {
+        uint32_t a0, a1, a2, a3;
+        if (kFp8) {
+          // A byte pair of the transposed load is (dim 2g, dim 2g+1) of keys 2t
+          // and 2t+1: MMA rows g and g+8 stand for dims 2g and 2g+1.
+          const uint32_t u = __byte_perm(vf[mt >> 1][2 * (mt & 1)], 0u, 0x3120);
+          const uint32_t w = __byte_perm(vf[mt >> 1][2 * (mt & 1) + 1], 0u, 0x3120);
+          a0 = f16x2_of_e4m3x2(u);
+          a1 = f16x2_of_e4m3x2(u >> 16);
+          a2 = f16x2_of_e4m3x2(w);
+          a3 = f16x2_of_e4m3x2(w >> 16);
+        } else {
+          const uint32_t(&r)[4] = vf[mt % kFrag];
+          a0 = r[0], a1 = r[1], a2 = r[2], a3 = r[3];
         }
-      } else {
-#pragma unroll
-        for (int mt = 0; mt < 8; ++mt) {
-          const int c = 2 * mt + v_chs;
-          const uint32_t addr =
-              vb + (c >> 3) * (kTileBytes / 2) + v_row * 128 + (((c & 7) ^ (v_row & 7)) << 4);
-          uint32_t a0, a1, a2, a3;
-          ldsm_x4_t(addr, a0, a1, a2, a3);
-          if (part) {
-            a0 &= keep0;
-            a1 &= keep0;
-            a2 &= keep1;
-            a3 &= keep1;
-          }
-          mma16816(o[mt], a0, a1, a2, a3, pb0, pb1);
+        if (part) {
+          a0 &= keep0;
+          a1 &= keep0;
+          a2 &= keep1;
+          a3 &= keep1;
         }
+        mma16816(o[mt], a0, a1, a2, a3, pb0, pb1);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bars[kStages + st]));
     }
 #pragma unroll
     for (int off = 4; off <= 16; off <<= 1) {
