@@ -162,8 +162,8 @@ SIGNATURES = {
                                                                _vp, _FP8, _vp, _i32, _i32, _DIMS, _vp]),
     "grout_kv_read_paged_fp8": (ctypes.c_int, [_FP8, _vp, _i32, _vp, _vp, _i32, _i64, _vp, _vp, _i64,
                                                _DIMS, _vp]),
-    "grout_attn_decode_window_splits": (_i32, [_i32, _i32, _i32, _i32, _DIMS]),
-    "grout_attn_decode_window_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _DIMS]),
+    "grout_attn_decode_window_splits": (_i32, [_i32, _i32, _i32, _i32, _i32, _DIMS]),
+    "grout_attn_decode_window_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _DIMS]),
     "grout_attn_decode_window": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _i32,
                                                 _i32, _i32, _DIMS, _vp, _sz, _vp]),
     "grout_attn_decode_paged_window": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp,
@@ -907,18 +907,20 @@ def kv_read_paged_fp8(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v
     return k_out, v_out
 
 
-def decode_window_splits(batch, max_kv_len, window, sinks, num_q_heads, num_kv_heads, max_seq):
-    """Split count of the window decode calls (window 0: the whole context)."""
+def decode_window_splits(batch, max_kv_len, window, sinks, num_q_heads, num_kv_heads, max_seq,
+                         fp8=False):
+    """Split count of the window decode calls (fp8: of attention_decode_paged_fp8,
+    where window 0 is the whole context)."""
     dims = make_dims(num_q_heads, num_kv_heads, max_seq)
-    return lib().grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, dims)
+    return lib().grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, int(fp8), dims)
 
 
 def decode_window_workspace_bytes(batch, max_kv_len, window, sinks, num_q_heads, num_kv_heads,
-                                  max_seq, num_splits=0):
+                                  max_seq, num_splits=0, fp8=False):
     """Workspace bytes of the window decode calls (num_splits 0: the automatic count)."""
     dims = make_dims(num_q_heads, num_kv_heads, max_seq)
     return lib().grout_attn_decode_window_workspace_bytes(batch, max_kv_len, window, sinks,
-                                                          num_splits, dims)
+                                                          num_splits, int(fp8), dims)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -929,7 +931,7 @@ def _window_need(dev, *args):
 
 
 def _decode_window(fn, cache_args, q, out, dev, position, max_kv_len, window, sinks, num_splits,
-                   workspace, hkv, max_seq, qk_scale, scale_f16):
+                   workspace, hkv, max_seq, qk_scale, scale_f16, fp8=False):
     """The tail of the window decode calls: fn(q, *cache_args, position, out, ...)."""
     B, hq, _ = q.shape
     _cuda(out, "out", torch.float16, dev)
@@ -944,7 +946,7 @@ def _decode_window(fn, cache_args, q, out, dev, position, max_kv_len, window, si
             raise GroutError(1, f"workspace must be a contiguous tensor on cuda:{dev}")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     else:
-        need = _window_need(dev, B, max_kv_len, window, sinks, hq, hkv, max_seq, num_splits)
+        need = _window_need(dev, B, max_kv_len, window, sinks, hq, hkv, max_seq, num_splits, fp8)
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
             ws, ws_bytes = workspace.data_ptr(), need
@@ -1010,7 +1012,8 @@ def attention_decode_paged_fp8(q, k_pages, v_pages, k_scales, v_scales, page_tab
     stride = _table(page_table, q.size(0), dev)
     return _decode_window(lib().grout_attn_decode_paged_fp8, (pages, page_table.data_ptr(), stride),
                           q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
-                          stride * page_size if max_seq is None else max_seq, qk_scale, scale_f16)
+                          stride * page_size if max_seq is None else max_seq, qk_scale, scale_f16,
+                          True)
 
 
 def _chunk_query(q, out):

@@ -1098,23 +1098,48 @@ static int64_t window_tiles(int32_t max_kv_len, int32_t window, int32_t sinks) {
   return std::min(all, ((int64_t)sinks + 63) / 64 + ((int64_t)window + 62) / 64 + 1);
 }
 
+// Split count of the window decode for `tiles` 64-key tiles and `units` (KV
+// head, sequence) pairs.  f16 tiles stream at the memory's rate from one CTA
+// per SM; an 8-bit tile takes as long to consume and half as long to load, so
+// 8-bit calls aim at two.  Measured on B200 (64/8 heads; us, splits in
+// brackets): 8-bit, batch 1, 32768 keys: 28.8 [16], 21.3 [32], 22.7 [37]; batch
+// 4: 59.2 [5], 44.8 [8]; batch 8: 94.4 [3], 75.9 [4]; f16, batch 1, window
+// 16384: 18.8 [16], 19.2 [32]; window 1024: 7.3 [9], 8.7 [4]; batch 4, window
+// 4096: 18.0 [4], 18.4 [5], 25.2 [9].
+static int choose_window_splits(int64_t units, int64_t tiles, int num_sms, bool fp8) {
+  int64_t n = (fp8 ? num_sms * 7 / 4 : num_sms) / units;
+  // shorter splits than this cost more in the merge than they save
+  n = std::min(n, std::max<int64_t>(1, tiles / (fp8 ? 4 : 2)));
+  if (n > kDecodeMaxClusterSplits) {  // workspace and a merge launch
+    n = std::min<int64_t>({n, std::max<int64_t>(kDecodeMaxClusterSplits, tiles / 4), 64});
+    if (!fp8 && units * kDecodeMaxClusterSplits >= (num_sms * 5) / 8) n = kDecodeMaxClusterSplits;
+  }
+  // Clusters of more than 8 that do not all get an SM per CTA leave SMs idle.
+  if (n > 8 && n <= kDecodeMaxClusterSplits && units * n > num_sms)
+    n = tiles / 4 > kDecodeMaxClusterSplits ? kDecodeMaxClusterSplits + 1 : 8;
+  // Long splits of a batch that fills the SMs: halve them, so that a ragged
+  // batch evens out.
+  if (n <= 4 && tiles / std::max<int64_t>(n, 1) >= 256 && units * n <= 2 * num_sms) n = 2 * std::max<int64_t>(n, 1);
+  return (int)std::max<int64_t>(n, 1);
+}
+
 int32_t grout_attn_decode_window_splits(int32_t batch, int32_t max_kv_len, int32_t window,
-                                        int32_t sinks, const grout_attn_dims* dims) {
+                                        int32_t sinks, int32_t fp8, const grout_attn_dims* dims) {
   if (!dims || batch <= 0 || max_kv_len <= 0 || dims->num_kv_heads <= 0 || window < 0 || sinks < 0)
     return 1;
   DeviceState* ds;
   int sms = 148;
   if (current_state(&ds) == GROUT_OK) sms = ds->num_sms;
-  const int64_t keys = std::min<int64_t>(window_tiles(max_kv_len, window, sinks) * 64, INT32_MAX);
-  return choose_splits(batch, (int32_t)keys, dims->num_kv_heads, sms);
+  return choose_window_splits((int64_t)batch * dims->num_kv_heads,
+                              window_tiles(max_kv_len, window, sinks), sms, fp8 != 0);
 }
 
 size_t grout_attn_decode_window_workspace_bytes(int32_t batch, int32_t max_kv_len, int32_t window,
-                                                int32_t sinks, int32_t num_splits,
+                                                int32_t sinks, int32_t num_splits, int32_t fp8,
                                                 const grout_attn_dims* dims) {
   if (!dims || batch <= 0 || dims->num_q_heads <= 0) return 0;
   if (num_splits <= 0)
-    num_splits = grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, dims);
+    num_splits = grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, fp8, dims);
   return decode_ws_bytes(batch, dims->num_q_heads, num_splits);
 }
 
@@ -1123,7 +1148,7 @@ size_t grout_attn_decode_window_workspace_bytes(int32_t batch, int32_t max_kv_le
 static grout_status window_decode_args(DecodeWindowArgs* a, const void* q,
                                        const uint32_t* d_position, void* out, int32_t batch,
                                        int32_t max_kv_len, int32_t window, int32_t sinks,
-                                       int32_t num_splits, const grout_attn_dims* dims,
+                                       int32_t num_splits, bool fp8, const grout_attn_dims* dims,
                                        void* workspace, size_t workspace_bytes) {
   if (!q || !out || !d_position) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
   if (!aligned16(q) || !aligned16(out))
@@ -1135,7 +1160,7 @@ static grout_status window_decode_args(DecodeWindowArgs* a, const void* q,
     return fail(GROUT_ERR_INVALID_ARG, "max_kv_len=%d must be in [1, max_seq=%d]", max_kv_len,
                 dims->max_seq);
   if (num_splits == 0)
-    num_splits = grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, dims);
+    num_splits = grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, fp8, dims);
   if (num_splits < 1 || num_splits > 1024)
     return fail(GROUT_ERR_INVALID_ARG, "num_splits=%d", num_splits);
   const size_t need = decode_ws_bytes(batch, dims->num_q_heads, num_splits);
@@ -1194,8 +1219,8 @@ grout_status grout_attn_decode_window(const void* q, const void* k_cache, const 
       (cache_batch_stride < cache_head_stride * dims->num_kv_heads || cache_batch_stride % 8))
     return fail(GROUT_ERR_INVALID_ARG, "cache_batch_stride=%lld", (long long)cache_batch_stride);
   DecodeWindowArgs a{};
-  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, dims,
-                          workspace, workspace_bytes);
+  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, false,
+                          dims, workspace, workspace_bytes);
   if (st != GROUT_OK) return st;
   CUtensorMap tk, tv;
   // a row's two 64-dim halves as a dimension of their own: one load per tile
@@ -1228,8 +1253,8 @@ grout_status grout_attn_decode_paged_window(const void* q, const void* k_pages,
   st = check_pages(k_pages, v_pages, num_pages, page_size, page_table, table_stride, dims);
   if (st != GROUT_OK) return st;
   DecodeWindowArgs a{};
-  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, dims,
-                          workspace, workspace_bytes);
+  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, false,
+                          dims, workspace, workspace_bytes);
   if (st != GROUT_OK) return st;
   a.page_table = page_table;
   a.table_stride = table_stride;
@@ -1264,8 +1289,8 @@ grout_status grout_attn_decode_paged_fp8(const void* q, const grout_fp8_pages* p
   st = check_fp8_pages(pages, page_table, table_stride, dims);
   if (st != GROUT_OK) return st;
   DecodeWindowArgs a{};
-  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, dims,
-                          workspace, workspace_bytes);
+  st = window_decode_args(&a, q, d_position, out, batch, max_kv_len, window, sinks, num_splits, true,
+                          dims, workspace, workspace_bytes);
   if (st != GROUT_OK) return st;
   a.k_scales = pages->k_scales;
   a.v_scales = pages->v_scales;

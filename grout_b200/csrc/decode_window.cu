@@ -57,15 +57,17 @@ constexpr int kCtlBytes = 256;     // full/empty barriers, abort flag, per-stage
 constexpr int kRecvRows = 16;
 constexpr int kRecvBytes = kRecvRows * (128 + 1) * 4;
 constexpr int kOffCtl = kRingBytes;
-constexpr int kOffRecv = kOffCtl + kCtlBytes;
+constexpr int kOffStat = kOffCtl + kCtlBytes;  // m, then l * 2^(m - M), of each warp and head
+constexpr int kStatBytes = 2 * 8 * 8 * 4;
+constexpr int kOffRecv = kOffStat + kStatBytes;
 constexpr int kOffScales = kOffRecv + kRecvBytes;  // 8-bit: [stage][K, V][64]
 constexpr int kSmemF16 = kOffScales + 1024;
 constexpr int kSmemFp8 = kSmemF16 + kMaxStages * 2 * kKeys * 4;
 
+// Each warp's O^T, scaled to the common maximum; 132: conflict-free writes
+// (lanes write 8 neighbouring dims of 4 head pairs) and 16-byte reads.
 struct RedSmem {
-  float o[8][128][9];  // [warp]; padded: the per-dimension merge reads are conflict-free
-  float m[8][8];
-  float l[8][8];
+  float o[8][8][132];  // [warp][head][dim]
 };
 static_assert(sizeof(RedSmem) <= kRingBytes, "the merge area must fit in the ring");
 
@@ -80,33 +82,40 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void st_dsmem_f32(float* local, uint32_t rank, float v) {
+__device__ __forceinline__ uint32_t peer_address(const float* local, uint32_t rank) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+  return remote;
 }
-
-// w_s = 2^(lse_s - max) / sum, out = sum_s w_s * O_s, rounded to f16.  Splits
-// without a visible key have lse = -inf and O = 0; if all have, the row is 0.
-// A NaN lse passes into the row.  get(s, want_lse) returns lse_s or O_s[d].
-template <typename Get>
-__device__ __forceinline__ __half merge_splits(int nks, Get get) {
-  float M = -INFINITY;
-  bool any = false;
-  for (int s = 0; s < nks; ++s) {
-    const float lse = get(s, true);
-    any |= lse != -INFINITY;
-    M = fmaxf(M, lse);
-  }
-  if (!any) return __float2half_rn(0.f);
-  float W = 0.f, O = 0.f;
-  for (int s = 0; s < nks; ++s) {
-    const float lse = get(s, true);
-    const float w = lse == -INFINITY ? 0.f : ex2(lse - M);
-    W += w;
-    O += w * get(s, false);
-  }
-  return __float2half_rn(O / W);
+__device__ __forceinline__ void st_peer(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_peer4(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+__device__ __forceinline__ void store_row4(__half* p, const float4& v, float scale) {
+  uint2 u;
+  u.x = pack_half2(v.x * scale, v.y * scale);
+  u.y = pack_half2(v.z * scale, v.w * scale);
+  *reinterpret_cast<uint2*>(p) = u;
+}
+__device__ __forceinline__ void fma4(float4& acc, float w, const float4& v) {
+  acc.x += w * v.x;
+  acc.y += w * v.y;
+  acc.z += w * v.z;
+  acc.w += w * v.w;
 }
 
 // The 64-key tiles that hold a visible key: the sinks' tiles, then those from
@@ -400,61 +409,78 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
       l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
   }
+  // ------------------------------------------------- merge of the warps
+  // Every warp scales its O to the maximum over all warps itself, so that the
+  // sum over warps is plain additions of 16-byte reads.
+  float* stat_m = reinterpret_cast<float*>(smem + kOffStat);  // [warp][head]
+  float* stat_l = stat_m + 64;
+  if (warp < kWarps && g == 0) {
+    stat_m[warp * 8 + 2 * t] = m0;
+    stat_m[warp * 8 + 2 * t + 1] = m1;
+  }
   __syncthreads();  // every stage consumed: the ring becomes the merge area
   // This split's result is valid unless it is empty or a wait gave up; an
   // invalid split contributes weight 0 to the merge.
   const bool valid = nt > 0 && !*abort_flag;
-
   RedSmem* red = reinterpret_cast<RedSmem*>(smem);
-  if (valid && warp < kWarps) {
+  if (warp < kWarps) {
+    float M0 = m0, M1 = m1;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float2 m = *reinterpret_cast<const float2*>(stat_m + w * 8 + 2 * t);
+      M0 = fmaxf(M0, m.x);
+      M1 = fmaxf(M1, m.y);
+    }
+    const float f0 = ex2(m0 - M0), f1 = ex2(m1 - M1);
+    if (g == 0) {
+      stat_l[warp * 8 + 2 * t] = l0 * f0;
+      stat_l[warp * 8 + 2 * t + 1] = l1 * f1;
+    }
+    float* o0 = red->o[warp][2 * t];
+    float* o1 = red->o[warp][2 * t + 1];
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
-      const int d0 = 16 * mt + (kFp8 ? 2 * g : g), d1 = d0 + (kFp8 ? 1 : 8);
-      red->o[warp][d0][2 * t] = o[mt][0];
-      red->o[warp][d0][2 * t + 1] = o[mt][1];
-      red->o[warp][d1][2 * t] = o[mt][2];
-      red->o[warp][d1][2 * t + 1] = o[mt][3];
-    }
-    if (g == 0) {
-      red->m[warp][2 * t] = m0;
-      red->m[warp][2 * t + 1] = m1;
-      red->l[warp][2 * t] = l0;
-      red->l[warp][2 * t + 1] = l1;
+      if (kFp8) {
+        *reinterpret_cast<float2*>(o0 + 16 * mt + 2 * g) = make_float2(o[mt][0] * f0, o[mt][2] * f0);
+        *reinterpret_cast<float2*>(o1 + 16 * mt + 2 * g) = make_float2(o[mt][1] * f1, o[mt][3] * f1);
+      } else {
+        o0[16 * mt + g] = o[mt][0] * f0;
+        o1[16 * mt + g] = o[mt][1] * f1;
+        o0[16 * mt + g + 8] = o[mt][2] * f0;
+        o1[16 * mt + g + 8] = o[mt][3] * f1;
+      }
     }
   }
   if (kCluster) cluster_wait();  // every CTA of the cluster runs
   __syncthreads();
-  if (warp < kWarps) {
-    const int d = threadIdx.x & 127;
-    for (int hd = threadIdx.x >> 7; hd < G; hd += kWarps / 4) {
-      float res = 0.f, lse = -INFINITY;
-      if (valid) {
-        float M = red->m[0][hd];
+  for (int hd = warp; warp < kWarps && hd < G; hd += kWarps) {  // a warp takes a head, a lane four dims
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f, lse = -INFINITY, inv = 0.f;
+    if (valid) {
+      float M = -INFINITY;
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) M = fmaxf(M, red->m[w][hd]);
-        float L = 0.f, O = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float sc = ex2(red->m[w][hd] - M);
-          L += red->l[w][hd] * sc;
-          O += red->o[w][d][hd] * sc;
-        }
-        if (L != 0.f) {  // L == 0: every key of the split was left out
-          res = O / L;
-          lse = M + __log2f(L);
-        }
+      for (int w = 0; w < kWarps; ++w) {
+        L += stat_l[w * 8 + hd];
+        M = fmaxf(M, stat_m[w * 8 + hd]);
+        fma4(acc, 1.f, *reinterpret_cast<const float4*>(&red->o[w][hd][4 * lane]));
       }
-      if (a.nks == 1) {
-        if (valid || !pos_ok) a.out[(head0 + hd) * 128 + d] = __float2half_rn(res);
-      } else if (kCluster) {
-        const int row = hd / a.nks * a.nks + split;
-        const uint32_t owner = hd % a.nks;
-        st_dsmem_f32(recv + row * 128 + d, owner, res);
-        if (d == 0) st_dsmem_f32(recv + kRecvRows * 128 + row, owner, lse);
-      } else {
-        a.part_o[((head0 + hd) * a.nks + split) * 128 + d] = res;
-        if (d == 0) a.part_lse[(head0 + hd) * a.nks + split] = lse;
+      if (L != 0.f) {  // L == 0: every key of the split was left out
+        inv = 1.f / L;
+        lse = M + __log2f(L);
       }
+    }
+    if (a.nks == 1) {
+      if (valid || !pos_ok) store_row4(a.out + (head0 + hd) * 128 + 4 * lane, acc, inv);
+    } else if (kCluster) {
+      const int row = hd / a.nks * a.nks + split;
+      const uint32_t to = peer_address(recv, hd % a.nks);
+      st_peer4(to + (row * 128 + 4 * lane) * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+      if (lane == 0) st_peer(to + (kRecvRows * 128 + row) * 4, lse);
+    } else {
+      const int64_t row = (head0 + hd) * a.nks + split;
+      reinterpret_cast<float4*>(a.part_o + row * 128)[lane] =
+          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (lane == 0) a.part_lse[row] = lse;
     }
   }
   if (kCluster) {
@@ -462,28 +488,49 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
     // after this one nobody touches a peer's memory.
     cluster_arrive();
     cluster_wait();
-    if (threadIdx.x < 128) {
-      const int d = threadIdx.x;
-      for (int hd = (int)cluster_ctarank(); hd < G; hd += a.nks) {
-        const float* po = recv + hd / a.nks * a.nks * 128 + d;
-        const float* lse = recv + kRecvRows * 128 + hd / a.nks * a.nks;
-        a.out[(head0 + hd) * 128 + d] = merge_splits(a.nks, [&](int s, bool want_lse) {
-          return want_lse ? lse[s] : po[s * 128];
-        });
-      }
+    for (int hd = (int)cluster_ctarank() + warp * a.nks; warp < kWarps && hd < G; hd += kWarps * a.nks) {
+      const int row0 = hd / a.nks * a.nks;
+      // w_s = 2^(lse_s - max) / sum, out = sum_s w_s * O_s, rounded to f16.
+      // Splits without a visible key have lse = -inf and O = 0; if all have,
+      // the row is 0.  A NaN lse passes into the row.
+      const float lse = lane < a.nks ? recv[kRecvRows * 128 + row0 + lane] : -INFINITY;
+      const float M = warp_max(lse);
+      const float w = lse == -INFINITY ? 0.f : ex2(lse - M);
+      const float W = warp_sum(w);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = 0; s < a.nks; ++s)
+        fma4(acc, __shfl_sync(0xffffffffu, w, s),
+             reinterpret_cast<const float4*>(recv + (row0 + s) * 128)[lane]);
+      store_row4(a.out + (head0 + hd) * 128 + 4 * lane, acc, W != 0.f ? 1.f / W : 0.f);
     }
   }
 }
 
-// Workspace merge, one CTA per (sequence, query head), one thread per dim.
+// Workspace merge, one CTA per (sequence, query head): every warp forms the
+// weights, takes every fourth split, and the four sums meet in shared memory.
 __global__ void __launch_bounds__(128) decode_window_merge_kernel(const DecodeWindowArgs a) {
+  __shared__ float4 part[4][32];
   const int64_t row = blockIdx.x;
-  const int d = threadIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* lse = a.part_lse + row * a.nks;
-  const float* po = a.part_o + row * a.nks * 128 + d;
-  a.out[row * 128 + d] = merge_splits(a.nks, [&](int s, bool want_lse) {
-    return want_lse ? lse[s] : po[s * 128];
-  });
+  const float4* po = reinterpret_cast<const float4*>(a.part_o + row * a.nks * 128) + lane;
+  float M = -INFINITY, W = 0.f;
+  for (int s = lane; s < a.nks; s += 32) M = fmaxf(M, lse[s]);
+  M = warp_max(M);
+  for (int s = lane; s < a.nks; s += 32) W += lse[s] == -INFINITY ? 0.f : ex2(lse[s] - M);
+  W = warp_sum(W);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = warp; s < a.nks; s += 4) {
+    const float w = lse[s] == -INFINITY ? 0.f : ex2(lse[s] - M);
+    fma4(acc, w, po[(int64_t)s * 32]);
+  }
+  part[warp][lane] = acc;
+  __syncthreads();
+  if (warp == 0) {
+    for (int w = 1; w < 4; ++w) fma4(acc, 1.f, part[w][lane]);
+    store_row4(a.out + row * 128 + 4 * lane, acc, W != 0.f ? 1.f / W : 0.f);
+  }
 }
 
 template <bool kFp8, bool kPaged, bool kCluster>

@@ -488,13 +488,14 @@ grout_status grout_kv_read_paged_fp8(const grout_fp8_pages* pages, const int32_t
  * pages that lie wholly outside may be freed (any table entry, -1 for one)
  * and their rows may hold anything. */
 
-/* Split count of the window decode entry points for num_splits = 0, and the
- * workspace bytes they need (0 up to 16 splits); window 0 = the whole
- * context (8-bit caches). */
+/* Split count of the window decode entry points for num_splits = 0 (fp8: of
+ * grout_attn_decode_paged_fp8; window 0 = the whole context), and the
+ * workspace bytes they need for a split count, 0 = that one (none up to 16
+ * splits). */
 int32_t grout_attn_decode_window_splits(int32_t batch, int32_t max_kv_len, int32_t window,
-                                        int32_t sinks, const grout_attn_dims* dims);
+                                        int32_t sinks, int32_t fp8, const grout_attn_dims* dims);
 size_t grout_attn_decode_window_workspace_bytes(int32_t batch, int32_t max_kv_len, int32_t window,
-                                                int32_t sinks, int32_t num_splits,
+                                                int32_t sinks, int32_t num_splits, int32_t fp8,
                                                 const grout_attn_dims* dims);
 
 /* Window forms of grout_attn_decode_ex and grout_attn_decode_paged; arguments

@@ -160,15 +160,25 @@ def test_prefill_refusals(L):
 
 
 def test_window_split_counts(L):
-    """A window bounds what a split count is chosen for, whatever the context."""
+    """A window bounds what a split count is chosen for, whatever the context;
+    a cluster's splits need no workspace."""
     d = _dims(ms=1 << 20)
-    a = [L.grout_attn_decode_window_splits(1, n, 1024, 4, d) for n in (2048, 32768, 1 << 20)]
-    assert a[0] == a[1] == a[2] >= 1
-    assert L.grout_attn_decode_window_splits(1, 32768, 0, 0, d) == L.grout_attn_decode_splits(1, 32768, d)
-    assert L.grout_attn_decode_window_splits(64, 32768, 4096, 4, d) == 1
-    assert L.grout_attn_decode_window_splits(1, 2 ** 20, 2 ** 31 - 1, 2 ** 31 - 1, d) >= 1
-    assert L.grout_attn_decode_window_workspace_bytes(2, 4096, 1024, 4, 16, d) == 0
-    assert L.grout_attn_decode_window_workspace_bytes(2, 4096, 1024, 4, 17, d) == 2 * 64 * 17 * 129 * 4
+    count = L.grout_attn_decode_window_splits
+    for fp8 in (0, 1):
+        a = [count(1, n, 1024, 4, fp8, d) for n in (2048, 32768, 1 << 20)]
+        assert a[0] == a[1] == a[2] >= 1
+        assert count(1, 2 ** 20, 2 ** 31 - 1, 2 ** 31 - 1, fp8, d) >= 1
+        for hq, hkv in ((64, 8), (8, 1), (8, 8)):
+            d2 = _dims(hq=hq, hkv=hkv, ms=1 << 20)
+            for B in (1, 2, 3, 5, 8, 17, 40, 300):
+                for n in (1, 64, 1000, 5000, 40000, 1 << 20):
+                    s = count(B, n, 0, 0, fp8, d2)
+                    assert 1 <= s <= max(1, -(-n // 64)) and s <= 64
+                    need = L.grout_attn_decode_window_workspace_bytes(B, n, 0, 0, 0, fp8, d2)
+                    assert need == (0 if s <= 16 else B * hq * s * 129 * 4)
+    assert count(64, 32768, 4096, 4, 0, d) == 1
+    assert L.grout_attn_decode_window_workspace_bytes(2, 4096, 1024, 4, 16, 0, d) == 0
+    assert L.grout_attn_decode_window_workspace_bytes(2, 4096, 1024, 4, 17, 0, d) == 2 * 64 * 17 * 129 * 4
 
 
 def test_python_refuses_what_is_not_on_the_gpu():
