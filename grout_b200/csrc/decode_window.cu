@@ -45,6 +45,7 @@ namespace grout {
 namespace {
 
 constexpr int kKeys = 64;  // keys per tile
+constexpr float kSlack = 8.0f;  // log2 units: weights stay below 2^8, well inside f16
 constexpr int kRingBytes = 98304;
 constexpr int kMaxStages = 6;
 // Consumer warps; one more produces.
@@ -135,9 +136,10 @@ struct TileList {
   __device__ __forceinline__ bool sees(int key) const {
     return key < kv_len && (key >= lo || key < sinks);
   }
-  // whether some of the 16 keys from `base` on are not seen
-  __device__ __forceinline__ bool partial(int base) const {
-    return base + 16 > kv_len || (base < lo && base + 16 > sinks);
+  // whether tile i of the list may hold keys that are not seen: the sinks'
+  // last tile, the window's first one, the last one
+  __device__ __forceinline__ bool partial(int i) const {
+    return i == sink_tiles - 1 || i == sink_tiles || i == n - 1;
   }
 };
 
@@ -324,16 +326,15 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
       for (int i = 0; i < kFrag; ++i) {
         const uint32_t(&r)[4] = kf[i];
         if (kFp8) {
-          mma16816(sc, f16x2_of_e4m3x2(r[0]), f16x2_of_e4m3x2(r[1]), f16x2_of_e4m3x2(r[0] >> 16),
-                   f16x2_of_e4m3x2(r[1] >> 16), qb[2 * i][0], qb[2 * i][1]);
-          mma16816(sd, f16x2_of_e4m3x2(r[2]), f16x2_of_e4m3x2(r[3]), f16x2_of_e4m3x2(r[2] >> 16),
-                   f16x2_of_e4m3x2(r[3] >> 16), qb[2 * i + 1][0], qb[2 * i + 1][1]);
+          mma16816(sc, f16x2_of_e4m3_lo(r[0]), f16x2_of_e4m3_lo(r[1]), f16x2_of_e4m3_hi(r[0]),
+                   f16x2_of_e4m3_hi(r[1]), qb[2 * i][0], qb[2 * i][1]);
+          mma16816(sd, f16x2_of_e4m3_lo(r[2]), f16x2_of_e4m3_lo(r[3]), f16x2_of_e4m3_hi(r[2]),
+                   f16x2_of_e4m3_hi(r[3]), qb[2 * i + 1][0], qb[2 * i + 1][1]);
         } else {
           mma16816(i & 1 ? sd : sc, r[0], r[1], r[2], r[3], qb[i][0], qb[i][1]);
         }
       }
-      const int kbase = list.key0(t0 + it) + k16;
-      const bool part = none || list.partial(kbase);
+      const bool part = none || list.partial(t0 + it);
       float lv0 = 0.f, lv1 = 0.f, iv0 = 1.f, iv1 = 1.f;
       if (kFp8) {
         lv0 = __log2f(v0);
@@ -345,19 +346,24 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
       float s2 = fmaf(sc[2] + sd[2], f1, lv1), s3 = fmaf(sc[3] + sd[3], f1, lv1);
       uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;  // V halves: keys 2t, 2t+1 / 2t+8, 2t+9
       if (part) {
+        const int kbase = list.key0(t0 + it) + k16;
         if (none || !list.sees(kbase + g)) s0 = s1 = -INFINITY, iv0 = 1.f;
         if (none || !list.sees(kbase + g + 8)) s2 = s3 = -INFINITY, iv1 = 1.f;
         const int q = kbase + 2 * t;
         keep0 = none ? 0u : (list.sees(q) ? 0xFFFFu : 0u) | (list.sees(q + 1) ? 0xFFFF0000u : 0u);
         keep1 = none ? 0u : (list.sees(q + 8) ? 0xFFFFu : 0u) | (list.sees(q + 9) ? 0xFFFF0000u : 0u);
       }
-      float mx0 = fmaxf(s0, s2), mx1 = fmaxf(s1, s3);
+      // m is a reference, not the maximum: it moves (and O is rescaled) only
+      // when a score passes it by more than kSlack, so the weights stay below
+      // 2^kSlack and most tiles need one vote instead of the reduction.
+      const float c0 = m0 + kSlack, c1 = m1 + kSlack;
+      if (__any_sync(0xffffffffu, s0 > c0 || s1 > c1 || s2 > c0 || s3 > c1)) {
+        float mx0 = fmaxf(s0, s2), mx1 = fmaxf(s1, s3);
 #pragma unroll
-      for (int off = 4; off <= 16; off <<= 1) {
-        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
-        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
-      }
-      if (__any_sync(0xffffffffu, mx0 > m0 || mx1 > m1)) {
+        for (int off = 4; off <= 16; off <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+        }
         const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
         const float al0 = ex2(m0 - mn0), al1 = ex2(m1 - mn1);
         l0 *= al0;
@@ -386,10 +392,10 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
           // and 2t+1: MMA rows g and g+8 stand for dims 2g and 2g+1.
           const uint32_t u = __byte_perm(vf[mt >> 1][2 * (mt & 1)], 0u, 0x3120);
           const uint32_t w = __byte_perm(vf[mt >> 1][2 * (mt & 1) + 1], 0u, 0x3120);
-          a0 = f16x2_of_e4m3x2(u);
-          a1 = f16x2_of_e4m3x2(u >> 16);
-          a2 = f16x2_of_e4m3x2(w);
-          a3 = f16x2_of_e4m3x2(w >> 16);
+          a0 = f16x2_of_e4m3_lo(u);
+          a1 = f16x2_of_e4m3_hi(u);
+          a2 = f16x2_of_e4m3_lo(w);
+          a3 = f16x2_of_e4m3_hi(w);
         } else {
           const uint32_t(&r)[4] = vf[mt % kFrag];
           a0 = r[0], a1 = r[1], a2 = r[2], a3 = r[3];

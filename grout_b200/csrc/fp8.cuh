@@ -28,6 +28,17 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
 }
+// The low / high two of four e4m3 codes -> packed f16 pair (exact; low byte -> low half).
+__device__ __forceinline__ uint32_t f16x2_of_e4m3_lo(uint32_t codes) {
+  uint32_t r;
+  asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l; }" : "=r"(r) : "r"(codes));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2_of_e4m3_hi(uint32_t codes) {
+  uint32_t r;
+  asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h; }" : "=r"(r) : "r"(codes));
+  return r;
+}
 // Two e4m3 codes -> packed f16 pair (exact; low byte -> low half).
 __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t codes) {
   uint32_t r;
