@@ -947,6 +947,15 @@ static grout_status check_fp8_pages(const grout_fp8_pages* p, const int32_t* pag
   return GROUT_OK;
 }
 
+// The write kernel counts (token, head) rows in 32 bits.
+static grout_status check_write_rows(int64_t rows, const grout_attn_dims* dims) {
+  const int64_t heads = (int64_t)dims->num_q_heads + 2 * (int64_t)dims->num_kv_heads;
+  if (heads > INT32_MAX || rows * heads > INT32_MAX)
+    return fail(GROUT_ERR_UNSUPPORTED, "%lld tokens x %lld heads: at most 2^31 - 1 rows a call",
+                (long long)rows, (long long)heads);
+  return GROUT_OK;
+}
+
 static Fp8Pages fp8_pages_of(const grout_fp8_pages* p) {
   return Fp8Pages{static_cast<uint8_t*>(p->k), static_cast<uint8_t*>(p->v), p->k_scales, p->v_scales};
 }
@@ -967,6 +976,7 @@ grout_status grout_qk_norm_rope_kv_decode_paged_fp8(
   if (!d_position) return fail(GROUT_ERR_INVALID_ARG, "d_position is null");
   st = check_fp8_pages(pages, page_table, table_stride, dims);
   if (st != GROUT_OK) return st;
+  if ((st = check_write_rows(batch, dims)) != GROUT_OK) return st;
   DeviceState* ds;
   st = current_state(&ds);
   if (st != GROUT_OK) return st;
@@ -1011,6 +1021,7 @@ grout_status grout_qk_norm_rope_kv_prefill_paged_fp8(
     if (!p) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
     if (!aligned16(p)) return fail(GROUT_ERR_INVALID_ARG, "pointer %p is not 16-byte aligned", p);
   }
+  if ((st = check_write_rows(seq_len, dims)) != GROUT_OK) return st;
   // one table row of ceil(max_seq / page_size) entries
   st = check_fp8_pages(pages, page_table, INT64_MAX, dims);
   if (st != GROUT_OK) return st;

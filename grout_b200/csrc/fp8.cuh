@@ -39,13 +39,6 @@ __device__ __forceinline__ uint32_t f16x2_of_e4m3_hi(uint32_t codes) {
   asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h; }" : "=r"(r) : "r"(codes));
   return r;
 }
-// Two e4m3 codes -> packed f16 pair (exact; low byte -> low half).
-__device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t codes) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes));
-  return r;
-}
-
 // Quantises an octet's row: lane j holds elements 8j..8j+7 (lo) and
 // 64+8j..64+8j+7 (hi).  codes_lo/hi are the lane's 8-byte chunks; returns the
 // row's scale (the same in every lane).

@@ -23,11 +23,11 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
   const int j = threadIdx.x & 7;  // lane within the octet
   const unsigned mask = 0xFFu << (threadIdx.x & 24);
   const uint32_t heads = (uint32_t)(a.hq + 2 * a.hkv);
-  const uint64_t ntask = (uint64_t)a.rows * heads;
+  const uint32_t ntask = (uint32_t)a.rows * heads;  // the host keeps it and the last step below 2^32
   const uint32_t step = (gridDim.x * blockDim.x) >> 3;
-  for (uint64_t task = (blockIdx.x * blockDim.x + threadIdx.x) >> 3; task < ntask; task += step) {
-    const uint32_t s = (uint32_t)(task / heads);
-    const int hh = (int)(task - (uint64_t)s * heads);
+  for (uint32_t task = (blockIdx.x * blockDim.x + threadIdx.x) >> 3; task < ntask; task += step) {
+    const uint32_t s = task / heads;
+    const int hh = (int)(task - s * heads);
     const bool is_q = hh < a.hq;
     const bool is_v = hh >= a.hq + a.hkv;
     const int kh = hh - a.hq - (is_v ? a.hkv : 0);
@@ -49,13 +49,13 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
     const uint4 xh = ldg16(src + 64 + 8 * j);
     int64_t slot = 0;  // cache row: (page * hkv + kh) * page_size + row in page
     if (!is_q) {
-      const int64_t pg = pos / a.page_size;
+      const uint32_t pg = (uint32_t)pos / (uint32_t)a.page_size;
       const int32_t page = a.page_table[(kDecode ? (int64_t)s * a.table_stride : 0) + pg];
       if (page < 0 || page >= a.num_pages) {
         if (j == 0 && a.err) atomicCAS(a.err, 0, DEV_ERR_PAGE);
         continue;
       }
-      slot = ((int64_t)page * a.hkv + kh) * a.page_size + (pos - pg * a.page_size);
+      slot = ((int64_t)page * a.hkv + kh) * a.page_size + (uint32_t)pos - pg * (uint32_t)a.page_size;
     }
     float lo[8], hi[8];
     if (is_v) {
@@ -86,56 +86,71 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
 }
 
 // Read-back: packed output row r of sequence b (cu[b] <= r < cu[b+1]) is cache
-// position first[b] + r - cu[b].  One octet per (row, KV head): lane j turns
-// 16 codes of K and 16 of V into f16(code * scale) and stores 32 bytes of each.
-constexpr int kReadRows = 32;  // octets of a 256-thread block
-__global__ void __launch_bounds__(256) kv_read_fp8_kernel(const KvReadFp8Args a) {
-  const int j = threadIdx.x & 7;
-  const uint64_t task = (uint64_t)blockIdx.x * kReadRows + (threadIdx.x >> 3);
-  const int64_t row = (int64_t)(task / (uint32_t)a.hkv);
-  const int kh = (int)(task - (uint64_t)row * (uint32_t)a.hkv);
-  if (row >= a.rows) return;
-  // last sequence whose first row is <= row (empty sequences own no row)
-  int lo = 0, hi = a.batch;  // cu[lo] <= row < cu[hi] if the row has an owner
-  if (row < a.cu[0] || row >= a.cu[a.batch]) return;  // rows of no sequence stay as they are
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  const int64_t pos = (a.first ? (int64_t)a.first[lo] : 0) + (row - a.cu[lo]);
-  int64_t slot = -1;
-  if (pos < 0 || pos >= a.max_seq) {
-    if (j == 0 && kh == 0 && a.err) atomicCAS(a.err, 0, DEV_ERR_POSITION);
-  } else {
-    const int64_t pg = pos / a.page_size;
-    const int32_t page = __ldg(a.page_table + (int64_t)lo * a.table_stride + pg);
-    if (page < 0 || page >= a.num_pages) {
-      if (j == 0 && a.err) atomicCAS(a.err, 0, DEV_ERR_PAGE);
-    } else {
-      slot = ((int64_t)page * a.hkv + kh) * a.page_size + (pos - pg * a.page_size);
-    }
-  }
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};  // a row that cannot be read is zero
-    if (slot >= 0) {
-      const uint4 c = ldg16((kv ? a.pages.v : a.pages.k) + slot * kHeadDim + 16 * j);
-      const float scale = __ldg((kv ? a.pages.v_scales : a.pages.k_scales) + slot);
-      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-      uint32_t h[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t p = f16x2_of_e4m3x2(w[i >> 1] >> (16 * (i & 1)));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-        h[i] = pack_half2(__fmul_rn(f.x, scale), __fmul_rn(f.y, scale));
+// position first[b] + r - cu[b].  A warp takes kReadTasks neighbouring (row, KV
+// head) pairs: a lane each finds their sequence and cache row, then half-warps
+// turn them, K in the lower and V in the upper half, 8 codes a lane (8-byte
+// loads, 16-byte stores: both rows' 128 and 256 bytes are whole lines), all loads first.
+constexpr int kReadTasks = 8;
+constexpr int kReadWarps = 8;
+__global__ void __launch_bounds__(32 * kReadWarps) kv_read_fp8_kernel(const KvReadFp8Args a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t task0 = ((int64_t)blockIdx.x * kReadWarps + (threadIdx.x >> 5)) * kReadTasks;
+  int64_t slot_l = -1, out_l = -1;  // of task0 + lane: cache row (-1: zeros), output offset (-1: none)
+  if (lane < kReadTasks && task0 + lane < a.rows * a.hkv) {
+    const int64_t row = (task0 + lane) / a.hkv;
+    const int kh = (int)(task0 + lane - row * a.hkv);
+    if (row >= a.cu[0] && row < a.cu[a.batch]) {  // rows of no sequence stay as they are
+      // the last sequence whose first row is <= row (empty sequences own no row)
+      int lo = 0, hi = a.batch;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= row) lo = mid;
+        else hi = mid;
       }
-      o[0] = make_uint4(h[0], h[1], h[2], h[3]);
-      o[1] = make_uint4(h[4], h[5], h[6], h[7]);
+      out_l = row * a.out_row_stride + (int64_t)kh * kHeadDim;
+      const int64_t pos = (a.first ? (int64_t)a.first[lo] : 0) + (row - a.cu[lo]);
+      if (pos < 0 || pos >= a.max_seq) {
+        if (a.err) atomicCAS(a.err, 0, DEV_ERR_POSITION);
+      } else {
+        const uint32_t pg = (uint32_t)pos / (uint32_t)a.page_size;
+        const int32_t page = __ldg(a.page_table + (int64_t)lo * a.table_stride + pg);
+        if (page < 0 || page >= a.num_pages) {
+          if (a.err) atomicCAS(a.err, 0, DEV_ERR_PAGE);
+        } else {
+          slot_l = ((int64_t)page * a.hkv + kh) * a.page_size + (uint32_t)pos - pg * (uint32_t)a.page_size;
+        }
+      }
     }
-    __half* dst = (kv ? a.v_out : a.k_out) + row * a.out_row_stride + (int64_t)kh * kHeadDim + 16 * j;
-    *reinterpret_cast<uint4*>(dst) = o[0];
-    *reinterpret_cast<uint4*>(dst + 8) = o[1];
+  }
+  const bool v = lane >= 16;
+  const int j = lane & 15;
+  const uint8_t* codes = (v ? a.pages.v : a.pages.k) + 8 * j;
+  const float* scales = v ? a.pages.v_scales : a.pages.k_scales;
+  __half* out = (v ? a.v_out : a.k_out) + 8 * j;
+  uint2 c[kReadTasks];
+  float scale[kReadTasks];
+#pragma unroll
+  for (int u = 0; u < kReadTasks; ++u) {
+    const int64_t slot = __shfl_sync(0xffffffffu, slot_l, u);
+    c[u] = make_uint2(0, 0);  // a row that cannot be read is zero
+    scale[u] = 0.f;
+    if (slot >= 0) {
+      c[u] = __ldg(reinterpret_cast<const uint2*>(codes + slot * kHeadDim));
+      scale[u] = __ldg(scales + slot);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kReadTasks; ++u) {
+    const int64_t off = __shfl_sync(0xffffffffu, out_l, u);
+    const uint32_t p[4] = {f16x2_of_e4m3_lo(c[u].x), f16x2_of_e4m3_hi(c[u].x), f16x2_of_e4m3_lo(c[u].y),
+                           f16x2_of_e4m3_hi(c[u].y)};
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i]));
+      h[i] = pack_half2(__fmul_rn(f.x, scale[u]), __fmul_rn(f.y, scale[u]));
+    }
+    if (off >= 0) *reinterpret_cast<uint4*>(out + off) = make_uint4(h[0], h[1], h[2], h[3]);
   }
 }
 
@@ -156,9 +171,10 @@ cudaError_t launch_qk_norm_rope_kv_fp8(const NormRopeFp8Args& a, int num_sms, cu
 }
 
 cudaError_t launch_kv_read_fp8(const KvReadFp8Args& a, cudaStream_t s) {
-  const int64_t blocks = (a.rows * a.hkv + kReadRows - 1) / kReadRows;
+  const int64_t per = kReadWarps * kReadTasks;
+  const int64_t blocks = (a.rows * a.hkv + per - 1) / per;
   if (blocks == 0) return cudaSuccess;
-  kv_read_fp8_kernel<<<(unsigned)blocks, 256, 0, s>>>(a);
+  kv_read_fp8_kernel<<<(unsigned)blocks, 32 * kReadWarps, 0, s>>>(a);
   return cudaGetLastError();
 }
 
