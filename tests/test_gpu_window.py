@@ -230,8 +230,9 @@ def test_prefill_many_items(grout, batch, hq, hkv):
     check(out, ref, bound)
 
 
-def test_prefill_of_a_full_window_equals_plain_prefill(grout):
-    """A window as long as the context: the plain kernel's bits."""
+def test_prefill_of_a_full_window_agrees_with_plain_prefill(grout):
+    """A window as long as the context: both kernels (which take keys in
+    different blocks) are within the bound of the same result."""
     S, hq, hkv, n, p = 400, 16, 4, 900, 300
     q = normal(13, S, hq, D).half()
     k, v = _caches(1, hkv, n, 80)
@@ -239,7 +240,11 @@ def test_prefill_of_a_full_window_equals_plain_prefill(grout):
     grout.attention_prefill(q, k[0], v[0], a, p)
     grout.attention_prefill_varlen_window(q, k[0], v[0], b, None, S, hkv, D, n * D, 900, 0,
                                           position_start=torch.tensor([p], dtype=torch.int32, device="cuda"))
-    assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    ref, bound = _prefill_ref(q, k, v, [0, S], [p], 0, 0)
+    check(a, ref, bound)
+    check(b, ref, bound)
 
 
 def test_prefill_packed_keys(grout):
