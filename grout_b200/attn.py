@@ -796,10 +796,18 @@ def _norm_weights(q_norm_w, k_norm_w, dev):
 
 
 @functools.lru_cache(maxsize=1024)
+def _dims_of(num_q_heads, num_kv_heads, max_seq, rms_eps, qk_scale, flags):
+    return AttnDims(num_q_heads, num_kv_heads, HEAD_DIM, max_seq, rms_eps, qk_scale, flags)
+
+
 def _dims(num_q_heads, num_kv_heads, max_seq, rms_eps, qk_scale, flags):
-    """AttnDims of these numbers (read only)."""
-    return AttnDims(num_q_heads, num_kv_heads, HEAD_DIM, max_seq, rms_eps,
-                    float(qk_scale) if qk_scale else 0.0, flags)
+    """AttnDims of these numbers (read only; floats, so that the cache is by value)."""
+    return _dims_of(num_q_heads, num_kv_heads, max_seq, float(rms_eps), float(qk_scale or 0.0), flags)
+
+
+def _span(n):
+    """A window or sink count for an int32 argument, which would wrap a larger one silently."""
+    return n if -0x80000000 <= n <= 0x7FFFFFFF else (0x7FFFFFFF if n > 0 else -1)
 
 
 def qk_norm_rope_kv_decode_paged_fp8(qkv, q_norm_w, k_norm_w, rope_table, q_out, k_pages, v_pages,
@@ -912,14 +920,14 @@ def decode_window_splits(batch, max_kv_len, window, sinks, num_q_heads, num_kv_h
     """Split count of the window decode calls (fp8: of attention_decode_paged_fp8,
     where window 0 is the whole context)."""
     dims = make_dims(num_q_heads, num_kv_heads, max_seq)
-    return lib().grout_attn_decode_window_splits(batch, max_kv_len, window, sinks, int(fp8), dims)
+    return lib().grout_attn_decode_window_splits(batch, max_kv_len, _span(window), _span(sinks), int(fp8), dims)
 
 
 def decode_window_workspace_bytes(batch, max_kv_len, window, sinks, num_q_heads, num_kv_heads,
                                   max_seq, num_splits=0, fp8=False):
     """Workspace bytes of the window decode calls (num_splits 0: the automatic count)."""
     dims = make_dims(num_q_heads, num_kv_heads, max_seq)
-    return lib().grout_attn_decode_window_workspace_bytes(batch, max_kv_len, window, sinks,
+    return lib().grout_attn_decode_window_workspace_bytes(batch, max_kv_len, _span(window), _span(sinks),
                                                           num_splits, int(fp8), dims)
 
 
@@ -939,6 +947,7 @@ def _decode_window(fn, cache_args, q, out, dev, position, max_kv_len, window, si
         raise GroutError(1, "out shape mismatch")
     _positions(position, B, dev)
     num_splits = num_splits or 0
+    window, sinks = _span(window), _span(sinks)
     ws, ws_bytes = None, 0
     if workspace is not None:
         if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.is_contiguous()
@@ -1060,7 +1069,7 @@ def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_k
         q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k.data_ptr(), v.data_ptr(),
         kv_batch_stride, kv_row_stride, kv_head_stride, kv_rows, cu,
         _starts(position_start, B, dev), _starts(kv_start, B, dev, "kv_start"), B, max_q_len)
-    _enqueue(dev, lib().grout_attn_prefill_varlen_window, args, window, sinks,
+    _enqueue(dev, lib().grout_attn_prefill_varlen_window, args, _span(window), _span(sinks),
              _dims(hq, num_kv_heads, 1 << 30, 0.0, qk_scale, 0))
     return out
 
@@ -1080,7 +1089,7 @@ def attention_prefill_paged_window(q, k_pages, v_pages, page_table, out, window,
         q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k_pages.data_ptr(), v_pages.data_ptr(),
         num_pages, page_size, page_table.data_ptr(), stride, cu, _starts(position_start, B, dev), B,
         max_q_len)
-    _enqueue(dev, lib().grout_attn_prefill_paged_window, args, window, sinks,
+    _enqueue(dev, lib().grout_attn_prefill_paged_window, args, _span(window), _span(sinks),
              _dims(hq, hkv, stride * page_size if max_seq is None else max_seq, 0.0, qk_scale, 0))
     return out
 

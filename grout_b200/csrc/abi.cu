@@ -1323,6 +1323,9 @@ grout_status grout_attn_decode_paged_fp8(const void* q, const grout_fp8_pages* p
   return GROUT_OK;
 }
 
+// Position arithmetic of the window prefill stays in 31 bits.
+constexpr int64_t kMaxKeys = INT32_MAX - 4096;
+
 // The checks and the launch that the window prefill entry points share; `a`
 // comes with the cache fields set (max_keys: positions per sequence), dk and sk
 // are the K/V maps' dims and strides.
@@ -1369,16 +1372,13 @@ static grout_status window_prefill(PrefillWindowArgs* a, const void* q, void* ou
   a->hq = (int32_t)hq;
   a->hkv = (int32_t)hkv;
   a->scale_log2 = qk_scale(dims) / logf(2.0f);
-  a->window = window;
-  a->sinks = sinks;
+  a->window = (int32_t)std::min<int64_t>(window, kMaxKeys);  // sees every key
+  a->sinks = (int32_t)std::min<int64_t>(sinks, kMaxKeys);
   a->err = ds->err;
   CUDA_TRY(launch_prefill_window(*a, max_q_len, ds->num_sms, tq, tk, tv,
                                  reinterpret_cast<cudaStream_t>(stream)));
   return GROUT_OK;
 }
-
-// Position arithmetic of the window prefill stays in 31 bits.
-constexpr int64_t kMaxKeys = INT32_MAX - 4096;
 
 grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* p, int32_t window,
                                               int32_t sinks, const grout_attn_dims* dims,

@@ -130,11 +130,10 @@ struct Item {
   int n0, n_kv;     // KV tiles of query tile 0, of the item (tile 1 takes all)
   bool two;         // the item has a second query tile
   bool alt;         // (kShort) it has not, but two KV tiles or more: chain t takes those of parity t
-  // KV tiles of chain t, and its i-th one
+  // KV tiles of chain t
   __device__ __forceinline__ int count(int t) const {
     return alt ? (n_kv + 1 - t) >> 1 : (t == 0 ? n0 : (two ? n_kv : 0));
   }
-  __device__ __forceinline__ int entry(int t, int i) const { return alt ? 2 * i + t : i; }
   int nblk, sink_blk, skip;  // 64-key blocks; entry i is block i or, past the sinks, i + skip
   int wlo, vis_end; // keys some row sees: n < sinks, and wlo <= n < vis_end
   // first key of block entry i
@@ -174,8 +173,8 @@ struct Walk {
     }
     P = a.pos0 ? a.pos0[n] : 0;
     const int ks = a.kv_start ? a.kv_start[n] : 0;
-    if (S <= 0) return;
-    if (q_start < 0 || (int64_t)q_start + S > a.q_rows || P < 0 || ks < 0 ||
+    if (S == 0) return;
+    if (S < 0 || q_start < 0 || (int64_t)q_start + S > a.q_rows || P < 0 || ks < 0 ||
         (int64_t)ks + P + S > a.max_keys) {
       if (a.err) atomicCAS(a.err, 0, DEV_ERR_POSITION);
       return;
@@ -295,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     return has;
   };
-  Item it;
+  Item it = {};
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 12) {

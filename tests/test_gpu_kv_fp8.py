@@ -354,3 +354,33 @@ def test_serving_run(grout):
         ck, cv = cache(done + i + 1)
         for o, w, sk in ((out, window, sinks), (full, 0, 0)):
             check(o, *attention64(q_out, ck, cv, pos.long(), w, sk, SCALE_F16))
+
+
+def test_offsets_past_32_bits(grout):
+    """Pools of more than 2^32 bytes of codes: pages at the far end are written (the query rows in place), read back and attended to."""
+    hq, hkv, ps, S = 8, 1, 1024, 1500
+    pages = 2 ** 32 // (hkv * ps * D) + 4
+    pools = [torch.empty(pages, hkv, ps, D, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in "kv"]
+    pools += [torch.empty(pages, hkv, ps, device="cuda") for _ in "kv"]
+    table = torch.tensor([[pages - 1, pages - 3]], dtype=torch.int32, device="cuda")
+    q, k, v = (normal(400 + j, S, h, D).half() for j, h in enumerate((hq, hkv, hkv)))
+    w = torch.ones(D, dtype=torch.float16, device="cuda")
+    rope = grout.rope_table(THETA, 2 * ps)
+    near = [torch.zeros(2, hkv, ps, D, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in "kv"]
+    near += [torch.zeros(2, hkv, ps, device="cuda") for _ in "kv"]
+    q_near = torch.empty_like(q)
+    grout.qk_norm_rope_kv_prefill_paged_fp8(q, k, v, w, w, rope, q_near, *near, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 0, EPS)
+    grout.qk_norm_rope_kv_prefill_paged_fp8(q, k, v, w, w, rope, q, *pools, table[0], 0, EPS)
+    cu = torch.tensor([0, S], dtype=torch.int32, device="cuda")
+    ko, vo = (torch.empty(S, hkv, D, dtype=torch.float16, device="cuda") for _ in "kv")
+    grout.kv_read_paged_fp8(*pools, table, ko, vo, cu)
+    out = torch.empty(1, hq, D, dtype=torch.float16, device="cuda")
+    pos = torch.tensor([S - 1], dtype=torch.int32, device="cuda")
+    grout.attention_decode_paged_fp8(q[-1:], *pools, table, pos, out, S)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    assert torch.equal(q, q_near)
+    ck, cv = (values(c, s).transpose(1, 2).reshape(2 * ps, hkv, D)[:S] for c, s in ((near[0], near[2]), (near[1], near[3])))
+    for got, want in ((ko, ck), (vo, cv)):  # f16(code * scale): the product and the result are rounded
+        assert ((got.double() - want).abs() <= want.abs() * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25).all()
+    check(out, *attention64(q[-1:], ck, cv, pos.long(), 0, 0, SCALE_F16))

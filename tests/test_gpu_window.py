@@ -309,3 +309,154 @@ def test_graph_of_a_prefill_chunk(grout):
         grout.check_device_error()
         ref, bound = _prefill_ref(q, k, v, [0, m], [p], window, sinks)
         check(out[:m], ref, bound)
+
+
+@pytest.mark.parametrize("hq,hkv", [(3, 3), (6, 2), (7, 1), (33, 3), (100, 1), (128, 1)])
+def test_prefill_of_any_group(grout, hq, hkv):
+    """Groups that leave rows of the query tile unused, up to one token a tile."""
+    lens, firsts, n = [70, 0, 3], [500, 0, 17], 576
+    cu = torch.tensor([0] + lens).cumsum(0).tolist()
+    q = normal(17, cu[-1], hq, D, scale=1.5).half()
+    k, v = _caches(3, hkv, n, 120)
+    out = torch.full_like(q, NAN)
+    for window, sinks in ((9, 2), (300, 0)):
+        grout.attention_prefill_varlen_window(q, k, v, out, torch.tensor(cu, dtype=torch.int32, device="cuda"), 70, hkv, D, n * D, window, sinks,
+                                              kv_batch_stride=hkv * n * D, kv_rows=n,
+                                              position_start=torch.tensor(firsts, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        grout.check_device_error()
+        ref, bound = _prefill_ref(q, k, v, cu, firsts, window, sinks)
+        check(out, ref, bound)
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (8, 1), (4, 4)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (100, 4), (500, 130), (2 ** 31 - 1, 0), (2 ** 40, 2 ** 40)])
+def test_prefill_of_short_chunks(grout, hq, hkv, window, sinks):
+    """More sequences than a warp looks at together, empty ones among them, no
+    chunk longer than a query tile, contexts from one key to many tiles."""
+    B, ps, most = 75, 64, 13
+    lens = [(5 * i + 3) % (most + 1) if i % 9 else 0 for i in range(B)]
+    firsts = [(i * 83) % 1200 if i % 5 else 0 for i in range(B)]
+    ends = [a + b for a, b in zip(lens, firsts)]
+    n = max(ends)
+    cu = torch.tensor([0] + lens).cumsum(0).tolist()
+    q = normal(18, cu[-1], hq, D, scale=1.5).half()
+    k, v = _caches(B, hkv, n, 130)
+    k, v = (_hide(c, ends, window, sinks, firsts) for c in (k, v))
+    (kp, vp), table = page_pool([k, v], ps, 6)
+    out = torch.full_like(q, NAN)
+    grout.attention_prefill_paged_window(q, kp, vp, table, out, window, sinks, max_q_len=most,
+                                         cu_seqlens_q=torch.tensor(cu, dtype=torch.int32, device="cuda"),
+                                         position_start=torch.tensor(firsts, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    ref, bound = _prefill_ref(q, k, v, cu, firsts, min(window, 2 ** 30), min(sinks, 2 ** 30))
+    check(out, ref, bound)
+
+
+def test_prefill_takes_lengths_from_the_device(grout):
+    """max_q_len only sizes the launch: sequences may be longer."""
+    hq, hkv, window, sinks = 8, 2, 90, 3
+    lens, firsts = [260, 5, 100], [0, 300, 7]
+    n = 320
+    cu = torch.tensor([0] + lens).cumsum(0).tolist()
+    q = normal(19, cu[-1], hq, D).half()
+    k, v = _caches(3, hkv, n, 140)
+    for most in (1, 32, 33, 260, 4000):
+        out = torch.full_like(q, NAN)
+        grout.attention_prefill_varlen_window(q, k, v, out, torch.tensor(cu, dtype=torch.int32, device="cuda"), most, hkv, D, n * D, window, sinks,
+                                              kv_batch_stride=hkv * n * D, kv_rows=n,
+                                              position_start=torch.tensor(firsts, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        grout.check_device_error()
+        ref, bound = _prefill_ref(q, k, v, cu, firsts, window, sinks)
+        check(out, ref, bound)
+
+
+@pytest.mark.parametrize("bad", ["position", "negative", "past_rows", "decreasing"])
+@pytest.mark.parametrize("most", [4, 100])
+def test_prefill_leaves_out_what_does_not_fit(grout, bad, most):
+    """A sequence past the cache or the query rows has no items: its rows stay
+    as they were, 0x200 is recorded, the others are right."""
+    hq, hkv, ps, window, sinks = 8, 2, 64, 60, 2
+    lens, firsts, n = [4, 3, 4], [40, 100, 252], 256
+    cu = [0, 4, 7, 11]
+    q = normal(20, 11, hq, D).half()
+    k, v = _caches(3, hkv, n, 150)
+    (kp, vp), table = page_pool([k, v], ps, 7)
+    given_cu, given_first, left = list(cu), list(firsts), [1]
+    if bad == "position":
+        given_first[1] = 254
+    elif bad == "negative":
+        given_first[1] = -5
+    elif bad == "past_rows":
+        given_cu[3], left = 12, [2]
+    else:
+        given_cu[1:3], left = [7, 4], [0, 1, 2]  # rows 0..6 and 4..10 (past the cache at 252): none is checked
+    out = torch.full_like(q, 7.0)
+    grout.attention_prefill_paged_window(q, kp, vp, table, out, window, sinks, max_q_len=most,
+                                         cu_seqlens_q=torch.tensor(given_cu, dtype=torch.int32, device="cuda"),
+                                         position_start=torch.tensor(given_first, dtype=torch.int32, device="cuda"))
+    with pytest.raises(grout.GroutError, match="0x200"):
+        grout.check_device_error()
+    ref, bound = _prefill_ref(q, k, v, cu, firsts, window, sinks)
+    for b in range(3):
+        at = slice(cu[b], cu[b + 1])
+        if b not in left:
+            check(out[at], ref[at], bound[at])
+        elif bad != "decreasing":
+            assert (out[at] == 7.0).all()
+
+
+def test_offsets_past_32_bits(grout):
+    """f16 pools of more than 2^32 bytes and more than 2^31 elements: only the
+    pages at the far end are used."""
+    hq, hkv, ps, window, sinks = 8, 1, 1024, 500, 70
+    pages = 2 ** 31 // (hkv * ps * D) + 4
+    k, v = (normal(160 + i, 1, hkv, 2 * ps, D).half() for i in (0, 1))
+    kp, vp = (torch.empty(pages, hkv, ps, D, dtype=torch.float16, device="cuda") for _ in "kv")
+    table = torch.tensor([[pages - 1, pages - 3]], dtype=torch.int32, device="cuda")
+    for pool, c in ((kp, k), (vp, v)):
+        pool[pages - 1], pool[pages - 3] = c[0, :, :ps], c[0, :, ps:]
+    q = normal(21, 40, hq, D).half()
+    out = torch.empty_like(q)
+    grout.attention_prefill_paged_window(q, kp, vp, table, out, window, sinks, position_start=torch.tensor([1300], dtype=torch.int32, device="cuda"))
+    one = torch.empty_like(q[:1])
+    pos = torch.tensor([1339], dtype=torch.int32, device="cuda")
+    grout.attention_decode_paged_window(q[39:], kp, vp, table, pos, one, 2 * ps, window, sinks)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    ref, bound = _prefill_ref(q, k, v, [0, 40], [1300], window, sinks)
+    check(out, ref, bound)
+    ref, bound = attention64(q[39:], k[0].transpose(0, 1), v[0].transpose(0, 1), pos.long(), window, sinks, SCALE_F16)
+    check(one, ref, bound)
+
+
+def test_calls_on_two_streams_at_once(grout):
+    """Decode with its own workspace and a chunk, on two streams, many times:
+    the results are those of the calls alone, bit for bit."""
+    hq, hkv, n, window, sinks = 8, 1, 8192, 6000, 4
+    q = normal(22, 2, 64, hq, D).half()
+    k, v = _caches(1, hkv, n, 170)
+    pos = torch.tensor([8000], dtype=torch.int32, device="cuda")
+    first = torch.tensor([5000], dtype=torch.int32, device="cuda")
+
+    def run(i):
+        a, b = torch.full_like(q[i, :1], NAN), torch.full_like(q[i], NAN)
+        grout.attention_decode_window(q[i, :1], k, v, pos, a, n, window, sinks, num_splits=30)
+        grout.attention_prefill_varlen_window(q[i], k, v, b, None, 64, hkv, D, n * D, window, sinks, kv_rows=n, position_start=first)
+        return a, b
+
+    want = [run(i) for i in (0, 1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in (0, 1)]
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    for i in (0, 1):
+        for pair in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(pair, want[i]))

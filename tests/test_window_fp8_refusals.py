@@ -200,3 +200,15 @@ def test_python_refuses_what_is_not_on_the_gpu():
     for call in calls:
         with pytest.raises(attn.GroutError, match="CUDA tensor"):
             call()
+
+
+def test_kept_structs_follow_the_values(L):
+    """An epsilon or scale given as a tensor counts by its value at the call."""
+    t = torch.tensor(0.25)
+    assert attn._dims(8, 8, 64, t, t, 0).qk_scale == 0.25
+    t.mul_(2)
+    d = attn._dims(8, 8, 64, t, t, 0)
+    assert d.qk_scale == 0.5 and d.rms_eps == 0.5
+    # counts past 32 bits: as large (or as bad) as the largest that fits
+    assert attn.decode_window_splits(1, 4096, 2 ** 40 + 1, 0, 64, 8, 4096) == attn.decode_window_splits(1, 4096, 4096, 0, 64, 8, 4096)
+    assert attn._span(-(2 ** 40)) == -1 and attn._span(17) == 17 and attn._span(2 ** 32) == 2 ** 31 - 1
