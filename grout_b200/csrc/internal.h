@@ -127,6 +127,7 @@ struct NormRopeFp8Args {
   int32_t hkv;
   int32_t max_seq;
   float eps;
+  float neg_zero;  // -0, set by the launch (octet_norm_rope_f32x2)
   int* err;
   const int32_t* page_table;
   int64_t table_stride;

@@ -86,6 +86,75 @@ __device__ __forceinline__ void octet_norm_rope_f32(const uint4& xl, const uint4
   }
 }
 
+// ---- The same on f32x2 pairs: two correctly rounded operations an
+// instruction, so the same bits at half the instructions.  A product is formed
+// as a * b + nz with nz = -0 (exact, whatever the product's sign): mul.rn.f32x2
+// followed by add.rn.f32x2 came out contracted to one rounding; with an nz that
+// the compiler cannot know to be zero it cannot.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b, float2 nz) {
+  float2 d;
+  asm("{ .reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7};"
+      " fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d; }"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(nz.x), "f"(nz.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b;"
+      " mov.b64 {%0, %1}, d; }"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; sub.rn.f32x2 d, a, b;"
+      " mov.b64 {%0, %1}, d; }"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ void unpack4(const uint4& u, float2 (&f)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+__device__ __forceinline__ uint4 pack4(const float2 (&f)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(f[i].x, f[i].y);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void octet_norm_rope_f32x2(const uint4& xl, const uint4& xh,
+                                                      const uint4& wl, const uint4& wh,
+                                                      const float2 (&cs)[4], const float2 (&sn)[4],
+                                                      float eps, float2 nz, unsigned mask, float2 (&ylo)[4],
+                                                      float2 (&yhi)[4]) {
+  float2 lo[4], hi[4], w[4], t[4];
+  unpack4(xl, lo);
+  unpack4(xh, hi);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t[e] = add2(mul2(lo[e], lo[e], nz), mul2(hi[e], hi[e], nz));
+  float ss = __fadd_rn(__fadd_rn(__fadd_rn(t[0].x, t[0].y), __fadd_rn(t[1].x, t[1].y)),
+                       __fadd_rn(__fadd_rn(t[2].x, t[2].y), __fadd_rn(t[3].x, t[3].y)));
+#pragma unroll
+  for (int off = 4; off >= 1; off >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(mask, ss, off, 8));
+  const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 0.0078125f), eps)));
+  const float2 inv = make_float2(r, r);
+  unpack4(wl, w);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) lo[e] = mul2(mul2(lo[e], inv, nz), w[e], nz);
+  unpack4(wh, w);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) hi[e] = mul2(mul2(hi[e], inv, nz), w[e], nz);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    ylo[e] = sub2(mul2(lo[e], cs[e], nz), mul2(hi[e], sn[e], nz));
+    yhi[e] = add2(mul2(hi[e], cs[e], nz), mul2(lo[e], sn[e], nz));
+  }
+}
+
 // The same, rounded to f16 once.
 __device__ __forceinline__ void octet_norm_rope(const uint4& xl, const uint4& xh,
                                                 const float (&wl)[8], const float (&wh)[8],
