@@ -1113,10 +1113,10 @@ static int64_t window_tiles(int32_t max_kv_len, int32_t window, int32_t sinks) {
 // head, sequence) pairs.  f16 tiles stream at the memory's rate from one CTA
 // per SM; an 8-bit tile takes as long to consume and half as long to load, so
 // 8-bit calls aim at two.  Measured on B200 (64/8 heads; us, splits in
-// brackets): 8-bit, batch 1, 32768 keys: 28.8 [16], 21.3 [32], 22.7 [37]; batch
-// 4: 59.2 [5], 44.8 [8]; batch 8: 94.4 [3], 75.9 [4]; f16, batch 1, window
-// 16384: 18.8 [16], 19.2 [32]; window 1024: 7.3 [9], 8.7 [4]; batch 4, window
-// 4096: 18.0 [4], 18.4 [5], 25.2 [9].
+// brackets): 8-bit, batch 1, 32768 keys: 25.2 [16], 19.8 [32], 21.1 [37]; batch
+// 4: 61.8 [4], 49.7 [6], 42.7 [8]; batch 8: 90.3 [3], 74.1 [4]; f16, batch 1,
+// window 16384: 16.2 [16], 18.1 [32]; window 1024: 5.6 [9], 6.6 [4]; batch 4,
+// window 4096: 16.2 [4], 16.5 [6], 21.8 [9].
 static int choose_window_splits(int64_t units, int64_t tiles, int num_sms, bool fp8) {
   int64_t n = (fp8 ? num_sms * 7 / 4 : num_sms) / units;
   // shorter splits than this cost more in the merge than they save

@@ -34,6 +34,14 @@
 // Keys that are not seen get no weight and their V rows are zeroed before the
 // product, so that whatever they hold (an unwritten page, a NaN) stays out.
 //
+// Measured on B200: f16, 64 sequences, window 4096 behind 64 sinks, 64/8 heads
+// (1.09 GB): 154 us, 7.1 TB/s; 8-bit, 64 ragged sequences of up to 8192 keys,
+// 32/8 heads (0.75 GB): 112 us, 6.7 TB/s.  A 64-key tile of 8-bit keys takes a
+// group about 0.8 us; two CTAs per SM, two groups each, just keep up with the
+// memory.  One sequence is latency: 5.6 us for a window of 1024 (launch, position,
+// first tile, two merges), 19.5 us for 32768 8-bit keys (69 MB; 9 us of it
+// would be there for 1024 keys, the merge launch among them).
+//
 // Range checks on the device as in decode.cu: a position >= max_seq records
 // 0x200 and the row is zero; a page-table entry outside the pool that holds a
 // visible key records 0x201 and its tile is left out of the softmax.

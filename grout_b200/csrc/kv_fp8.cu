@@ -5,7 +5,8 @@
 // 1587-1599); the norm and rotation are those of norm_rope.cu (reference
 // src/kernels.rs:4845-5452) with the same bits, fp8.cuh says how a row is
 // quantised.  Pools: codes [num_pages][hkv][page_size][128] e4m3, scales
-// [num_pages][hkv][page_size] f32.  Both kernels are bound by HBM: every byte is read once and written once.
+// [num_pages][hkv][page_size] f32.  Every byte is read once and written once;
+// long calls are bound by HBM, a single token by latency.
 #include "fp8.cuh"
 #include "internal.h"
 #include "norm_rope.cuh"
@@ -169,7 +170,9 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkBlocks)
 // position first[b] + r - cu[b].  A warp takes kReadTasks neighbouring (row, KV
 // head) pairs: a lane each finds their sequence and cache row, then half-warps
 // turn them, K in the lower and V in the upper half, 8 codes a lane (8-byte
-// loads, 16-byte stores: both rows' 128 and 256 bytes are whole lines), all loads first.
+// loads, 16-byte stores: both rows' 128 and 256 bytes are whole lines), all
+// loads first.  Sixteen histories, 90,000 rows of 8 heads (0.56 GB): 89.5 us, 6.25
+// TB/s (a row at a time per half-warp, its sequence searched there: 109 us).
 constexpr int kReadTasks = 8;
 constexpr int kReadWarps = 8;
 __global__ void __launch_bounds__(32 * kReadWarps) kv_read_fp8_kernel(const KvReadFp8Args a) {

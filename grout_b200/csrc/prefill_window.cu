@@ -7,7 +7,7 @@
 //
 // The pipeline is prefill.cu's (persistent CTAs, 512 threads: two softmax
 // warpgroups, one output warpgroup, a TMA warp, an MMA warp; S and P in TMEM,
-// P feeds the PV MMA from there; one-pass softmax with a lazily moved
+// P feeds the PV MMA from there; one pass over the keys with a lazily moved
 // reference maximum).  What a window changes:
 //
 // Rows.  A 128-row query tile holds floor(128 / G) tokens with all G query
@@ -31,6 +31,18 @@
 // an out-of-range coordinate with zeros), and warp 14 clears the unseen
 // rows of the at most three partial blocks of an item in shared memory before
 // the MMA warp may use their V tile.
+//
+// Bound by the tensor cores and the chain S -> P -> PV -> next S of each of two
+// query tiles: in long windows a 128-key tile of both takes 3600 cycles, 2048
+// of them MMA; a chain's turn is 1300 waiting for S (PV and QK are 1024), 480
+// for the maximum, 1290 for the exponentials, 110 for the hand-over.  Measured
+// on B200: 8192 tokens, window 1024, 4 sinks, 32/8 heads: 147 us, 0.88 PFLOP/s
+// of visible keys (0.98 with the blocks' unseen keys); six chunks of up to 700
+// tokens, window 4096, 64/8 heads: 480 us, 0.93 PFLOP/s.  At that rate the GPU
+// is at its power limit (about 1.6 GHz), so that fewer cycles in the softmax
+// (masks in a pass of their own, P handed over in halves) did not shorten it.
+// 64-key blocks with two S buffers per tile took 221 us: the MMA warp could not
+// issue and wait for them as fast.
 #include "internal.h"
 #include "prefill_common.cuh"
 #include "ptx.cuh"
@@ -699,7 +711,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         // Two passes over S, a 64-key block at a time (rolled: code that is
         // unrolled over all 128 columns does not stay in the instruction
-        // cache beside the other roles' code, and leaves no registers).
+        // cache beside the other roles' code, and leaves no registers; 8192
+        // tokens, window 1024: 188 -> 161 us).
         // Pass 1: the row maximum; masked scores go back to S.
         float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
         const bool masked = j < j_lo || j >= j_hi;
