@@ -20,7 +20,6 @@ range problems raise GroutError before any launch, like the reference's
 device is not sm_100 the call raises.
 """
 import ctypes
-import functools
 import math
 import os
 
@@ -193,6 +192,29 @@ def lib():
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+_BIND_ENTRIES = (  # in the order of the binding's table
+    "grout_attn_last_error", "grout_qk_norm_rope_kv_decode_paged_fp8", "grout_qk_norm_rope_kv_prefill_paged_fp8",
+    "grout_kv_read_paged_fp8", "grout_attn_decode_window_workspace_bytes", "grout_attn_decode_window",
+    "grout_attn_decode_paged_window", "grout_attn_decode_paged_fp8", "grout_attn_prefill_varlen_window",
+    "grout_attn_prefill_paged_window",
+)
+_bind = None
+
+
+def _load_bind():
+    """The compiled binding of the window and 8-bit cache calls (csrc/bind.cpp),
+    which checks their arguments and calls into lib()."""
+    global _bind
+    L = lib()
+    try:
+        from . import _bind as b
+    except ImportError as e:
+        raise GroutError(3, f"grout_b200/_bind.so: {e}: run `python -m grout_b200.build`")
+    b.use(GroutError, tuple(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BIND_ENTRIES))
+    _bind = b
+    return b
 
 
 def _check(status):
@@ -699,110 +721,9 @@ def attention_decode_noalloc(q, k_cache, v_cache, position, out, max_kv_len, qk_
 
 # ------------------------------------- 8-bit paged cache, sliding windows
 #
-# A decode step's kernel takes a few microseconds, so what these calls do on
-# the host is kept short: one test per tensor (its message is only made when it
-# fails), and structs and sizes that depend on plain numbers alone are kept.
-
-
-# The current stream's handle without a Stream object around it: 0.07 us
-# against 1.25 us for torch.cuda.current_stream(dev).cuda_stream.
-_raw_stream = torch._C._cuda_getCurrentRawStream if torch.cuda._is_compiled() else None
-
-
-def _enqueue(dev, fn, *args):
-    """Calls fn(*args, stream) on the current stream of device dev."""
-    if dev == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev))
-    if status:
-        _check(status)
-
-
-def _refuse_tensor(t, name, dtype, dev):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
-    _need(t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
-    _need(t.is_contiguous(), f"{name} must be contiguous")
-    raise GroutError(1, f"{name} is on {t.device}, not on cuda:{dev}")
-
-
-def _device_of(t, name, dtype):
-    """The device index of t, a contiguous CUDA tensor of the type."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.is_contiguous()):
-        _refuse_tensor(t, name, dtype, None)
-    return t.get_device()
-
-
-def _cuda(t, name, dtype, dev):
-    """t must be a contiguous CUDA tensor of the type on device dev."""
-    try:
-        if t.get_device() == dev and t.dtype is dtype and t.is_contiguous():
-            return
-    except AttributeError:  # not a tensor
-        pass
-    _refuse_tensor(t, name, dtype, dev)
-
-
-def _positions(t, n, dev):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == dev and t.numel() >= n
-            and (t.dtype is torch.int32 or t.dtype is torch.uint32) and t.is_contiguous()):
-        raise GroutError(1, "position must be a contiguous device int32/uint32 tensor with one entry "
-                            f"per sequence on cuda:{dev}")
-
-
-def _table(t, batch, dev):
-    """[batch, table_stride] page table; returns the stride."""
-    _cuda(t, "page_table", torch.int32, dev)
-    if t.dim() != 2 or t.size(0) < batch:
-        raise GroutError(1, f"page_table must be [batch, table_stride]: {tuple(t.shape)}")
-    return t.size(1)
-
-
-def _kv_pages(k_pages, v_pages, dtype, dev):
-    _cuda(k_pages, "k_pages", dtype, dev)
-    _cuda(v_pages, "v_pages", dtype, dev)
-    shape = k_pages.shape
-    if len(shape) != 4 or shape[3] != HEAD_DIM:
-        raise GroutError(1, f"k_pages must be [num_pages, Hkv, page_size, 128]: {tuple(shape)}")
-    if v_pages.shape != shape:
-        raise GroutError(1, "v_pages shape mismatch")
-    return shape
-
-
-def _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev):
-    """The C struct of an 8-bit page pool, its KV heads and page size."""
-    num_pages, hkv, page_size, _ = shape = _kv_pages(k_pages, v_pages, torch.float8_e4m3fn, dev)
-    _cuda(k_scales, "k_scales", torch.float32, dev)
-    _cuda(v_scales, "v_scales", torch.float32, dev)
-    if k_scales.shape != shape[:3] or v_scales.shape != shape[:3]:
-        raise GroutError(1, "k_scales and v_scales must be [num_pages, Hkv, page_size]: "
-                            f"{tuple(k_scales.shape)}, {tuple(v_scales.shape)}")
-    return Fp8Pages(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-                    num_pages, page_size), hkv, page_size
-
-
-def _rope(t, max_seq, dev):
-    _cuda(t, "rope_table", torch.float32, dev)
-    if t.dim() != 2 or t.size(1) != HEAD_DIM or t.size(0) < max_seq:
-        raise GroutError(1, f"rope_table must be [>= max_seq={max_seq}, 128] f32: {tuple(t.shape)}")
-
-
-def _norm_weights(q_norm_w, k_norm_w, dev):
-    _cuda(q_norm_w, "q_norm_w", torch.float16, dev)
-    _cuda(k_norm_w, "k_norm_w", torch.float16, dev)
-    if q_norm_w.numel() != HEAD_DIM or k_norm_w.numel() != HEAD_DIM:
-        raise GroutError(1, "q_norm_w and k_norm_w must have 128 entries")
-
-
-@functools.lru_cache(maxsize=1024)
-def _dims_of(num_q_heads, num_kv_heads, max_seq, rms_eps, qk_scale, flags):
-    return AttnDims(num_q_heads, num_kv_heads, HEAD_DIM, max_seq, rms_eps, qk_scale, flags)
-
-
-def _dims(num_q_heads, num_kv_heads, max_seq, rms_eps, qk_scale, flags):
-    """AttnDims of these numbers (read only; floats, so that the cache is by value)."""
-    return _dims_of(num_q_heads, num_kv_heads, max_seq, float(rms_eps), float(qk_scale or 0.0), flags)
+# A decode step's kernel takes a few microseconds, so these calls go through
+# the compiled binding (csrc/bind.cpp), which checks the arguments as the
+# wrappers above do.
 
 
 def _span(n):
@@ -817,26 +738,8 @@ def qk_norm_rope_kv_decode_paged_fp8(qkv, q_norm_w, k_norm_w, rope_table, q_out,
     v_pages [num_pages, Hkv, page_size, 128] float8_e4m3fn with one f32 scale
     per row in k_scales, v_scales [num_pages, Hkv, page_size].  A row y is
     stored as scale = max|y| / 448, code = e4m3(y * (448 / max|y|))."""
-    dev = _device_of(qkv, "qkv", torch.float16)
-    _cuda(q_out, "q_out", torch.float16, dev)
-    _norm_weights(q_norm_w, k_norm_w, dev)
-    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    if hkv != num_kv_heads:
-        raise GroutError(1, f"k_pages has {hkv} KV heads, not {num_kv_heads}")
-    B = qkv.size(0) if qkv.dim() == 2 else 1
-    if qkv.numel() != B * (num_q_heads + 2 * hkv) * HEAD_DIM:
-        raise GroutError(1, f"qkv shape mismatch: {tuple(qkv.shape)}")
-    if q_out.numel() != B * num_q_heads * HEAD_DIM:
-        raise GroutError(1, f"q_out shape mismatch: {tuple(q_out.shape)}")
-    _positions(position, B, dev)
-    stride = _table(page_table, B, dev)
-    if max_seq is None:
-        max_seq = stride * page_size
-    _rope(rope_table, max_seq, dev)
-    _enqueue(dev, lib().grout_qk_norm_rope_kv_decode_paged_fp8, qkv.data_ptr(), q_norm_w.data_ptr(),
-             k_norm_w.data_ptr(), rope_table.data_ptr(), q_out.data_ptr(), pages,
-             page_table.data_ptr(), stride, position.data_ptr(), B,
-             _dims(num_q_heads, hkv, max_seq, eps, 0.0, 0))
+    (_bind or _load_bind()).write_decode(qkv, q_norm_w, k_norm_w, rope_table, q_out, k_pages, v_pages, k_scales,
+                                         v_scales, page_table, position, num_q_heads, num_kv_heads, eps, max_seq)
     return q_out
 
 
@@ -846,46 +749,9 @@ def qk_norm_rope_kv_prefill_paged_fp8(q, k, v, q_norm_w, k_norm_w, rope_table, q
     """qk_norm_rope_kv_prefill_paged into the 8-bit paged cache (see
     qk_norm_rope_kv_decode_paged_fp8): one sequence, page_table_row is its row
     of the page table."""
-    dev = _device_of(q, "q", torch.float16)
-    for t, n in ((k, "k"), (v, "v"), (q_out, "q_out")):
-        _cuda(t, n, torch.float16, dev)
-    _norm_weights(q_norm_w, k_norm_w, dev)
-    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    if q.dim() != 3 or q.size(2) != HEAD_DIM:
-        raise GroutError(1, f"q shape mismatch: {tuple(q.shape)}")
-    S, hq, _ = q.shape
-    if k.shape != (S, hkv, HEAD_DIM) or v.shape != k.shape:
-        raise GroutError(1, f"k/v shape mismatch: {tuple(k.shape)}, {tuple(v.shape)}")
-    if q_out.shape != q.shape:
-        raise GroutError(1, f"q_out shape mismatch: {tuple(q_out.shape)}")
-    _cuda(page_table_row, "page_table_row", torch.int32, dev)
-    if max_seq is None:
-        max_seq = page_table_row.numel() * page_size
-    if page_table_row.numel() * page_size < max_seq:
-        raise GroutError(1, "page_table_row shorter than max_seq")
-    _rope(rope_table, max_seq, dev)
-    _enqueue(dev, lib().grout_qk_norm_rope_kv_prefill_paged_fp8, q.data_ptr(), k.data_ptr(),
-             v.data_ptr(), hq * HEAD_DIM, hkv * HEAD_DIM, q_norm_w.data_ptr(), k_norm_w.data_ptr(),
-             rope_table.data_ptr(), q_out.data_ptr(), pages, page_table_row.data_ptr(),
-             int(position_start), S, _dims(hq, hkv, max_seq, eps, 0.0, 0))
+    (_bind or _load_bind()).write_prefill(q, k, v, q_norm_w, k_norm_w, rope_table, q_out, k_pages, v_pages, k_scales,
+                                          v_scales, page_table_row, position_start, eps, max_seq)
     return q_out
-
-
-def _cu_seqlens(t, dev):
-    """Device int32 [batch + 1]; returns the batch."""
-    _cuda(t, "cu_seqlens", torch.int32, dev)
-    if t.dim() != 1 or t.numel() < 1:
-        raise GroutError(1, f"cu_seqlens must be [batch + 1]: {tuple(t.shape)}")
-    return t.numel() - 1
-
-
-def _starts(t, batch, dev, name="position_start"):
-    if t is None:
-        return None
-    _cuda(t, name, torch.int32, dev)
-    if t.numel() < batch:
-        raise GroutError(1, f"{name} needs one entry per sequence")
-    return t.data_ptr()
 
 
 def kv_read_paged_fp8(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v_out, cu_seqlens,
@@ -897,21 +763,8 @@ def kv_read_paged_fp8(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v
     attention_prefill_varlen(_window) takes the result with kv_row_stride =
     Hkv * 128, kv_head_stride = 128, kv_start = cu_seqlens: attention of a
     chunk of new tokens over the 8-bit cache."""
-    dev = _device_of(k_out, "k_out", torch.float16)
-    _cuda(v_out, "v_out", torch.float16, dev)
-    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    shape = k_out.shape
-    if len(shape) != 3 or shape[1] != hkv or shape[2] != HEAD_DIM:
-        raise GroutError(1, f"k_out must be [rows, {hkv}, 128]: {tuple(shape)}")
-    if v_out.shape != shape:
-        raise GroutError(1, "v_out shape mismatch")
-    B = _cu_seqlens(cu_seqlens, dev)
-    start = _starts(position_start, B, dev)
-    stride = _table(page_table, B, dev)
-    _enqueue(dev, lib().grout_kv_read_paged_fp8, pages, page_table.data_ptr(), stride,
-             cu_seqlens.data_ptr(), start, B, shape[0], k_out.data_ptr(), v_out.data_ptr(),
-             hkv * HEAD_DIM,
-             _dims(hkv, hkv, stride * page_size if max_seq is None else max_seq, 0.0, 0.0, 0))
+    (_bind or _load_bind()).kv_read(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v_out, cu_seqlens,
+                                    position_start, max_seq)
     return k_out, v_out
 
 
@@ -931,67 +784,15 @@ def decode_window_workspace_bytes(batch, max_kv_len, window, sinks, num_q_heads,
                                                           num_splits, int(fp8), dims)
 
 
-@functools.lru_cache(maxsize=4096)
-def _window_need(dev, *args):
-    """decode_window_workspace_bytes on device dev (a function of the numbers alone)."""
-    with torch.cuda.device(dev):
-        return decode_window_workspace_bytes(*args)
-
-
-def _decode_window(fn, cache_args, q, out, dev, position, max_kv_len, window, sinks, num_splits,
-                   workspace, hkv, max_seq, qk_scale, scale_f16, fp8=False):
-    """The tail of the window decode calls: fn(q, *cache_args, position, out, ...)."""
-    B, hq, _ = q.shape
-    _cuda(out, "out", torch.float16, dev)
-    if out.shape != q.shape:
-        raise GroutError(1, "out shape mismatch")
-    _positions(position, B, dev)
-    num_splits = num_splits or 0
-    window, sinks = _span(window), _span(sinks)
-    ws, ws_bytes = None, 0
-    if workspace is not None:
-        if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.is_contiguous()
-                and workspace.get_device() == dev):
-            raise GroutError(1, f"workspace must be a contiguous tensor on cuda:{dev}")
-        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    else:
-        need = _window_need(dev, B, max_kv_len, window, sinks, hq, hkv, max_seq, num_splits, fp8)
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-            ws, ws_bytes = workspace.data_ptr(), need
-    _enqueue(dev, fn, q.data_ptr(), *cache_args, position.data_ptr(), out.data_ptr(), B, max_kv_len,
-             window, sinks, num_splits,
-             _dims(hq, hkv, max_seq, 0.0, qk_scale, FLAG_DECODE_SCALE_F16 if scale_f16 else 0),
-             ws, ws_bytes)
-    return out
-
-
-def _decode_query(q):
-    dev = _device_of(q, "q", torch.float16)
-    if q.dim() != 3 or q.size(2) != HEAD_DIM:
-        raise GroutError(1, f"q must be [B, Hq, 128]: {tuple(q.shape)}")
-    return dev
-
-
 def attention_decode_window(q, k_cache, v_cache, position, out, max_kv_len, window, sinks=0,
                             workspace=None, num_splits=None, qk_scale=None, scale_f16=True):
     """attention_decode over a sliding window: the query at position p sees the
     keys n <= p with n > p - window or n < sinks.  q, out [B, Hq, 128]; caches
     [B, Hkv, max_seq, 128]; only 64-key blocks that hold a visible key are
     read, the other rows may hold anything."""
-    dev = _decode_query(q)
-    _cuda(k_cache, "k_cache", torch.float16, dev)
-    _cuda(v_cache, "v_cache", torch.float16, dev)
-    shape = k_cache.shape
-    if len(shape) != 4 or shape[0] < q.size(0) or shape[3] != HEAD_DIM:
-        raise GroutError(1, f"k_cache must be [B, Hkv, max_seq, 128]: {tuple(shape)}")
-    if v_cache.shape != shape:
-        raise GroutError(1, "v_cache shape mismatch")
-    _, hkv, max_seq, _ = shape
-    return _decode_window(lib().grout_attn_decode_window,
-                          (k_cache.data_ptr(), v_cache.data_ptr(), hkv * max_seq * HEAD_DIM, max_seq * HEAD_DIM),
-                          q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
-                          max_seq, qk_scale, scale_f16)
+    (_bind or _load_bind()).decode_window(q, k_cache, v_cache, position, out, max_kv_len, window, sinks, workspace,
+                                          num_splits, qk_scale, scale_f16)
+    return out
 
 
 def attention_decode_paged_window(q, k_pages, v_pages, page_table, position, out, max_kv_len, window,
@@ -1000,14 +801,9 @@ def attention_decode_paged_window(q, k_pages, v_pages, page_table, position, out
     """attention_decode_paged over a sliding window (see
     attention_decode_window).  Pages that hold no visible key may be freed:
     their table entries are not looked at."""
-    dev = _decode_query(q)
-    num_pages, hkv, page_size, _ = _kv_pages(k_pages, v_pages, torch.float16, dev)
-    stride = _table(page_table, q.size(0), dev)
-    return _decode_window(lib().grout_attn_decode_paged_window,
-                          (k_pages.data_ptr(), v_pages.data_ptr(), num_pages, page_size,
-                           page_table.data_ptr(), stride),
-                          q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
-                          stride * page_size if max_seq is None else max_seq, qk_scale, scale_f16)
+    (_bind or _load_bind()).decode_paged_window(q, k_pages, v_pages, page_table, max_seq, position, out, max_kv_len,
+                                                window, sinks, workspace, num_splits, qk_scale, scale_f16)
+    return out
 
 
 def attention_decode_paged_fp8(q, k_pages, v_pages, k_scales, v_scales, page_table, position, out,
@@ -1016,32 +812,10 @@ def attention_decode_paged_fp8(q, k_pages, v_pages, k_scales, v_scales, page_tab
     """Split-K GQA decode over the 8-bit paged cache (see
     qk_norm_rope_kv_decode_paged_fp8); window 0 attends to the whole context,
     else as attention_decode_paged_window."""
-    dev = _decode_query(q)
-    pages, hkv, page_size = _fp8_pages(k_pages, v_pages, k_scales, v_scales, dev)
-    stride = _table(page_table, q.size(0), dev)
-    return _decode_window(lib().grout_attn_decode_paged_fp8, (pages, page_table.data_ptr(), stride),
-                          q, out, dev, position, max_kv_len, window, sinks, num_splits, workspace, hkv,
-                          stride * page_size if max_seq is None else max_seq, qk_scale, scale_f16,
-                          True)
-
-
-def _chunk_query(q, out):
-    dev = _device_of(q, "q", torch.float16)
-    if q.dim() != 3 or q.size(2) != HEAD_DIM:
-        raise GroutError(1, f"q must be [q_rows, Hq, 128]: {tuple(q.shape)}")
-    _cuda(out, "out", torch.float16, dev)
-    if out.shape != q.shape:
-        raise GroutError(1, "out shape mismatch")
-    return dev
-
-
-def _chunk_batch(cu_seqlens_q, max_q_len, rows, dev):
-    """(batch, cu_seqlens pointer, max_q_len) of a chunk call."""
-    if cu_seqlens_q is None:
-        return 1, None, rows if max_q_len is None else max_q_len
-    if max_q_len is None:
-        raise GroutError(1, "max_q_len is required with cu_seqlens_q")
-    return _cu_seqlens(cu_seqlens_q, dev), cu_seqlens_q.data_ptr(), max_q_len
+    (_bind or _load_bind()).decode_paged_fp8(q, k_pages, v_pages, k_scales, v_scales, page_table, max_seq, position,
+                                             out, max_kv_len, window, sinks, workspace, num_splits, qk_scale,
+                                             scale_f16)
+    return out
 
 
 def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads,
@@ -1051,26 +825,9 @@ def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_k
     """attention_prefill_varlen over a sliding window: the row at position p
     sees the keys n <= p with n > p - window or n < sinks.  Arguments as there;
     cu_seqlens_q None: one sequence of all q rows."""
-    dev = _chunk_query(q, out)
-    _cuda(k, "k", torch.float16, dev)
-    _cuda(v, "v", torch.float16, dev)
-    rows, hq, _ = q.shape
-    B, cu, max_q_len = _chunk_batch(cu_seqlens_q, max_q_len, rows, dev)
-    if kv_row_stride <= 0 or kv_head_stride <= 0 or kv_batch_stride < 0 or num_kv_heads <= 0:
-        raise GroutError(1, "bad kv strides")
-    # the furthest element that the strides address lies in k and v
-    fixed = max(0, B - 1) * kv_batch_stride + (num_kv_heads - 1) * kv_head_stride + HEAD_DIM
-    most = (min(k.numel(), v.numel()) - fixed) // kv_row_stride + 1
-    if kv_rows is None:
-        kv_rows = most
-    if not 0 < kv_rows <= most:
-        raise GroutError(1, f"kv_rows={kv_rows}: k and v hold {most} rows at these strides")
-    args = PrefillVarlenArgs(
-        q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k.data_ptr(), v.data_ptr(),
-        kv_batch_stride, kv_row_stride, kv_head_stride, kv_rows, cu,
-        _starts(position_start, B, dev), _starts(kv_start, B, dev, "kv_start"), B, max_q_len)
-    _enqueue(dev, lib().grout_attn_prefill_varlen_window, args, _span(window), _span(sinks),
-             _dims(hq, num_kv_heads, 1 << 30, 0.0, qk_scale, 0))
+    (_bind or _load_bind()).prefill_varlen(q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads, kv_row_stride,
+                                           kv_head_stride, window, sinks, kv_batch_stride, kv_rows, position_start,
+                                           kv_start, qk_scale)
     return out
 
 
@@ -1080,19 +837,6 @@ def attention_prefill_paged_window(q, k_pages, v_pages, page_table, out, window,
     """attention_prefill_paged over a sliding window (see
     attention_prefill_varlen_window).  Pages that hold no key a row of the
     chunk sees may be freed: their table entries are not looked at."""
-    dev = _chunk_query(q, out)
-    num_pages, hkv, page_size, _ = _kv_pages(k_pages, v_pages, torch.float16, dev)
-    rows, hq, _ = q.shape
-    B, cu, max_q_len = _chunk_batch(cu_seqlens_q, max_q_len, rows, dev)
-    stride = _table(page_table, B, dev)
-    args = PrefillPagedArgs(
-        q.data_ptr(), out.data_ptr(), hq * HEAD_DIM, rows, k_pages.data_ptr(), v_pages.data_ptr(),
-        num_pages, page_size, page_table.data_ptr(), stride, cu, _starts(position_start, B, dev), B,
-        max_q_len)
-    _enqueue(dev, lib().grout_attn_prefill_paged_window, args, _span(window), _span(sinks),
-             _dims(hq, hkv, stride * page_size if max_seq is None else max_seq, 0.0, qk_scale, 0))
+    (_bind or _load_bind()).prefill_paged(q, k_pages, v_pages, page_table, out, window, sinks, cu_seqlens_q,
+                                          position_start, max_q_len, max_seq, qk_scale)
     return out
-
-
-def default_scale(head_dim=HEAD_DIM):
-    return 1.0 / math.sqrt(head_dim)

@@ -202,13 +202,26 @@ def test_python_refuses_what_is_not_on_the_gpu():
             call()
 
 
-def test_kept_structs_follow_the_values(L):
-    """An epsilon or scale given as a tensor counts by its value at the call."""
-    t = torch.tensor(0.25)
-    assert attn._dims(8, 8, 64, t, t, 0).qk_scale == 0.25
-    t.mul_(2)
-    d = attn._dims(8, 8, 64, t, t, 0)
-    assert d.qk_scale == 0.5 and d.rms_eps == 0.5
-    # counts past 32 bits: as large (or as bad) as the largest that fits
-    assert attn.decode_window_splits(1, 4096, 2 ** 40 + 1, 0, 64, 8, 4096) == attn.decode_window_splits(1, 4096, 4096, 0, 64, 8, 4096)
-    assert attn._span(-(2 ** 40)) == -1 and attn._span(17) == 17 and attn._span(2 ** 32) == 2 ** 31 - 1
+def test_counts_past_32_bits(L):
+    """As large (or as bad) as the largest that fits, not wrapped."""
+    dims = (64, 8, 4096)
+    assert attn.decode_window_splits(1, 4096, 2 ** 40 + 1, 0, *dims) == attn.decode_window_splits(1, 4096, 4096, 0, *dims)
+    assert attn._span(-(2 ** 40)) < 0 and attn._span(17) == 17 and attn._span(2 ** 32) == 2 ** 31 - 1
+
+
+def test_binding_takes_its_arguments_only():
+    """Too few, too many or no arguments, and values that are no tensors."""
+    b = attn._load_bind()
+    names = ("write_decode", "write_prefill", "kv_read", "decode_window", "decode_paged_window", "decode_paged_fp8",
+             "prefill_varlen", "prefill_paged")
+    for name in names:
+        for n in (0, 1, 40):
+            with pytest.raises(TypeError, match="arguments"):
+                getattr(b, name)(*[None] * n)
+    for name, n in zip(names, (15, 15, 10, 12, 14, 16, 16, 12)):
+        with pytest.raises(attn.GroutError, match="CUDA tensor"):
+            getattr(b, name)(*[None] * n)
+    for bad in ((), (attn.GroutError,), (attn.GroutError, (1, 2)), (attn.GroutError, (0,) * 10)):
+        with pytest.raises((TypeError, ValueError)):
+            b.use(*bad)
+    attn._load_bind()
