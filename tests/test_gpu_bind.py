@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from window_ref import D, attention64, check, fp8_cache, normal
+from window_ref import D, SCALE_F16, attention64, check, fp8_cache, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +141,54 @@ def test_calls_from_several_threads(grout):
         t.join()
     assert not failed, failed
     grout.check_device_error()
+
+
+def test_empty_calls_and_unsigned_positions(grout):
+    """No sequences, no rows: nothing is launched, nothing is refused; positions
+    may be uint32."""
+    a = _args()
+    none = dict(q=_f16(0, HQ, D), out=_f16(0, HQ, D), position=_i32())
+    for name in NAMES[3:6]:
+        good = dict(a[name])
+        getattr(grout, name)(**{**good, **none})
+        getattr(grout, name)(**{**good, "position": good["position"].view(torch.uint32)})
+    grout.qk_norm_rope_kv_decode_paged_fp8(**{**a[NAMES[0]], "qkv": _f16(0, (HQ + 2 * HKV) * D), "q_out": _f16(0, HQ, D), "position": _i32()})
+    rows = lambda h: _f16(0, h, D)  # noqa: E731
+    grout.qk_norm_rope_kv_prefill_paged_fp8(**{**a[NAMES[1]], "q": rows(HQ), "k": rows(HKV), "v": rows(HKV), "q_out": rows(HQ)})
+    grout.kv_read_paged_fp8(**{**a[NAMES[2]], "k_out": rows(HKV), "v_out": rows(HKV), "cu_seqlens": _i32(0), "position_start": None})
+    for name in NAMES[6:]:
+        good = {k: v for k, v in a[name].items() if k not in ("position_start", "kv_start")}
+        getattr(grout, name)(**{**good, "q": rows(HQ), "out": rows(HQ), "cu_seqlens_q": None, "max_q_len": None})
+        getattr(grout, name)(**{**good, "cu_seqlens_q": _i32(0), "max_q_len": 0})
+        getattr(grout, name)(**{**good, "cu_seqlens_q": _i32(0, 0, 0), "max_q_len": 7})
+    torch.cuda.synchronize()
+    grout.check_device_error()
+
+
+def test_captured_calls_take_their_workspace_from_the_graph(grout):
+    """Two graphs and eager calls, each with a workspace of its own, in turn."""
+    n = 6000
+    q, k, v = normal(40, 1, HQ, D).half(), normal(41, 1, 1, n, D).half(), normal(42, 1, 1, n, D).half()
+    pos = _i32(0)
+    outs, graphs = [torch.empty_like(q) for _ in range(3)], []
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for out, splits in zip(outs, (20, 33)):
+            grout.attention_decode_window(q, k, v, pos, out, n, 5000, 4, num_splits=splits)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                grout.attention_decode_window(q, k, v, pos, out, n, 5000, 4, num_splits=splits)
+            graphs.append(g)
+    torch.cuda.current_stream().wait_stream(s)
+    for p in (5999, 10, 3000):
+        pos.fill_(p)
+        for g in graphs:
+            g.replay()
+        grout.attention_decode_window(q, k, v, pos, outs[2], n, 5000, 4, num_splits=40)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        grout.check_device_error()
+        for out in outs:
+            check(out, *attention64(q, k[0].transpose(0, 1), v[0].transpose(0, 1), pos.long(), 5000, 4, SCALE_F16))
