@@ -29,6 +29,8 @@ from .attn import (  # noqa: F401
     inv_freq,
     kv_read_paged_fp8,
     lib,
+    prefill_window_splits,
+    prefill_window_workspace_bytes,
     qk_norm_rope_kv_decode,
     qk_norm_rope_kv_decode_paged,
     qk_norm_rope_kv_decode_paged_fp8,

@@ -163,6 +163,8 @@ SIGNATURES = {
                                                _DIMS, _vp]),
     "grout_attn_decode_window_splits": (_i32, [_i32, _i32, _i32, _i32, _i32, _DIMS]),
     "grout_attn_decode_window_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _DIMS]),
+    "grout_attn_prefill_window_splits": (_i32, [_i32, _i32, _i64, _i32, _i32, _DIMS]),
+    "grout_attn_prefill_window_workspace_bytes": (_sz, [_i64, _i32, _DIMS]),
     "grout_attn_decode_window": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _i32,
                                                 _i32, _i32, _DIMS, _vp, _sz, _vp]),
     "grout_attn_decode_paged_window": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp,
@@ -171,9 +173,9 @@ SIGNATURES = {
     "grout_attn_decode_paged_fp8": (ctypes.c_int, [_vp, _FP8, _vp, _i32, _vp, _vp, _i32, _i32, _i32,
                                                    _i32, _i32, _DIMS, _vp, _sz, _vp]),
     "grout_attn_prefill_varlen_window": (ctypes.c_int, [ctypes.POINTER(PrefillVarlenArgs), _i32, _i32,
-                                                        _DIMS, _vp]),
+                                                        _i32, _DIMS, _vp, _sz, _vp]),
     "grout_attn_prefill_paged_window": (ctypes.c_int, [ctypes.POINTER(PrefillPagedArgs), _i32, _i32,
-                                                       _DIMS, _vp]),
+                                                       _i32, _DIMS, _vp, _sz, _vp]),
 }
 
 _lib = None
@@ -197,7 +199,8 @@ def lib():
 _BIND_ENTRIES = (  # in the order of the binding's table
     "grout_attn_last_error", "grout_qk_norm_rope_kv_decode_paged_fp8", "grout_qk_norm_rope_kv_prefill_paged_fp8",
     "grout_kv_read_paged_fp8", "grout_attn_decode_window_workspace_bytes", "grout_attn_decode_window",
-    "grout_attn_decode_paged_window", "grout_attn_decode_paged_fp8", "grout_attn_prefill_varlen_window",
+    "grout_attn_decode_paged_window", "grout_attn_decode_paged_fp8", "grout_attn_prefill_window_splits",
+    "grout_attn_prefill_window_workspace_bytes", "grout_attn_prefill_varlen_window",
     "grout_attn_prefill_paged_window",
 )
 _bind = None
@@ -784,6 +787,17 @@ def decode_window_workspace_bytes(batch, max_kv_len, window, sinks, num_q_heads,
                                                           num_splits, int(fp8), dims)
 
 
+def prefill_window_splits(batch, max_q_len, max_keys, window, sinks, num_q_heads, num_kv_heads):
+    """Split count of the window prefill calls (max_keys: kv_rows or max_seq)."""
+    dims = make_dims(num_q_heads, num_kv_heads, 1)
+    return lib().grout_attn_prefill_window_splits(batch, max_q_len, max_keys, _span(window), _span(sinks), dims)
+
+
+def prefill_window_workspace_bytes(q_rows, num_splits, num_q_heads, num_kv_heads):
+    """Workspace bytes of the window prefill calls for a split count."""
+    return lib().grout_attn_prefill_window_workspace_bytes(q_rows, num_splits, make_dims(num_q_heads, num_kv_heads, 1))
+
+
 def attention_decode_window(q, k_cache, v_cache, position, out, max_kv_len, window, sinks=0,
                             workspace=None, num_splits=None, qk_scale=None, scale_f16=True):
     """attention_decode over a sliding window: the query at position p sees the
@@ -821,22 +835,24 @@ def attention_decode_paged_fp8(q, k_pages, v_pages, k_scales, v_scales, page_tab
 def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads,
                                     kv_row_stride, kv_head_stride, window, sinks=0,
                                     kv_batch_stride=0, kv_rows=None, position_start=None,
-                                    kv_start=None, qk_scale=None):
+                                    kv_start=None, qk_scale=None, workspace=None, num_splits=None):
     """attention_prefill_varlen over a sliding window: the row at position p
     sees the keys n <= p with n > p - window or n < sinks.  Arguments as there;
-    cu_seqlens_q None: one sequence of all q rows."""
+    cu_seqlens_q None: one sequence of all q rows.  num_splits (at most 32): runs
+    that the keys of each block of rows are cut into, for few rows over a long
+    window; None: a count that suits the sizes."""
     (_bind or _load_bind()).prefill_varlen(q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads, kv_row_stride,
                                            kv_head_stride, window, sinks, kv_batch_stride, kv_rows, position_start,
-                                           kv_start, qk_scale)
+                                           kv_start, qk_scale, workspace, num_splits)
     return out
 
 
 def attention_prefill_paged_window(q, k_pages, v_pages, page_table, out, window, sinks=0,
                                    cu_seqlens_q=None, position_start=None, max_q_len=None,
-                                   max_seq=None, qk_scale=None):
+                                   max_seq=None, qk_scale=None, workspace=None, num_splits=None):
     """attention_prefill_paged over a sliding window (see
     attention_prefill_varlen_window).  Pages that hold no key a row of the
     chunk sees may be freed: their table entries are not looked at."""
     (_bind or _load_bind()).prefill_paged(q, k_pages, v_pages, page_table, out, window, sinks, cu_seqlens_q,
-                                          position_start, max_q_len, max_seq, qk_scale)
+                                          position_start, max_q_len, max_seq, qk_scale, workspace, num_splits)
     return out

@@ -1326,6 +1326,44 @@ grout_status grout_attn_decode_paged_fp8(const void* q, const grout_fp8_pages* p
 // Position arithmetic of the window prefill stays in 31 bits.
 constexpr int64_t kMaxKeys = INT32_MAX - 4096;
 
+// Split count of the window prefill: at most an item of work per SM, with
+// three 128-key tiles a split at least; the merge launch pays from about ten
+// tiles on.  Measured on B200 (us, splits in brackets): one sequence, 5 tokens, 64/8
+// heads, window 1000 (9 tiles): 14.9 [1], 15.3 [3], 13.5 [4]; 1500: 18.7 [1], 14.7
+// [4], 14.6 [8]; 4096: 38.2 [1], 18.1 [8], 18.0 [12], 24.6 [24]; 32005 keys: 276
+// [1], 52.8 [8], 40.1 [16], 51.8 [24]; 4 x 64 tokens, 16/2 heads, window 4096 (16
+// items): 69 [1], 29.7 [8], 44.6 [12]; 16 x 5 tokens, 32/8 heads, window 2000 (128
+// items): 33.3 [1], 46.4 [2].
+static int choose_prefill_window_splits(int64_t items, int64_t tiles, int num_sms) {
+  if (items <= 0 || tiles < 10) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({num_sms / items, tiles / 3, kPrefillWindowMaxSplits}));
+}
+
+int32_t grout_attn_prefill_window_splits(int32_t batch, int32_t max_q_len, int64_t max_keys,
+                                         int32_t window, int32_t sinks,
+                                         const grout_attn_dims* dims) {
+  if (!dims || batch <= 0 || batch > 65535 || max_q_len <= 0 || max_keys <= 0 || window <= 0 || sinks < 0 ||
+      dims->num_kv_heads <= 0 || dims->num_q_heads < dims->num_kv_heads)
+    return 1;
+  const int64_t group = dims->num_q_heads / dims->num_kv_heads;
+  if (group > 128) return 1;
+  const int64_t tok2 = 2 * (128 / group);
+  const int64_t items = ((int64_t)max_q_len + tok2 - 1) / tok2 * dims->num_kv_heads * batch;
+  // 64-key blocks: the sinks', and those of a window over tok2 rows that starts and ends inside blocks
+  const int64_t blocks = std::min((max_keys + 63) / 64, ((int64_t)sinks + 63) / 64 +
+                                                            (window + std::min<int64_t>(tok2, max_q_len) + 61) / 64 + 1);
+  DeviceState* ds;
+  int sms = 148;
+  if (current_state(&ds) == GROUT_OK) sms = ds->num_sms;
+  return choose_prefill_window_splits(items, (blocks + 1) / 2, sms);
+}
+
+size_t grout_attn_prefill_window_workspace_bytes(int64_t q_rows, int32_t num_splits,
+                                                 const grout_attn_dims* dims) {
+  if (!dims || q_rows <= 0 || num_splits <= 1 || dims->num_q_heads <= 0) return 0;
+  return (size_t)q_rows * dims->num_q_heads * num_splits * (128 + 1) * sizeof(float);
+}
+
 // The checks and the launch that the window prefill entry points share; `a`
 // comes with the cache fields set (max_keys: positions per sequence), dk and sk
 // are the K/V maps' dims and strides.
@@ -1334,7 +1372,8 @@ static grout_status window_prefill(PrefillWindowArgs* a, const void* q, void* ou
                                    const void* v, const uint64_t* dk, const uint64_t* sk,
                                    const int32_t* cu_seqlens_q, const int32_t* position_start,
                                    int32_t batch, int32_t max_q_len, int32_t window, int32_t sinks,
-                                   const grout_attn_dims* dims, grout_stream_t stream) {
+                                   int32_t num_splits, const grout_attn_dims* dims, void* workspace,
+                                   size_t workspace_bytes, grout_stream_t stream) {
   const int64_t hq = dims->num_q_heads, hkv = dims->num_kv_heads;
   if (!q || !out) return fail(GROUT_ERR_INVALID_ARG, "null pointer argument");
   if (!aligned16(q) || !aligned16(out))
@@ -1345,9 +1384,26 @@ static grout_status window_prefill(PrefillWindowArgs* a, const void* q, void* ou
     return fail(GROUT_ERR_INVALID_ARG, "q_row_stride=%lld", (long long)q_row_stride);
   if (q_rows <= 0 || q_rows > INT32_MAX || (!cu_seqlens_q && q_rows < max_q_len))
     return fail(GROUT_ERR_INVALID_ARG, "q_rows=%lld", (long long)q_rows);
+  if (num_splits < 0 || num_splits > kPrefillWindowMaxSplits || (num_splits > 1 && batch > 65535))
+    return fail(GROUT_ERR_INVALID_ARG, "num_splits=%d (at most %d; batch=%d, at most 65535 with splits)",
+                num_splits, kPrefillWindowMaxSplits, batch);
+  if (workspace && !aligned16(workspace))
+    return fail(GROUT_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+  if (num_splits == 0) {
+    num_splits = grout_attn_prefill_window_splits(batch, max_q_len, a->max_keys, window, sinks, dims);
+    if (!workspace || workspace_bytes < grout_attn_prefill_window_workspace_bytes(q_rows, num_splits, dims))
+      num_splits = 1;
+  }
+  const size_t need = grout_attn_prefill_window_workspace_bytes(q_rows, num_splits, dims);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(GROUT_ERR_INVALID_ARG, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,
+                workspace ? workspace_bytes : (size_t)0);
   DeviceState* ds;
   grout_status st = current_state(&ds);
   if (st != GROUT_OK) return st;
+  a->nsplit = num_splits;
+  a->part_o = need ? static_cast<float*>(workspace) : nullptr;
+  a->part_lse = need ? static_cast<float*>(workspace) + (size_t)q_rows * hq * num_splits * 128 : nullptr;
   const int32_t group = (int32_t)(hq / hkv);
   a->group = group;
   a->tok = 128 / group;
@@ -1381,8 +1437,9 @@ static grout_status window_prefill(PrefillWindowArgs* a, const void* q, void* ou
 }
 
 grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* p, int32_t window,
-                                              int32_t sinks, const grout_attn_dims* dims,
-                                              grout_stream_t stream) {
+                                              int32_t sinks, int32_t num_splits,
+                                              const grout_attn_dims* dims, void* workspace,
+                                              size_t workspace_bytes, grout_stream_t stream) {
   if (!p) return fail(GROUT_ERR_INVALID_ARG, "args is null");
   grout_status st = check_dims(dims, 128);
   if (st != GROUT_OK) return st;
@@ -1412,12 +1469,13 @@ grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* p
   a.max_keys = p->kv_rows;
   return window_prefill(&a, p->q, p->out, p->q_row_stride, p->q_rows, p->k, p->v, dk, sk,
                         p->cu_seqlens_q, p->position_start, p->batch, p->max_q_len, window, sinks,
-                        dims, stream);
+                        num_splits, dims, workspace, workspace_bytes, stream);
 }
 
 grout_status grout_attn_prefill_paged_window(const grout_prefill_paged_args* p, int32_t window,
-                                             int32_t sinks, const grout_attn_dims* dims,
-                                             grout_stream_t stream) {
+                                             int32_t sinks, int32_t num_splits,
+                                             const grout_attn_dims* dims, void* workspace,
+                                             size_t workspace_bytes, grout_stream_t stream) {
   if (!p) return fail(GROUT_ERR_INVALID_ARG, "args is null");
   grout_status st = check_dims(dims, 128);
   if (st != GROUT_OK) return st;
@@ -1443,7 +1501,7 @@ grout_status grout_attn_prefill_paged_window(const grout_prefill_paged_args* p, 
   a.max_keys = std::min<int64_t>(dims->max_seq, kMaxKeys);
   return window_prefill(&a, p->q, p->out, p->q_row_stride, p->q_rows, p->k_pages, p->v_pages, dk, sk,
                         p->cu_seqlens_q, p->position_start, p->batch, p->max_q_len, window, sinks,
-                        dims, stream);
+                        num_splits, dims, workspace, workspace_bytes, stream);
 }
 
 grout_status grout_qkv_proj_norm_rope_kv_prefill(

@@ -41,6 +41,8 @@ struct Api {
   decltype(&grout_attn_decode_window) decode_window;
   decltype(&grout_attn_decode_paged_window) decode_paged_window;
   decltype(&grout_attn_decode_paged_fp8) decode_paged_fp8;
+  decltype(&grout_attn_prefill_window_splits) prefill_splits;
+  decltype(&grout_attn_prefill_window_workspace_bytes) prefill_workspace;
   decltype(&grout_attn_prefill_varlen_window) prefill_varlen;
   decltype(&grout_attn_prefill_paged_window) prefill_paged;
 } g_api = {};
@@ -307,6 +309,29 @@ void kv_read(PyObject* const* a) {
   });
 }
 
+// The caller's workspace, or one of this call's own (given back to the
+// stream's allocator after the launch).
+struct Workspace {
+  bool given;
+  void* ptr = nullptr;
+  size_t bytes = 0;
+  at::Tensor own;
+  Workspace(PyObject* o, int dev) : given(o != Py_None) {
+    if (!given) return;
+    if (!THPVariable_Check(o) || !THPVariable_Unpack(o).is_cuda() || !THPVariable_Unpack(o).is_contiguous() ||
+        THPVariable_Unpack(o).get_device() != dev)
+      refuse("workspace must be a contiguous tensor on cuda:%d", dev);
+    ptr = THPVariable_Unpack(o).data_ptr();
+    bytes = (size_t)THPVariable_Unpack(o).nbytes();
+  }
+  void make(size_t need, const at::Tensor& like) {
+    if (!need) return;
+    own = at::empty({(int64_t)need}, like.options().dtype(at::kByte));
+    ptr = own.data_ptr();
+    bytes = need;
+  }
+};
+
 const at::Tensor& decode_query(PyObject* o, int* dev) {
   const at::Tensor& q = tensor(o, "q", at::kHalf, dev);
   if (q.dim() != 3 || q.size(2) != kD) refuse("q must be [B, Hq, 128]: %s", shape_of(q).c_str());
@@ -328,26 +353,10 @@ void decode_tail(PyObject* const* a, const at::Tensor& q, int64_t hkv, int64_t m
   if (scale_f16 < 0) throw PythonError{};
   const grout_attn_dims d =
       dims_of(q.size(1), hkv, max_seq, 0.f, scale_of(a[7]), scale_f16 ? GROUT_FLAG_DECODE_SCALE_F16 : 0);
-  void* ws = nullptr;
-  size_t bytes = 0;
-  if (a[5] != Py_None) {
-    if (!THPVariable_Check(a[5]) || !THPVariable_Unpack(a[5]).is_cuda() ||
-        !THPVariable_Unpack(a[5]).is_contiguous() || THPVariable_Unpack(a[5]).get_device() != dev)
-      refuse("workspace must be a contiguous tensor on cuda:%d", dev);
-    const at::Tensor& t = THPVariable_Unpack(a[5]);
-    ws = t.data_ptr();
-    bytes = (size_t)t.nbytes();
-  }
+  Workspace ws(a[5], dev);
   enqueue(dev, [&](grout_stream_t s) {
-    at::Tensor own;  // given back to the stream's allocator after the launch
-    if (a[5] == Py_None) {
-      bytes = g_api.decode_workspace(B, max_kv_len, window, sinks, splits, fp8 ? 1 : 0, &d);
-      if (bytes) {
-        own = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-        ws = own.data_ptr();
-      }
-    }
-    return f(pos, out.data_ptr(), B, max_kv_len, window, sinks, splits, &d, ws, bytes, s);
+    if (!ws.given) ws.make(g_api.decode_workspace(B, max_kv_len, window, sinks, splits, fp8 ? 1 : 0, &d), q);
+    return f(pos, out.data_ptr(), B, max_kv_len, window, sinks, splits, &d, ws.ptr, ws.bytes, s);
   });
 }
 
@@ -422,8 +431,27 @@ Chunk chunk_batch(PyObject* cu, PyObject* max_q_len, int64_t rows, int* dev) {
                static_cast<const int32_t*>(t.data_ptr())};
 }
 
+// The tail of the chunk calls; a: workspace, num_splits.
+template <class Args, class F>
+void chunk_call(PyObject* const* a, const at::Tensor& q, const Args& g, int64_t max_keys, int32_t window,
+                int32_t sinks, const grout_attn_dims& d, int dev, F f) {
+  Workspace ws(a[0], dev);
+  int32_t splits = a[1] == Py_None ? 0 : as_i32(a[1], "num_splits");
+  enqueue(dev, [&](grout_stream_t s) {
+    if (!ws.given) {
+      if (splits == 0) {
+        // without positions a sequence's keys are the chunk itself
+        const int64_t keys = g.position_start ? max_keys : std::min<int64_t>(max_keys, g.max_q_len);
+        splits = g_api.prefill_splits(g.batch, g.max_q_len, keys, window, sinks, &d);
+      }
+      ws.make(g_api.prefill_workspace(g.q_rows, splits, &d), q);
+    }
+    return f(&g, window, sinks, splits, &d, ws.ptr, ws.bytes, s);
+  });
+}
+
 // q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads, kv_row_stride, kv_head_stride, window, sinks,
-// kv_batch_stride, kv_rows, position_start, kv_start, qk_scale
+// kv_batch_stride, kv_rows, position_start, kv_start, qk_scale, workspace, num_splits
 void prefill_varlen(PyObject* const* a) {
   int dev = -1;
   void* out;
@@ -460,10 +488,11 @@ void prefill_varlen(PyObject* const* a) {
   g.max_q_len = c.max_q_len;
   const int32_t window = span(a[9]), sinks = span(a[10]);
   const grout_attn_dims d = dims_of(q.size(1), hkv, 1 << 30, 0.f, scale_of(a[15]), 0);
-  enqueue(dev, [&](grout_stream_t s) { return g_api.prefill_varlen(&g, window, sinks, &d, s); });
+  chunk_call(a + 16, q, g, rows, window, sinks, d, dev, g_api.prefill_varlen);
 }
 
-// q, k_pages, v_pages, page_table, out, window, sinks, cu_seqlens_q, position_start, max_q_len, max_seq, qk_scale
+// q, k_pages, v_pages, page_table, out, window, sinks, cu_seqlens_q, position_start, max_q_len, max_seq, qk_scale,
+// workspace, num_splits
 void prefill_paged(PyObject* const* a) {
   int dev = -1;
   void* out;
@@ -489,7 +518,7 @@ void prefill_paged(PyObject* const* a) {
   const int32_t window = span(a[5]), sinks = span(a[6]);
   const int64_t max_seq = a[10] == Py_None ? table.size(1) * p.page_size : as_i32(a[10], "max_seq");
   const grout_attn_dims d = dims_of(q.size(1), p.hkv, max_seq, 0.f, scale_of(a[11]), 0);
-  enqueue(dev, [&](grout_stream_t s) { return g_api.prefill_paged(&g, window, sinks, &d, s); });
+  chunk_call(a + 12, q, g, max_seq, window, sinks, d, dev, g_api.prefill_paged);
 }
 
 // Runs an entry point; C++ exceptions end here.
@@ -549,7 +578,7 @@ PyMethodDef g_methods[] = {
     {"use", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&use)), METH_FASTCALL, nullptr},
     GROUT_FN(write_decode, 15),  GROUT_FN(write_prefill, 15),       GROUT_FN(kv_read, 10),
     GROUT_FN(decode_window, 12), GROUT_FN(decode_paged_window, 14), GROUT_FN(decode_paged_fp8, 16),
-    GROUT_FN(prefill_varlen, 16), GROUT_FN(prefill_paged, 12),      {nullptr, nullptr, 0, nullptr}};
+    GROUT_FN(prefill_varlen, 18), GROUT_FN(prefill_paged, 14),      {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_bind", "Checks and calls of the window and 8-bit cache entry points.",
                         -1, g_methods};
 

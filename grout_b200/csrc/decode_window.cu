@@ -48,6 +48,7 @@
 #include "fp8.cuh"
 #include "internal.h"
 #include "ptx.cuh"
+#include "split_merge.cuh"
 
 namespace grout {
 namespace {
@@ -103,28 +104,6 @@ __device__ __forceinline__ void st_peer4(uint32_t addr, const float4& v) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y),
                "f"(v.z), "f"(v.w)
                : "memory");
-}
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  return v;
-}
-__device__ __forceinline__ void store_row4(__half* p, const float4& v, float scale) {
-  uint2 u;
-  u.x = pack_half2(v.x * scale, v.y * scale);
-  u.y = pack_half2(v.z * scale, v.w * scale);
-  *reinterpret_cast<uint2*>(p) = u;
-}
-__device__ __forceinline__ void fma4(float4& acc, float w, const float4& v) {
-  acc.x += w * v.x;
-  acc.y += w * v.y;
-  acc.z += w * v.z;
-  acc.w += w * v.w;
 }
 
 // The 64-key tiles that hold a visible key: the sinks' tiles, then those from

@@ -255,7 +255,11 @@ struct PrefillWindowArgs {
   int32_t table_stride;
   int32_t page_size;
   int32_t num_pages;
+  int32_t nsplit;       // splits of an item's keys, at most kPrefillWindowMaxSplits; 1: none
+  float* part_o;        // [q_rows][hq][nsplit][128] split results
+  float* part_lse;      // [q_rows][hq][nsplit] their log2-sum-exp
 };
+constexpr int kPrefillWindowMaxSplits = 32;
 // tm_q: 3-D {128, hq, q_rows}, box {64, hq / hkv, tok}; tm_k / tm_v: 4-D
 // {128, kv_rows, hkv, B} or {128, page_size, hkv, num_pages}, box {64, 64, 1,
 // 1}; all 128B swizzle.  max_q_len sizes the grid only.

@@ -20,6 +20,12 @@
 // (kShort), both chains take the one tile, one the even and one the odd key
 // tiles, and the output warps join the two.
 //
+// Splits.  Calls with few items and long windows cut each item's keys into
+// nsplit runs of tiles, an item of its own each (kSplit): the output warps store
+// normalised f32 rows and their log2-sum-exp, a second kernel merges them.  One
+// sequence, 5 tokens, 64/8 heads: window 4096 38 -> 18 us (8 splits), 32005 keys
+// 276 -> 40 us (16).
+//
 // Keys.  An item streams the 64-key blocks that hold a key one of its rows
 // sees (the sinks' blocks, then from the first row's window on), two blocks
 // to a 128-key tile whether they are neighbours or not.  TMA loads
@@ -43,9 +49,12 @@
 // (masks in a pass of their own, P handed over in halves) did not shorten it.
 // 64-key blocks with two S buffers per tile took 221 us: the MMA warp could not
 // issue and wait for them as fast.
+#include <algorithm>
+
 #include "internal.h"
 #include "prefill_common.cuh"
 #include "ptx.cuh"
+#include "split_merge.cuh"
 
 namespace grout {
 namespace {
@@ -140,6 +149,8 @@ __device__ __forceinline__ uint32_t bits_below(int n) {
 struct Item {
   int b, kh, q0, S, P, q_start;
   int n0, n_kv;     // KV tiles of query tile 0, of the item (tile 1 takes all)
+  int t0, last;     // (kSplit) KV tile 0 is tile t0 of the whole list; index of the list's last one
+  int sp, nch;      // (kSplit) split, number of splits that have tiles
   bool two;         // the item has a second query tile
   bool alt;         // (kShort) it has not, but two KV tiles or more: chain t takes those of parity t
   // KV tiles of chain t
@@ -156,18 +167,18 @@ struct Item {
     return k + kBlk > vis_end || (k < wlo && k + kBlk > sinks);
   }
   // whether V tile j may have rows to clear: it holds the sinks' last block, the
-  // window's first one or the item's last one
+  // window's first one or the list's last one
   __device__ __forceinline__ bool clears(int j) const {
-    return j == (sink_blk - 1) >> 1 || j == sink_blk >> 1 || j == n_kv - 1;
+    return j + t0 == (sink_blk - 1) >> 1 || j + t0 == sink_blk >> 1 || j == last;
   }
 };
 
 // Walks this CTA's items: entry r * grid + c of the list (r * grid + grid - 1
 // - c in odd rounds, so that the longer items at the front even out), which
-// numbers, sequence by sequence, token blocks in descending order, KV heads
-// fastest.  A sequence whose lengths or positions fit neither the query rows
+// numbers, sequence by sequence, token blocks in descending order, KV heads,
+// splits fastest.  A sequence whose lengths or positions fit neither the query rows
 // nor the cache has no items (device error 0x200).
-template <bool kShort>
+template <bool kShort, bool kSplit>
 struct Walk {
   int r = 0, b = -1, base = 0, cnt = 0;
   int S = 0, P = 0, pairs = 0, q_start = 0;
@@ -192,63 +203,84 @@ struct Walk {
       return;
     }
     pairs = (S + 2 * a.tok - 1) / (2 * a.tok);
-    cnt = pairs * a.hkv;
+    cnt = pairs * a.hkv * (kSplit ? a.nsplit : 1);
   }
 
   // Called by whole warps: past the current sequence, each lane reads one of
   // the next 32 (one after the other would cost a memory latency each).
   __device__ __forceinline__ bool next(const PrefillWindowArgs& a, Item& it) {
     const int G = gridDim.x, c = blockIdx.x, lane = threadIdx.x & 31;
-    const int k = r * G + ((r & 1) ? G - 1 - c : c);
-    ++r;
-    while (k >= base + cnt) {
-      if (b >= a.batch - 1) return false;
-      base += cnt;
-      Walk<kShort> w;
-      w.enter(a, b + 1 + lane);
-      int sum = w.cnt;  // of the lanes up to this one
+    for (;;) {  // (past the splits without tiles)
+      const int k = r * G + ((r & 1) ? G - 1 - c : c);
+      ++r;
+      while (k >= base + cnt) {
+        if (b >= a.batch - 1) return false;
+        base += cnt;
+        Walk w;
+        w.enter(a, b + 1 + lane);
+        int sum = w.cnt;  // of the lanes up to this one
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, sum, off);
-        if (lane >= off) sum += y;
+        for (int off = 1; off < 32; off <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, sum, off);
+          if (lane >= off) sum += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, k < base + sum);
+        const int src = hit ? __ffs(hit) - 1 : 31;
+        base += __shfl_sync(0xffffffffu, sum - w.cnt, src);
+        cnt = __shfl_sync(0xffffffffu, w.cnt, src);
+        S = __shfl_sync(0xffffffffu, w.S, src);
+        P = __shfl_sync(0xffffffffu, w.P, src);
+        pairs = __shfl_sync(0xffffffffu, w.pairs, src);
+        q_start = __shfl_sync(0xffffffffu, w.q_start, src);
+        b += 1 + src;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, k < base + sum);
-      const int src = hit ? __ffs(hit) - 1 : 31;
-      base += __shfl_sync(0xffffffffu, sum - w.cnt, src);
-      cnt = __shfl_sync(0xffffffffu, w.cnt, src);
-      S = __shfl_sync(0xffffffffu, w.S, src);
-      P = __shfl_sync(0xffffffffu, w.P, src);
-      pairs = __shfl_sync(0xffffffffu, w.pairs, src);
-      q_start = __shfl_sync(0xffffffffu, w.q_start, src);
-      b += 1 + src;
+      int local = k - base;
+      it.sp = 0;
+      if (kSplit) {
+        it.sp = local % a.nsplit;
+        local /= a.nsplit;
+      }
+      const int back = local / a.hkv;  // pairs behind this one
+      const int pair = pairs - 1 - back;
+      it.b = b;
+      it.kh = local - back * a.hkv;
+      it.S = S;
+      it.P = P;
+      it.q_start = q_start;
+      it.q0 = pair * 2 * a.tok;
+      it.two = S > it.q0 + a.tok;
+      const int end0 = P + min(it.q0 + a.tok, S);
+      it.vis_end = P + min(it.q0 + 2 * a.tok, S);
+      it.wlo = max(0, P + it.q0 - a.window + 1);
+      const int first = it.wlo / kBlk;
+      it.sink_blk = min(first, (int)(((int64_t)a.sinks + kBlk - 1) / kBlk));
+      it.skip = first - it.sink_blk;
+      it.nblk = (it.vis_end + kBlk - 1) / kBlk - it.skip;
+      it.n_kv = (it.nblk + 1) / 2;
+      it.n0 = ((end0 + kBlk - 1) / kBlk - it.skip + 1) / 2;
+      it.t0 = 0;
+      it.last = it.n_kv - 1;
+      it.nch = 1;
+      if (kSplit) {
+        // runs of tps tiles of query tile 0; the last run takes tile 1's further ones too
+        const int tps = (it.n0 + a.nsplit - 1) / a.nsplit;
+        it.nch = (it.n0 + tps - 1) / tps;
+        if (it.sp >= it.nch) continue;
+        it.t0 = it.sp * tps;
+        const int end = min(it.n0, it.t0 + tps);
+        it.n_kv = (end == it.n0 ? it.n_kv : end) - it.t0;
+        it.n0 = end - it.t0;
+        it.last -= it.t0;
+      }
+      it.alt = kShort && !it.two && it.n_kv > 1;
+      return true;
     }
-    const int local = k - base;
-    const int back = local / a.hkv;  // pairs behind this one
-    const int pair = pairs - 1 - back;
-    it.b = b;
-    it.kh = local - back * a.hkv;
-    it.S = S;
-    it.P = P;
-    it.q_start = q_start;
-    it.q0 = pair * 2 * a.tok;
-    it.two = S > it.q0 + a.tok;
-    const int end0 = P + min(it.q0 + a.tok, S);
-    it.vis_end = P + min(it.q0 + 2 * a.tok, S);
-    it.wlo = max(0, P + it.q0 - a.window + 1);
-    const int first = it.wlo / kBlk;
-    it.sink_blk = min(first, (int)(((int64_t)a.sinks + kBlk - 1) / kBlk));
-    it.skip = first - it.sink_blk;
-    it.nblk = (it.vis_end + kBlk - 1) / kBlk - it.skip;
-    it.n_kv = (it.nblk + 1) / 2;
-    it.n0 = ((end0 + kBlk - 1) / kBlk - it.skip + 1) / 2;
-    it.alt = kShort && !it.two && it.n_kv > 1;
-    return true;
   }
 };
 
 // kShort: no sequence is longer than a query tile; its items have one tile, and
 // both chains work on it (code that the other calls do not carry).
-template <bool kPaged, bool kShort>
+template <bool kPaged, bool kShort, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_window_kernel(const __grid_constant__ CUtensorMap tm_q,
                           const __grid_constant__ CUtensorMap tm_k,
@@ -294,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   auto next_item = [&](Item& x) -> bool {
     const int4 p0 = ld_shared4(place), p1 = ld_shared4(place + 16);
-    Walk<kShort> w;
+    Walk<kShort, kSplit> w;
     w.r = p0.x, w.b = p0.y, w.base = p0.z, w.cnt = p0.w;
     w.S = p1.x, w.P = p1.y, w.pairs = p1.z, w.q_start = p1.w;
     const bool has = w.next(a, x);
@@ -357,10 +389,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         it = nx;
         const int ks = a.kv_start ? a.kv_start[it.b] : 0;
         if (!(ok = load_q(0, nq0))) break;
-        int row_l = 0, outer_l = 0;  // of entry 2 * (j & ~15) + lane
+        int row_l = 0, outer_l = 0;  // of entry 2 * (t0 + (j & ~15)) + lane
         for (int j = 0; ok && j < it.n_kv; ++j) {
           if ((j & 15) == 0) {
-            const int e = 2 * j + lane;
+            const int e = 2 * (j + it.t0) + lane;
             // past the last block: an out-of-range coordinate, filled with zeros
             row_l = kPaged ? 0 : a.kv_rows;
             outer_l = kPaged ? a.num_pages : (a.kv_batched ? it.b : 0);
@@ -553,7 +585,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int iv = ring + 1;
           ok = wait(kBarFull + ring_slot(iv), ring_parity(iv), 50);
           if (!ok) break;
-          for (int e = 2 * j; e < min(2 * j + 2, it.nblk); ++e) {
+          const int e0 = 2 * (j + it.t0);
+          for (int e = e0; e < min(e0 + 2, it.nblk); ++e) {
             if (!it.partial(e, a.sinks)) continue;  // (a second block past the last is TMA's zeros)
             const int key = it.key0(e);
             const int lo0 = max(0, a.sinks - key), hi0 = min(kBlk, it.wlo - key);  // before the window
@@ -616,6 +649,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           w1 *= inv;
           const int row_q = it.q0 + t * a.tok + tok;
           const bool valid = tok < a.tok && row_q < it.S;
+          float* prow = nullptr;  // (kSplit) this split's row
+          if (kSplit && valid) {
+            const int64_t at = ((int64_t)(it.q_start + row_q) * a.hq + it.kh * G + head) * a.nsplit;
+            prow = a.part_o + (at + it.sp) * 128;
+            const float m = join ? fmaxf(row_stat(1, n0, 0), row_stat(1, n1, 1)) : row_stat(1, t ? n1 : n0, t);
+            a.part_lse[at + it.sp] = l != 0.f ? m + __log2f(l) : -INFINITY;
+            for (int s = it.nch; it.sp == 0 && s < a.nsplit; ++s) a.part_lse[at + s] = -INFINITY;
+          }
           __half* orow = a.out + (int64_t)(it.q_start + row_q) * a.q_row_stride +
                          (int64_t)(it.kh * G + head) * 128;
           const uint32_t tO = tmem + 256 + t * 128 + lane_off;
@@ -642,7 +683,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (t == 1 || join) mbar_arrive(bar(kBarOempty + 1));
               }
             }
-            if (valid) {
+            if (kSplit) {
+              float4* dst = reinterpret_cast<float4*>(prow + c * 32);
+#pragma unroll
+              for (int v = 0; v < 8; ++v)
+                if (valid)
+                  dst[v] = make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
+                                       __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3]));
+            } else if (valid) {
               uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
 #pragma unroll
               for (int v = 0; v < 4; ++v) {
@@ -674,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // hold only keys that every row of the tile sees.
     const int tok = row / a.group;
     uint32_t rec = 0, rec_next = smem_base + kOffMask + warp * 32;
-    int n_next = 0, lo_next = 0, hi_next = 0;
+    int n_next = 0, lo_next = 0, hi_next = 0, t0_next = 0;
     bool alt_next = false;
     auto next_tile = [&]() -> bool {
       Item x = {};
@@ -685,6 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) st_shared4(rec_next, first, x.sink_blk, x.skip, x.vis_end);
       __syncwarp();
       n_next = x.count(t);
+      t0_next = x.t0;
       alt_next = x.alt;
       // blocks from low_all on lie in every row's window, those before
       // first + 1 past no row's position
@@ -697,13 +746,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     bool has = next_tile();
     while (ok && has) {
-      const int n_t = n_next, j_lo = lo_next, j_hi = hi_next;
+      const int n_t = n_next, j_lo = lo_next, j_hi = hi_next, t0 = t0_next;
       const bool alt = alt_next;
       rec = rec_next;
       rec_next ^= 16;
       float m_run = -INFINITY, l = 0.f;  // m_run: the max P is exponentiated against
       for (int i = 0; i < n_t; ++i) {
-        const int j = alt ? 2 * i + t : i;  // KV tile of the item
+        const int j = t0 + (alt ? 2 * i + t : i);  // KV tile of the list
         if (i == n_t - 1) has = next_tile();  // while S is computed
         ok = wait(kBarS + t, sc, 30 + t);
         if (!ok) break;
@@ -844,11 +893,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Merge of the splits: a warp takes a (row, query head) of sequence blockIdx.y, a
+// lane four dims.  w_s = 2^(lse_s - max) / sum, out = sum_s w_s * O_s, rounded
+// once; splits without a visible key have lse = -inf; a NaN lse passes on.
+__global__ void __launch_bounds__(128) prefill_window_merge_kernel(const PrefillWindowArgs a) {
+  Walk<false, false> seq;
+  seq.enter(a, blockIdx.y);
+  if (seq.cnt == 0) return;  // no rows, or left out
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t rows = (int64_t)seq.S * a.hq;
+  for (int64_t i = (int64_t)blockIdx.x * 4 + warp; i < rows; i += (int64_t)gridDim.x * 4) {
+    const int64_t at = ((int64_t)seq.q_start * a.hq + i) * a.nsplit;
+    const float lse = lane < a.nsplit ? a.part_lse[at + lane] : -INFINITY;
+    const float M = warp_max(lse);
+    const float w = lse == -INFINITY ? 0.f : ex2(lse - M);
+    const float W = warp_sum(w);
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + at * 128) + lane;
+    const unsigned some = __ballot_sync(0xffffffffu, lse != -INFINITY);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      if (some >> s & 1) fma4(acc, ws, po[(int64_t)s * 32]);  // the others were not written
+    }
+    const int64_t row = i / a.hq;
+    store_row4(a.out + (seq.q_start + row) * a.q_row_stride + (i - row * a.hq) * 128 + 4 * lane, acc,
+               W != 0.f ? 1.f / W : 0.f);
+  }
+}
+
+template <bool kPaged, bool kShort>
+constexpr auto kernel_of(bool split) {
+  return split ? prefill_window_kernel<kPaged, kShort, true> : prefill_window_kernel<kPaged, kShort, false>;
+}
+
 }  // namespace
 
 cudaError_t prefill_window_set_attributes() {
-  for (auto k : {prefill_window_kernel<false, false>, prefill_window_kernel<true, false>,
-                 prefill_window_kernel<false, true>, prefill_window_kernel<true, true>}) {
+  for (auto k : {kernel_of<false, false>(false), kernel_of<true, false>(false), kernel_of<false, true>(false),
+                 kernel_of<true, true>(false), kernel_of<false, false>(true), kernel_of<true, false>(true),
+                 kernel_of<false, true>(true), kernel_of<true, true>(true)}) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return e;
   }
@@ -858,16 +941,21 @@ cudaError_t prefill_window_set_attributes() {
 cudaError_t launch_prefill_window(const PrefillWindowArgs& a, int32_t max_q_len, int num_sms,
                                   const CUtensorMap& tm_q, const CUtensorMap& tm_k,
                                   const CUtensorMap& tm_v, cudaStream_t s) {
-  const int64_t items = (int64_t)((max_q_len + 2 * (int64_t)a.tok - 1) / (2 * a.tok)) * a.hkv * a.batch;
+  const int64_t items =
+      (int64_t)((max_q_len + 2 * (int64_t)a.tok - 1) / (2 * a.tok)) * a.hkv * a.batch * a.nsplit;
   if (items == 0) return cudaSuccess;
   const int grid = (int)(items < num_sms ? items : num_sms);
   // Drafts of 5 tokens x 4 heads, 32 sequences, window 1024: 50 us with one
   // chain a tile, 42 with two.  Carrying that code too, long prompts took 158
   // instead of 147 us (8192 tokens) and 293 instead of 249 us (window 64).
-  const bool brief = max_q_len <= a.tok;
-  auto k = a.page_table ? (brief ? prefill_window_kernel<true, true> : prefill_window_kernel<true, false>)
-                        : (brief ? prefill_window_kernel<false, true> : prefill_window_kernel<false, false>);
+  const bool brief = max_q_len <= a.tok, split = a.nsplit > 1;
+  auto k = a.page_table ? (brief ? kernel_of<true, true>(split) : kernel_of<true, false>(split))
+                        : (brief ? kernel_of<false, true>(split) : kernel_of<false, false>(split));
   k<<<grid, kThreads, kSmemBytes, s>>>(tm_q, tm_k, tm_v, a);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !split) return e;
+  const int64_t blocks = std::min<int64_t>(((int64_t)max_q_len * a.hq + 3) / 4, 16 * num_sms);
+  prefill_window_merge_kernel<<<dim3((unsigned)blocks, (unsigned)a.batch), 128, 0, s>>>(a);
   return cudaGetLastError();
 }
 

@@ -515,6 +515,15 @@ grout_status grout_attn_decode_paged_window(const void* q, const void* k_pages,
                                             int32_t window, int32_t sinks, int32_t num_splits,
                                             const grout_attn_dims* dims, void* workspace,
                                             size_t workspace_bytes, grout_stream_t stream);
+/* Split count of the window prefill entry points for num_splits = 0 (max_keys:
+ * kv_rows or dims->max_seq, less if the caller knows that no sequence ends later),
+ * and the workspace bytes of a split count (none for 1). */
+int32_t grout_attn_prefill_window_splits(int32_t batch, int32_t max_q_len, int64_t max_keys,
+                                         int32_t window, int32_t sinks,
+                                         const grout_attn_dims* dims);
+size_t grout_attn_prefill_window_workspace_bytes(int64_t q_rows, int32_t num_splits,
+                                                 const grout_attn_dims* dims);
+
 /* Window forms of grout_attn_prefill_varlen (cu_seqlens_q may be NULL with
  * batch 1: one sequence of max_q_len rows) and grout_attn_prefill_paged;
  * arguments as there; a group of up to 128 query heads per KV head.  Keys
@@ -523,13 +532,19 @@ grout_status grout_attn_decode_paged_window(const void* q, const void* k_pages,
  * error 0x200.  Query rows are worked on in blocks of 2 * floor(128 / group)
  * neighbours: a V row that one of them sees must be finite for the others (a
  * weight of 0 times an infinity is a NaN); all other rows may hold anything.
- * A page outside the pool that holds a visible key reads as zeros (0x201). */
+ * A page outside the pool that holds a visible key reads as zeros (0x201).
+ * max_q_len sizes the launch: sequences may be longer or shorter.  num_splits: 1 to
+ * 32 runs that each query block's keys are cut into (for few rows over a long
+ * window), merged through the workspace (16-byte aligned); 0: the automatic
+ * count for kv_rows or max_seq, or 1 where the workspace does not hold it. */
 grout_status grout_attn_prefill_varlen_window(const grout_prefill_varlen_args* args,
-                                              int32_t window, int32_t sinks,
-                                              const grout_attn_dims* dims, grout_stream_t stream);
+                                              int32_t window, int32_t sinks, int32_t num_splits,
+                                              const grout_attn_dims* dims, void* workspace,
+                                              size_t workspace_bytes, grout_stream_t stream);
 grout_status grout_attn_prefill_paged_window(const grout_prefill_paged_args* args, int32_t window,
-                                             int32_t sinks, const grout_attn_dims* dims,
-                                             grout_stream_t stream);
+                                             int32_t sinks, int32_t num_splits,
+                                             const grout_attn_dims* dims, void* workspace,
+                                             size_t workspace_bytes, grout_stream_t stream);
 /* Decode over the 8-bit paged cache; window 0 (then sinks 0) = every key. */
 grout_status grout_attn_decode_paged_fp8(const void* q, const grout_fp8_pages* pages,
                                          const int32_t* page_table, int32_t table_stride,

@@ -460,3 +460,65 @@ def test_calls_on_two_streams_at_once(grout):
     for i in (0, 1):
         for pair in got[i]:
             assert all(torch.equal(x, y) for x, y in zip(pair, want[i]))
+
+
+@pytest.mark.parametrize("lens,firsts", CHUNKS + [([3] * 9, [10, 700, 0, 129, 64, 2000, 1, 1500, 333])])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (129, 70), (1000, 64), (9000, 5)])
+@pytest.mark.parametrize("page_size", [0, 192])
+@pytest.mark.parametrize("splits", [2, 5, 32])
+def test_prefill_splits(grout, lens, firsts, window, sinks, page_size, splits):
+    """Keys cut into runs, more of them than tiles among the counts: same results,
+    rows behind the last sequence left alone, whatever the workspace held."""
+    hq, hkv = 10, 2
+    B, n = len(lens), max(a + b for a, b in zip(lens, firsts))
+    cu = torch.tensor([0] + lens).cumsum(0).tolist()
+    rows = cu[-1]
+    q = torch.full((rows + 3, hq, D), NAN, device="cuda").half()
+    q[:rows] = normal(31, rows, hq, D, scale=1.5).half()
+    k, v = _caches(B, hkv, n, 180)
+    ends = [a + b for a, b in zip(lens, firsts)]
+    k, v = (_hide(c, ends, window, sinks, firsts) for c in (k, v))
+    out = torch.full_like(q, 7.0)
+    dcu, first = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (cu, firsts))
+    need = grout.prefill_window_workspace_bytes(rows + 3, splits, hq, hkv)
+    ws = torch.full((need // 4,), NAN, device="cuda")
+    if page_size:
+        (kp, vp), table = page_pool([k, v], page_size, 4)
+        table = free_pages(table, page_size, [max(0, p - window + 1) for p in firsts], sinks)
+        grout.attention_prefill_paged_window(q, kp, vp, table, out, window, sinks, cu_seqlens_q=dcu, position_start=first, max_q_len=max(lens),
+                                             workspace=ws, num_splits=splits)
+    else:
+        grout.attention_prefill_varlen_window(q, k, v, out, dcu, max(lens), hkv, D, n * D, window, sinks, kv_batch_stride=hkv * n * D, kv_rows=n,
+                                              position_start=first, workspace=ws, num_splits=splits)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    assert (out[rows:] == 7.0).all()
+    ref, bound = _prefill_ref(q, k, v, cu, firsts, window, sinks)
+    check(out[:rows], ref, bound)
+
+
+def test_prefill_of_few_rows_over_a_long_context(grout):
+    """The automatic count splits; a NaN in a seen key makes its rows NaN, a
+    sequence that does not fit is left out."""
+    hq, hkv, n, S = 16, 2, 20000, 6
+    assert grout.prefill_window_splits(1, S, n, n, 0, hq, hkv) > 8
+    q = normal(32, S, hq, D).half()
+    k, v = _caches(1, hkv, n, 190)
+    out = torch.full_like(q, NAN)
+    call = lambda p, w: grout.attention_prefill_varlen_window(q, k, v, out, None, S, hkv, D, n * D, w, 3, kv_rows=n,  # noqa: E731
+                                                              position_start=torch.tensor([p], dtype=torch.int32, device="cuda"))
+    for p in (n - S, 5000, 40, 0):
+        for w in (n, 10000):
+            call(p, w)
+            torch.cuda.synchronize()
+            grout.check_device_error()
+            ref, bound = _prefill_ref(q, k, v, [0, S], [p], w, 3)
+            check(out, ref, bound)
+    k[0, 1, 7777, 5] = NAN
+    call(15000, n)
+    assert torch.isnan(out[:, hq // 2:]).all() and torch.isfinite(out[:, : hq // 2]).all()
+    out.fill_(7.0)
+    call(n - 3, n)
+    with pytest.raises(grout.GroutError, match="0x200"):
+        grout.check_device_error()
+    assert (out == 7.0).all()

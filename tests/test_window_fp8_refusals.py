@@ -126,17 +126,17 @@ def test_read_refusals(L):
 
 
 def test_prefill_refusals(L):
-    def varlen(window=10, sinks=2, dims=None, **bad):
+    def varlen(window=10, sinks=2, dims=None, splits=1, ws=None, ws_bytes=0, **bad):
         a = attn.PrefillVarlenArgs(P, P, 64 * 128, 100, P, P, 0, 128, 4096 * 128, 4096, P, None, None, 2, 100)
         for k, v in bad.items():
             setattr(a, k, v)
-        return L.grout_attn_prefill_varlen_window(a, window, sinks, dims or _dims(), None)
+        return L.grout_attn_prefill_varlen_window(a, window, sinks, splits, dims or _dims(), ws, ws_bytes, None)
 
-    def paged(window=10, sinks=2, dims=None, **bad):
+    def paged(window=10, sinks=2, dims=None, splits=1, ws=None, ws_bytes=0, **bad):
         a = attn.PrefillPagedArgs(P, P, 64 * 128, 100, P, P, 64, 64, P, 64, P, None, 2, 100)
         for k, v in bad.items():
             setattr(a, k, v)
-        return L.grout_attn_prefill_paged_window(a, window, sinks, dims or _dims(), None)
+        return L.grout_attn_prefill_paged_window(a, window, sinks, splits, dims or _dims(), ws, ws_bytes, None)
 
     for call in (varlen, paged):
         _refused(L, 1, "window", call(window=0))
@@ -149,14 +149,43 @@ def test_prefill_refusals(L):
         _refused(L, 1, "q_row_stride", call(q_row_stride=63 * 128))
         _refused(L, 1, "batch", call(batch=-1))
         _refused(L, 2, "head_dim", call(dims=_dims(hd=64)))
+        _refused(L, 1, "num_splits", call(splits=-1))
+        _refused(L, 1, "num_splits", call(splits=33))
+        _refused(L, 1, "num_splits", call(splits=2, batch=65536, ws=P, ws_bytes=1 << 40))
+        _refused(L, 1, "workspace", call(splits=2))
+        _refused(L, 1, "workspace", call(splits=3, ws=P, ws_bytes=100 * 64 * 3 * 129 * 4 - 1))
+        _refused(L, 1, "workspace", call(splits=0, ws=ODD, ws_bytes=1 << 40))
         assert call(batch=0) == 0 and call(max_q_len=0) == 0
     _refused(L, 1, "null", varlen(k=None))
     _refused(L, 1, "kv strides", varlen(kv_row_stride=0))
     _refused(L, 1, "kv strides", varlen(kv_head_stride=12))
     _refused(L, 1, "page_size", paged(page_size=100))
     _refused(L, 1, "table_stride", paged(table_stride=63))
-    assert L.grout_attn_prefill_varlen_window(None, 1, 0, _dims(), None) == 1
-    assert L.grout_attn_prefill_paged_window(None, 1, 0, _dims(), None) == 1
+    assert L.grout_attn_prefill_varlen_window(None, 1, 0, 1, _dims(), None, 0, None) == 1
+    assert L.grout_attn_prefill_paged_window(None, 1, 0, 1, _dims(), None, 0, None) == 1
+
+
+def test_prefill_split_counts(L):
+    """One where there are items enough or the window is short, at most 32, and
+    no more than an item for each SM."""
+    count = L.grout_attn_prefill_window_splits
+    d = _dims()
+    assert count(1, 5, 1 << 20, 300, 4, d) == 1
+    assert count(1, 8192, 1 << 20, 1 << 20, 0, d) == 1
+    assert count(32, 5, 1 << 20, 1 << 20, 0, d) == 1
+    assert count(1, 5, 64, 1 << 20, 0, d) == 1
+    for bad in ((0, 5, 100, 10, 0), (1, 0, 100, 10, 0), (1, 5, 0, 10, 0), (1, 5, 100, 0, 0), (1, 5, 100, 10, -1), (65536, 1, 1 << 20, 1 << 20, 0)):
+        assert count(*bad, d) == 1
+    for B in (1, 2, 7):
+        for S in (1, 16, 17, 100, 2 ** 31 - 1):
+            for n in (1, 2000, 40000, 2 ** 31 - 1, 2 ** 62):
+                for w, sinks in ((1, 0), (2000, 4), (2 ** 31 - 1, 2 ** 31 - 1)):
+                    k = count(B, S, n, w, sinks, d)
+                    assert 1 <= k <= 32
+                    if k > 1:
+                        assert k * B * 8 * -(-S // 32) <= 148 and n >= 10 * 64
+    ws = L.grout_attn_prefill_window_workspace_bytes
+    assert ws(5, 1, d) == 0 and ws(5, 4, d) == 5 * 64 * 4 * 129 * 4
 
 
 def test_window_split_counts(L):
@@ -218,10 +247,10 @@ def test_binding_takes_its_arguments_only():
         for n in (0, 1, 40):
             with pytest.raises(TypeError, match="arguments"):
                 getattr(b, name)(*[None] * n)
-    for name, n in zip(names, (15, 15, 10, 12, 14, 16, 16, 12)):
+    for name, n in zip(names, (15, 15, 10, 12, 14, 16, 18, 14)):
         with pytest.raises(attn.GroutError, match="CUDA tensor"):
             getattr(b, name)(*[None] * n)
-    for bad in ((), (attn.GroutError,), (attn.GroutError, (1, 2)), (attn.GroutError, (0,) * 10)):
+    for bad in ((), (attn.GroutError,), (attn.GroutError, (1, 2)), (attn.GroutError, (0,) * 12)):
         with pytest.raises((TypeError, ValueError)):
             b.use(*bad)
     attn._load_bind()
