@@ -740,7 +740,7 @@ def qk_norm_rope_kv_decode_paged_fp8(qkv, q_norm_w, k_norm_w, rope_table, q_out,
     """qk_norm_rope_kv_decode_paged into the 8-bit paged cache: k_pages,
     v_pages [num_pages, Hkv, page_size, 128] float8_e4m3fn with one f32 scale
     per row in k_scales, v_scales [num_pages, Hkv, page_size].  A row y is
-    stored as scale = max|y| / 448, code = e4m3(y * (448 / max|y|))."""
+    stored as scale = max|y| / 448, code = e4m3(y * 448 / max|y|)."""
     (_bind or _load_bind()).write_decode(qkv, q_norm_w, k_norm_w, rope_table, q_out, k_pages, v_pages, k_scales,
                                          v_scales, page_table, position, num_q_heads, num_kv_heads, eps, max_seq)
     return q_out

@@ -21,7 +21,7 @@ namespace {
 // token's [Q | K | V] heads, as in norm_rope.cu.  Q rows are normalised,
 // rotated and rounded to f16; K rows are normalised, rotated and quantised
 // from f32 (one rounding, not an f16 one first); V rows are quantised.  One
-// token of 64/8 heads: 2.8 us, a launch and three dependent loads (position,
+// token of 64/8 heads: 2.6 us, a launch and three dependent loads (position,
 // page, nothing behind it): latency.
 __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRopeFp8Args a) {
   const int j = threadIdx.x & 7;  // lane within the octet
@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
   const uint32_t heads = (uint32_t)(a.hq + 2 * a.hkv);
   const uint32_t ntask = (uint32_t)a.rows * heads;  // the host keeps it and the last step below 2^32
   const uint32_t step = (gridDim.x * blockDim.x) >> 3;
+  const float2 nz = make_float2(a.neg_zero, a.neg_zero);
   for (uint32_t task = (blockIdx.x * blockDim.x + threadIdx.x) >> 3; task < ntask; task += step) {
     const uint32_t s = task / heads;
     const int hh = (int)(task - s * heads);
@@ -53,25 +54,24 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
       }
       slot = ((int64_t)page * a.hkv + kh) * a.page_size + (uint32_t)pos - pg * (uint32_t)a.page_size;
     }
-    float lo[8], hi[8];
+    float2 lo[4], hi[4];
     if (is_v) {
-      unpack8(xl, lo);
-      unpack8(xh, hi);
+      unpack4(xl, lo);
+      unpack4(xh, hi);
     } else {
-      float wl[8], wh[8], cs[8], sn[8];
+      float2 cs[4], sn[4];
       const __half* w = is_q ? a.q_w : a.k_w;
-      unpack8(ldg16(w + 8 * j), wl);
-      unpack8(ldg16(w + 64 + 8 * j), wh);
       load_cos_sin(a.table + pos * kHeadDim, j, cs, sn);
-      octet_norm_rope_f32(xl, xh, wl, wh, cs, sn, a.eps, mask, lo, hi);
+      octet_norm_rope_f32x2(xl, xh, ldg16(w + 8 * j), ldg16(w + 64 + 8 * j), cs, sn, a.eps,
+                            nz, mask, lo, hi);
     }
     if (is_q) {
       __half* dst = a.q_out + ((int64_t)s * a.hq + hh) * kHeadDim;
-      *reinterpret_cast<uint4*>(dst + 8 * j) = pack8(lo);
-      *reinterpret_cast<uint4*>(dst + 64 + 8 * j) = pack8(hi);
+      *reinterpret_cast<uint4*>(dst + 8 * j) = pack4(lo);
+      *reinterpret_cast<uint4*>(dst + 64 + 8 * j) = pack4(hi);
     } else {
       uint2 clo, chi;
-      const float scale = octet_quantise(lo, hi, mask, clo, chi);
+      const float scale = octet_quantise(lo, hi, nz, mask, clo, chi);
       uint8_t* dst = (is_v ? a.pages.v : a.pages.k) + slot * kHeadDim;
       *reinterpret_cast<uint2*>(dst + 8 * j) = clo;
       *reinterpret_cast<uint2*>(dst + 64 + 8 * j) = chi;
@@ -84,9 +84,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
 // or K and V of a KV head, over every per-th token: the norm weights stay in
 // registers, the angles are read once for two rows, and the next token's rows
 // are loaded while this one's are worked on.  4096 tokens of 64/8 heads (161
-// MB): 32.0 us, 5.0 TB/s; a row per octet and scalar arithmetic took 35.1 us,
+// MB): 33.5 us, 4.8 TB/s; a row per octet and scalar arithmetic took 35.1 us,
 // the schedulers issuing in 72 % of the cycles and L1 busy with angles for 61 %.
-// 5 blocks of 128 threads (96 registers): 33.2 with 4, 35.1 with 6 (spills).
+// 5 blocks of 128 threads (96 registers): 4 % slower with 4, 10 % with 6 (spills).
 constexpr int kChunkThreads = 128;
 constexpr int kChunkBlocks = 5;  // per SM
 __global__ void __launch_bounds__(kChunkThreads, kChunkBlocks)
@@ -123,8 +123,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkBlocks)
     const uint4 x0 = nx[0], x1 = nx[1], x2 = nx[2], x3 = nx[3];
     const int pos = a.pos0 + s;
     float2 cs[4], sn[4];
-    load_cos_sin(a.table + (int64_t)pos * kHeadDim, j, reinterpret_cast<float(&)[8]>(cs),
-                 reinterpret_cast<float(&)[8]>(sn));
+    load_cos_sin(a.table + (int64_t)pos * kHeadDim, j, cs, sn);
     int32_t page = 0;
     uint32_t in_page = 0;
     if (!is_q) {
@@ -155,8 +154,7 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkBlocks)
           unpack4(x3, hi);
         }
         uint2 clo, chi;
-        const float scale = octet_quantise(reinterpret_cast<float(&)[8]>(lo),
-                                           reinterpret_cast<float(&)[8]>(hi), mask, clo, chi);
+        const float scale = octet_quantise(lo, hi, nz, mask, clo, chi);
         uint8_t* dst = (row ? a.pages.v : a.pages.k) + slot * kHeadDim + 8 * j;
         *reinterpret_cast<uint2*>(dst) = clo;
         *reinterpret_cast<uint2*>(dst + 64) = chi;

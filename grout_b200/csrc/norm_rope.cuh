@@ -57,13 +57,13 @@ __device__ __forceinline__ void load_cos_sin(const float* trow, int j, float (&c
 }
 
 // RMSNorm of the octet's row (x = [xl | xh] as lane j's 16-byte chunks),
-// scaled by the norm weight (wl, wh) and rotated by (cs, sn), in f32.  `mask`
-// is the octet's lane mask for the butterfly.
-__device__ __forceinline__ void octet_norm_rope_f32(const uint4& xl, const uint4& xh,
-                                                    const float (&wl)[8], const float (&wh)[8],
-                                                    const float (&cs)[8], const float (&sn)[8],
-                                                    float eps, unsigned mask, float (&ylo)[8],
-                                                    float (&yhi)[8]) {
+// scaled by the norm weight (wl, wh), rotated by (cs, sn) and rounded to f16
+// once.  `mask` is the octet's lane mask for the butterfly.
+__device__ __forceinline__ void octet_norm_rope(const uint4& xl, const uint4& xh,
+                                                const float (&wl)[8], const float (&wh)[8],
+                                                const float (&cs)[8], const float (&sn)[8],
+                                                float eps, unsigned mask, uint4& out_lo,
+                                                uint4& out_hi) {
   float lo[8], hi[8];
   unpack8(xl, lo);
   unpack8(xh, hi);
@@ -77,6 +77,7 @@ __device__ __forceinline__ void octet_norm_rope_f32(const uint4& xl, const uint4
   // ss / 128 is an exact power-of-two scaling; the correctly rounded
   // reciprocal equals the IEEE quotient 1.0f / x.
   const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 0.0078125f), eps)));
+  float ylo[8], yhi[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float nlo = __fmul_rn(__fmul_rn(lo[e], inv), wl[e]);
@@ -84,20 +85,23 @@ __device__ __forceinline__ void octet_norm_rope_f32(const uint4& xl, const uint4
     ylo[e] = __fsub_rn(__fmul_rn(nlo, cs[e]), __fmul_rn(nhi, sn[e]));
     yhi[e] = __fadd_rn(__fmul_rn(nhi, cs[e]), __fmul_rn(nlo, sn[e]));
   }
+  out_lo = pack8(ylo);
+  out_hi = pack8(yhi);
 }
 
-// ---- The same on f32x2 pairs: two correctly rounded operations an
+// ---- The same, without the rounding to f16, on f32x2 pairs: two correctly rounded operations an
 // instruction, so the same bits at half the instructions.  A product is formed
 // as a * b + nz with nz = -0 (exact, whatever the product's sign): mul.rn.f32x2
 // followed by add.rn.f32x2 came out contracted to one rounding; with an nz that
 // the compiler cannot know to be zero it cannot.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b, float2 nz) {
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
   asm("{ .reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7};"
       " fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d; }"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(nz.x), "f"(nz.y));
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b, float2 nz) { return fma2(a, b, nz); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
   asm("{ .reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b;"
@@ -126,6 +130,16 @@ __device__ __forceinline__ uint4 pack4(const float2 (&f)[4]) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+__device__ __forceinline__ void load_cos_sin(const float* trow, int j, float2 (&cs)[4], float2 (&sn)[4]) {
+  const float4 c0 = __ldg(reinterpret_cast<const float4*>(trow + 8 * j));
+  const float4 c1 = __ldg(reinterpret_cast<const float4*>(trow + 8 * j + 4));
+  const float4 s0 = __ldg(reinterpret_cast<const float4*>(trow + 64 + 8 * j));
+  const float4 s1 = __ldg(reinterpret_cast<const float4*>(trow + 64 + 8 * j + 4));
+  cs[0] = make_float2(c0.x, c0.y), cs[1] = make_float2(c0.z, c0.w);
+  cs[2] = make_float2(c1.x, c1.y), cs[3] = make_float2(c1.z, c1.w);
+  sn[0] = make_float2(s0.x, s0.y), sn[1] = make_float2(s0.z, s0.w);
+  sn[2] = make_float2(s1.x, s1.y), sn[3] = make_float2(s1.z, s1.w);
+}
 __device__ __forceinline__ void octet_norm_rope_f32x2(const uint4& xl, const uint4& xh,
                                                       const uint4& wl, const uint4& wh,
                                                       const float2 (&cs)[4], const float2 (&sn)[4],
@@ -153,18 +167,6 @@ __device__ __forceinline__ void octet_norm_rope_f32x2(const uint4& xl, const uin
     ylo[e] = sub2(mul2(lo[e], cs[e], nz), mul2(hi[e], sn[e], nz));
     yhi[e] = add2(mul2(hi[e], cs[e], nz), mul2(lo[e], sn[e], nz));
   }
-}
-
-// The same, rounded to f16 once.
-__device__ __forceinline__ void octet_norm_rope(const uint4& xl, const uint4& xh,
-                                                const float (&wl)[8], const float (&wh)[8],
-                                                const float (&cs)[8], const float (&sn)[8],
-                                                float eps, unsigned mask, uint4& out_lo,
-                                                uint4& out_hi) {
-  float ylo[8], yhi[8];
-  octet_norm_rope_f32(xl, xh, wl, wh, cs, sn, eps, mask, ylo, yhi);
-  out_lo = pack8(ylo);
-  out_hi = pack8(yhi);
 }
 
 }  // namespace grout

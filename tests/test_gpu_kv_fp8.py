@@ -33,12 +33,11 @@ def _norm_rope32(x, w, tab, pos):
 
 
 def _quantise32(y):
-    """f32 rows -> (code bytes, scales), the same operations in the same order."""
+    """f32 rows -> (code bytes, scales): quotient and scale rounded to f32 once."""
     top = np.abs(y).max(-1)
     zero = top <= 2.0 ** -25
-    with np.errstate(divide="ignore"):
-        inv = np.where(zero, np.float32(0), np.float32(448) / top).astype(np.float32)
-    x = np.clip(y * inv[..., None], -448, 448).astype(np.float32)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        x = np.where(zero[..., None], y * np.float32(0), y * np.float32(448) / top[..., None]).astype(np.float32)
     code = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
     return code, np.where(zero, np.float32(0), top / np.float32(448)).astype(np.float32)
 
@@ -384,3 +383,35 @@ def test_offsets_past_32_bits(grout):
     for got, want in ((ko, ck), (vo, cv)):  # f16(code * scale): the product and the result are rounded
         assert ((got.double() - want).abs() <= want.abs() * (2.0 ** -11 + 2.0 ** -23) + 2.0 ** -25).all()
     check(out, *attention64(q[-1:], ck, cv, pos.long(), 0, 0, SCALE_F16))
+
+
+def test_codes_are_those_of_the_formula(grout):
+    """V's codes against y * 448 / max|y| in 64 bits, bit for bit: rows that are
+    full of ties (the quotient midway between two codes), f16's whole range of
+    largest values, signed zeros."""
+    hkv, ps, S = 2, 1024, 1024
+    g = torch.Generator().manual_seed(9)
+    y = torch.randint(-2047, 2048, (S, hkv, D), generator=g).double()
+    top = torch.randint(1, 293, (S, hkv, 1), generator=g).double() * 7  # max = 7 t: y = 64 max (odd / 2^n) / 448 = t odd / 2^n is a tie
+    odd = torch.randint(1, 32, (S, hkv, D), generator=g).double() * 2 - 1
+    tie = odd * (top / 7) / 2.0 ** torch.randint(0, 3, (S, hkv, D), generator=g)
+    y = torch.where((torch.arange(S) % 2 == 0)[:, None, None] & (tie.abs() < top) & (tie.half().double() == tie), tie * torch.sign(y + 0.5), y.clamp(-top, top))
+    y[:, :, 3] = top[:, :, 0]
+    y[5, 0], y[6, 1, ::2] = -0.0, -0.0
+    v = (y * 2.0 ** torch.randint(-20, 5, (S, hkv, 1), generator=g)).half().cuda()
+    q, w = torch.zeros(S, 1 * hkv, D, dtype=torch.float16, device="cuda"), torch.ones(D, dtype=torch.float16, device="cuda")
+    pools, table = _pools(1, hkv, ps), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    grout.qk_norm_rope_kv_prefill_paged_fp8(q, torch.zeros_like(v), v, w, w, grout.rope_table(THETA, ps), torch.empty_like(q), *pools, table[0], 0, EPS)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    x = v.double()
+    m = x.abs().amax(-1, keepdim=True)
+    x = torch.where(m <= 2.0 ** -25, x * 0, x * 448 / m)
+    step = torch.exp2(torch.floor(torch.log2(x.abs().clamp(min=2.0 ** -30))).clamp(min=-6) - 3)
+    ties = ((x / step).abs() % 1 == 0.5).sum().item()
+    assert ties > 1000, ties
+    want = (torch.round(x / step) * step).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    got = pools[1].view(torch.uint8)[0].transpose(0, 1)
+    differ = (got != want) & ~((got & 0x7F == 0) & (want & 0x7F == 0))  # (the sign of a code that rounds to zero is torch.round's)
+    assert not differ.any(), differ.sum().item()
+    assert (got[5, 0] & 0x7F == 0).all() and (got[6, 1, ::2] == 0x80).all()
