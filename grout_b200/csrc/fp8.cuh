@@ -2,8 +2,7 @@
 //
 // A cache row (one token, one KV head) is 128 e4m3 codes and one f32 scale:
 //   scale = max|y| / 448, code = e4m3(y * 448 / max|y|),
-// scale and quotient rounded to f32 once, the code rounded to nearest even and
-// saturated.
+// the scale rounded to f32 once, the code to nearest even and saturated.
 // The row's largest value so uses e4m3's whole range; its smaller values keep
 // 3 mantissa bits down to max|y| / 28672 (the smallest normal code, 2^-6) and
 // a fixed step of max|y| / 229376 below that.  A row whose values an f16 cache would all round to
@@ -43,11 +42,14 @@ __device__ __forceinline__ uint32_t f16x2_of_e4m3_hi(uint32_t codes) {
 }
 // Quantises an octet's row: lane j holds elements 8j..8j+7 (lo) and
 // 64+8j..64+8j+7 (hi).  codes_lo/hi are the lane's 8-byte chunks; returns the
-// row's scale (the same in every lane).  q = y * f32(448 / max) carries two
-// roundings, which now and then turn a tie between two codes to the wrong side;
-// the residual 448 y - q * max (448 y is exact for f16 y) corrects it to the
-// quotient rounded once, and V's codes are the formula's bit for bit.  (4096 tokens,
-// 64/8 heads: 32.0 -> 33.5 us.)
+// row's scale (the same in every lane).  q = y * f32(448 f32(1 / max)) carries
+// three roundings, which now and then turn a value next to a tie between two
+// codes to the wrong side.  kExact (for V: f16 values, 448 y is exact): the
+// residual 448 y - q * max corrects it to the quotient rounded once, so the codes
+// are the formula's bit for bit.  K's f32 values carry the norm's roundings, which
+// do the same as often: there the correction would buy nothing.  (4096
+// tokens, 64/8 heads: 32.0 us without, 33.3 on V, 33.5 on both.)
+template <bool kExact>
 __device__ __forceinline__ float octet_quantise(const float2 (&lo)[4], const float2 (&hi)[4],
                                                 float2 nz, unsigned mask, uint2& codes_lo,
                                                 uint2& codes_hi) {
@@ -58,13 +60,13 @@ __device__ __forceinline__ float octet_quantise(const float2 (&lo)[4], const flo
 #pragma unroll
   for (int off = 4; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, off, 8));
   const bool zero = top <= kFp8ZeroRow;
-  const float inv = zero ? 0.f : __fdiv_rn(kE4m3Max, top);
-  const float rcp = inv * (1.f / kE4m3Max);
+  const float rcp = zero ? 0.f : __frcp_rn(top);
+  const float inv = __fmul_rn(rcp, kE4m3Max);
   const float2 inv2 = make_float2(inv, inv), nrcp2 = make_float2(-rcp, -rcp), top2 = make_float2(top, top),
                nmost = make_float2(-kE4m3Max, -kE4m3Max);
   const auto quotient = [&](const float2& y) {  // (the residual negated: -0 stays -0)
     const float2 q = mul2(y, inv2, nz);
-    return fma2(fma2(q, top2, mul2(y, nmost, nz)), nrcp2, q);
+    return kExact ? fma2(fma2(q, top2, mul2(y, nmost, nz)), nrcp2, q) : q;
   };
   float2 a[4], b[4];
 #pragma unroll

@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
       *reinterpret_cast<uint4*>(dst + 64 + 8 * j) = pack4(hi);
     } else {
       uint2 clo, chi;
-      const float scale = octet_quantise(lo, hi, nz, mask, clo, chi);
+      const float scale = is_v ? octet_quantise<true>(lo, hi, nz, mask, clo, chi)
+                               : octet_quantise<false>(lo, hi, nz, mask, clo, chi);
       uint8_t* dst = (is_v ? a.pages.v : a.pages.k) + slot * kHeadDim;
       *reinterpret_cast<uint2*>(dst + 8 * j) = clo;
       *reinterpret_cast<uint2*>(dst + 64 + 8 * j) = chi;
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
 // or K and V of a KV head, over every per-th token: the norm weights stay in
 // registers, the angles are read once for two rows, and the next token's rows
 // are loaded while this one's are worked on.  4096 tokens of 64/8 heads (161
-// MB): 33.5 us, 4.8 TB/s; a row per octet and scalar arithmetic took 35.1 us,
+// MB): 33.3 us, 4.9 TB/s; a row per octet and scalar arithmetic took 35.1 us,
 // the schedulers issuing in 72 % of the cycles and L1 busy with angles for 61 %.
 // 5 blocks of 128 threads (96 registers): 4 % slower with 4, 10 % with 6 (spills).
 constexpr int kChunkThreads = 128;
@@ -154,7 +155,8 @@ __global__ void __launch_bounds__(kChunkThreads, kChunkBlocks)
           unpack4(x3, hi);
         }
         uint2 clo, chi;
-        const float scale = octet_quantise(lo, hi, nz, mask, clo, chi);
+        const float scale = row ? octet_quantise<true>(lo, hi, nz, mask, clo, chi)
+                                : octet_quantise<false>(lo, hi, nz, mask, clo, chi);
         uint8_t* dst = (row ? a.pages.v : a.pages.k) + slot * kHeadDim + 8 * j;
         *reinterpret_cast<uint2*>(dst) = clo;
         *reinterpret_cast<uint2*>(dst + 64) = chi;

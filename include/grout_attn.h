@@ -434,9 +434,10 @@ grout_status grout_qk_norm_rope_kv_prefill_paged(
  *   k, v: [num_pages][num_kv_heads][page_size][128] e4m3 (one byte);
  *   k_scales, v_scales: [num_pages][num_kv_heads][page_size] f32;
  *   row y is stored as scale = max|y| / 448, code = e4m3(y * 448 / max|y|),
- *   the quotient rounded once, nearest even, and stands for code * scale; a row with max|y| <= 2^-25 is
- *   stored as zeros with scale 0.  A NaN stays a NaN, a row with an infinity
- *   reads back as NaN.
+ *   nearest even, and stands for code * scale (V's codes are exactly these, K's
+ *   carry the f32 roundings of its norm, rotation and factor 448 / max); a row
+ *   with max|y| <= 2^-25 is stored as zeros with scale 0.  A NaN stays a NaN, a
+ *   row with an infinity reads back as NaN.
  * page_size, page_table and bad table entries as for the f16 paged caches
  * (below 0 or >= num_pages: device error 0x201, writes skip the row,
  * attention leaves the tile out, read-back gives zeros). */

@@ -32,12 +32,14 @@ def _norm_rope32(x, w, tab, pos):
     return np.concatenate([lo * cos - hi * sin, hi * cos + lo * sin], -1)
 
 
-def _quantise32(y):
-    """f32 rows -> (code bytes, scales): quotient and scale rounded to f32 once."""
+def _quantise32(y, exact):
+    """f32 rows -> (code bytes, scales); exact (V): the quotient rounded to f32
+    once, else (K) y times the factor 448 (1 / max), each step rounded."""
     top = np.abs(y).max(-1)
     zero = top <= 2.0 ** -25
     with np.errstate(divide="ignore", invalid="ignore"):
-        x = np.where(zero[..., None], y * np.float32(0), y * np.float32(448) / top[..., None]).astype(np.float32)
+        x = y * np.float32(448) / top[..., None] if exact else y * (np.float32(448) * (np.float32(1) / top))[..., None]
+        x = np.where(zero[..., None], y * np.float32(0), x).astype(np.float32)
     code = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
     return code, np.where(zero, np.float32(0), top / np.float32(448)).astype(np.float32)
 
@@ -54,7 +56,7 @@ def _expect(pools, table, rows, ks, vs, ps):
     codes = [w.view(torch.uint8).cpu().numpy() for w in want[:2]]
     scales = [w.cpu().numpy() for w in want[2:]]
     for y, code, scale in ((ks, codes[0], scales[0]), (vs, codes[1], scales[1])):
-        c, s = _quantise32(y)
+        c, s = _quantise32(y, y is vs)
         for i, (b, p) in enumerate(rows):
             page = int(table[b, p // ps])
             code[page, :, p % ps] = c[i]
