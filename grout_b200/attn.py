@@ -840,7 +840,8 @@ def attention_prefill_varlen_window(q, k, v, out, cu_seqlens_q, max_q_len, num_k
     sees the keys n <= p with n > p - window or n < sinks.  Arguments as there;
     cu_seqlens_q None: one sequence of all q rows.  num_splits (at most 32): runs
     that the keys of each block of rows are cut into, for few rows over a long
-    window; None: a count that suits the sizes."""
+    window; None: a count that suits the sizes (and a workspace of the call's own of
+    64 MB, which counts every row of q)."""
     (_bind or _load_bind()).prefill_varlen(q, k, v, out, cu_seqlens_q, max_q_len, num_kv_heads, kv_row_stride,
                                            kv_head_stride, window, sinks, kv_batch_stride, kv_rows, position_start,
                                            kv_start, qk_scale, workspace, num_splits)

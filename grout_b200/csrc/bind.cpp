@@ -431,6 +431,8 @@ Chunk chunk_batch(PyObject* cu, PyObject* max_q_len, int64_t rows, int* dev) {
                static_cast<const int32_t*>(t.data_ptr())};
 }
 
+constexpr size_t kOwnWorkspace = 64u << 20;
+
 // The tail of the chunk calls; a: workspace, num_splits.
 template <class Args, class F>
 void chunk_call(PyObject* const* a, const at::Tensor& q, const Args& g, int64_t max_keys, int32_t window,
@@ -443,6 +445,10 @@ void chunk_call(PyObject* const* a, const at::Tensor& q, const Args& g, int64_t 
         // without positions a sequence's keys are the chunk itself
         const int64_t keys = g.position_start ? max_keys : std::min<int64_t>(max_keys, g.max_q_len);
         splits = g_api.prefill_splits(g.batch, g.max_q_len, keys, window, sinks, &d);
+        // An item of work per SM needs 20 MB at most; rows of q that no sequence
+        // has would need theirs too.
+        const size_t one = g_api.prefill_workspace(g.q_rows, 2, &d) / 2;
+        if (one) splits = (int32_t)std::min<size_t>(splits, std::max<size_t>(1, kOwnWorkspace / one));
       }
       ws.make(g_api.prefill_workspace(g.q_rows, splits, &d), q);
     }

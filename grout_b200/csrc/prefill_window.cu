@@ -954,7 +954,8 @@ cudaError_t launch_prefill_window(const PrefillWindowArgs& a, int32_t max_q_len,
   k<<<grid, kThreads, kSmemBytes, s>>>(tm_q, tm_k, tm_v, a);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !split) return e;
-  const int64_t blocks = std::min<int64_t>(((int64_t)max_q_len * a.hq + 3) / 4, 16 * num_sms);
+  const int64_t blocks = std::min<int64_t>(((int64_t)max_q_len * a.hq + 3) / 4,
+                                           std::max(1, 16 * num_sms / a.batch));
   prefill_window_merge_kernel<<<dim3((unsigned)blocks, (unsigned)a.batch), 128, 0, s>>>(a);
   return cudaGetLastError();
 }

@@ -522,3 +522,44 @@ def test_prefill_of_few_rows_over_a_long_context(grout):
     with pytest.raises(grout.GroutError, match="0x200"):
         grout.check_device_error()
     assert (out == 7.0).all()
+
+
+def test_split_prefill_in_a_graph_and_with_spare_rows(grout):
+    """The automatic split recorded once and replayed at other positions, lengths
+    and beside eager calls; a q of many spare rows is not split beyond its
+    workspace."""
+    hq, hkv, n, ps = 8, 2, 6000, 64
+    q = normal(33, 12, hq, D).half()
+    k, v = _caches(2, hkv, n, 200)
+    (kp, vp), table = page_pool([k, v], ps, 8)
+    cu, first = torch.tensor([0, 5, 12], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    assert grout.prefill_window_splits(2, 7, table.shape[1] * ps, 3500, 4, hq, hkv) > 4
+    outs = [torch.full_like(q, 7.0) for _ in range(2)]
+    call = lambda x, o: grout.attention_prefill_paged_window(x, kp, vp, table, o, 3500, 4, cu_seqlens_q=cu, position_start=first, max_q_len=7)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call(q, outs[0])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            call(q, outs[0])
+    torch.cuda.current_stream().wait_stream(s)
+    spare = torch.zeros(30000, hq, D, dtype=torch.float16, device="cuda")
+    spare[:12] = q
+    wide = torch.full_like(spare, 7.0)
+    for lens, at in (([5, 7], [5000, 100]), ([1, 2], [0, 5900]), ([0, 7], [9, 4000])):
+        cu.copy_(torch.tensor([0, lens[0], sum(lens)]))
+        first.copy_(torch.tensor(at))
+        for o in outs + [wide]:
+            o.fill_(7.0)
+        g.replay()
+        call(q, outs[1])
+        g.replay()
+        call(spare, wide)
+        torch.cuda.synchronize()
+        grout.check_device_error()
+        m = sum(lens)
+        ref, bound = _prefill_ref(q, k, v, [0, lens[0], m], at, 3500, 4)
+        for o in outs + [wide]:
+            check(o[:m], ref, bound)
+            assert (o[m:] == 7.0).all()
