@@ -722,6 +722,10 @@ def attention_decode_noalloc(q, k_cache, v_cache, position, out, max_kv_len, qk_
     return out
 
 
+def default_scale(head_dim=HEAD_DIM):
+    return 1.0 / math.sqrt(head_dim)
+
+
 # ------------------------------------- 8-bit paged cache, sliding windows
 #
 # A decode step's kernel takes a few microseconds, so these calls go through
