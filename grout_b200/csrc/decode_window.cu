@@ -106,6 +106,12 @@ __device__ __forceinline__ void st_peer4(uint32_t addr, const float4& v) {
                : "memory");
 }
 
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // The 64-key tiles that hold a visible key: the sinks' tiles, then those from
 // the window's first key on.  Entry i is tile i or, past the sinks, i + skip.
 struct TileList {
@@ -284,9 +290,11 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
         const float* sp = scales + 2 * st * kKeys + k16 + g;
         f0 *= sp[0];
         f1 *= sp[8];
-        // a zero row (scale 0) has zero codes: any positive scale serves
-        v0 = fmaxf(sp[kKeys], 0x1p-60f);
-        v1 = fmaxf(sp[kKeys + 8], 0x1p-60f);
+        // A zero row (scale 0) has zero codes: any positive scale serves.  (Below
+        // 2^-60 a row's values are under 2^-51, which no f16 output shows.)  A
+        // NaN stays one, as in the read-back.
+        v0 = fmax_nan(sp[kKeys], 0x1p-60f);
+        v1 = fmax_nan(sp[kKeys + 8], 0x1p-60f);
       }
       constexpr int kFrag = kFp8 ? 4 : 8;
       uint32_t kf[kFrag][4], vf[kFrag][4];

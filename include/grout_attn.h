@@ -437,7 +437,9 @@ grout_status grout_qk_norm_rope_kv_prefill_paged(
  *   nearest even, and stands for code * scale (V's codes are exactly these, K's
  *   carry the f32 roundings of its norm, rotation and factor 448 / max); a row
  *   with max|y| <= 2^-25 is stored as zeros with scale 0.  A NaN stays a NaN, a
- *   row with an infinity reads back as NaN.
+ *   row with an infinity reads back as NaN.  A row whose scale is NaN is NaN for
+ *   attention and read-back; scales are not negative (decode takes a V scale
+ *   below 2^-60, which f16 outputs cannot show, for that).
  * page_size, page_table and bad table entries as for the f16 paged caches
  * (below 0 or >= num_pages: device error 0x201, writes skip the row,
  * attention leaves the tile out, read-back gives zeros). */
