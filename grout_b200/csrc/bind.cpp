@@ -332,6 +332,16 @@ struct Workspace {
   }
 };
 
+// A split count, None or 0 the automatic one; refused here, before a workspace
+// of that size is asked for.
+int32_t splits_of(PyObject* o, int32_t most) {
+  const int32_t n = o == Py_None ? 0 : as_i32(o, "num_splits");
+  if (n < 0 || n > most) refuse("num_splits=%d must be in [0, %d]", n, most);
+  return n;
+}
+constexpr int32_t kMaxDecodeSplits = 1024, kMaxPrefillSplits = 32;  // as the entry points'
+constexpr int32_t kMaxSplitBatch = 65535;                           // of a split prefill
+
 const at::Tensor& decode_query(PyObject* o, int* dev) {
   const at::Tensor& q = tensor(o, "q", at::kHalf, dev);
   if (q.dim() != 3 || q.size(2) != kD) refuse("q must be [B, Hq, 128]: %s", shape_of(q).c_str());
@@ -348,7 +358,7 @@ void decode_tail(PyObject* const* a, const at::Tensor& q, int64_t hkv, int64_t m
   const int32_t B = i32_of(q.size(0), "batch");
   const uint32_t* pos = positions(a[0], B, dev);
   const int32_t max_kv_len = as_i32(a[2], "max_kv_len"), window = span(a[3]), sinks = span(a[4]);
-  const int32_t splits = a[6] == Py_None ? 0 : as_i32(a[6], "num_splits");
+  const int32_t splits = splits_of(a[6], kMaxDecodeSplits);
   const int scale_f16 = PyObject_IsTrue(a[8]);
   if (scale_f16 < 0) throw PythonError{};
   const grout_attn_dims d =
@@ -438,7 +448,9 @@ template <class Args, class F>
 void chunk_call(PyObject* const* a, const at::Tensor& q, const Args& g, int64_t max_keys, int32_t window,
                 int32_t sinks, const grout_attn_dims& d, int dev, F f) {
   Workspace ws(a[0], dev);
-  int32_t splits = a[1] == Py_None ? 0 : as_i32(a[1], "num_splits");
+  int32_t splits = splits_of(a[1], kMaxPrefillSplits);
+  if (splits > 1 && g.batch > kMaxSplitBatch)
+    refuse("num_splits=%d with batch=%d (at most %d with splits)", splits, g.batch, kMaxSplitBatch);
   enqueue(dev, [&](grout_stream_t s) {
     if (!ws.given) {
       if (splits == 0) {

@@ -39,3 +39,56 @@ def test_a_nan_value_scale_reaches_the_rows_that_see_it(grout, splits, row):
         k, v = (values(c, s).transpose(1, 2).reshape(n, hkv, D)[:300] for c, s in ((kc, ks), (vc, vs)))
         v[row, 1] = 0.0
         check(out, *attention64(q, k, v, pos.long(), 199, 100, SCALE_F16))
+
+
+def _calls(grout, B=2, hq=8, hkv=2):
+    """name -> (call with extra keywords, most splits)"""
+    f16 = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda")  # noqa: E731
+    q, out, kv = f16(B, hq, D), f16(B, hq, D), f16(B, hkv, 128, D)
+    codes = torch.zeros(B, hkv, 128, D, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scales = torch.zeros(B, hkv, 128, device="cuda")
+    table, pos = torch.arange(B, dtype=torch.int32, device="cuda").view(B, 1), torch.full((B,), 127, dtype=torch.int32, device="cuda")
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    return {
+        "decode": (lambda **x: grout.attention_decode_window(q, kv, kv, pos, out, 128, 100, 3, **x), 1024),
+        "paged": (lambda **x: grout.attention_decode_paged_window(q, kv, kv, table, pos, out, 128, 100, 3, **x), 1024),
+        "fp8": (lambda **x: grout.attention_decode_paged_fp8(q, codes, codes, scales, scales, table, pos, out, 128, **x), 1024),
+        "varlen": (lambda **x: grout.attention_prefill_varlen_window(q, kv, kv, out, cu, 1, hkv, D, 128 * D, 100, 3, kv_rows=128,
+                                                                     kv_batch_stride=hkv * 128 * D, position_start=pos, **x), 32),
+        "chunk": (lambda **x: grout.attention_prefill_paged_window(q, kv, kv, table, out, 100, 3, cu_seqlens_q=cu, position_start=pos, max_q_len=1, **x), 32),
+    }
+
+
+@pytest.mark.parametrize("name", ["decode", "paged", "fp8", "varlen", "chunk"])
+def test_split_counts_are_refused_before_a_workspace_is_made(grout, name):
+    call, most = _calls(grout)[name]
+    for n in (1, most, 0, None):
+        call(num_splits=n)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    for n in (-1, most + 1, 10 ** 5, 2 ** 31 - 1, -(2 ** 31)):
+        with pytest.raises(grout.GroutError, match="num_splits"):
+            call(num_splits=n)
+    assert torch.cuda.max_memory_allocated() == held
+    call()
+    torch.cuda.synchronize()
+    grout.check_device_error()
+
+
+def test_a_split_prefill_of_too_many_sequences_is_refused_before_a_workspace_is_made(grout):
+    B = 65536
+    q, out, kv = (torch.zeros(n, h, D, dtype=torch.float16, device="cuda") for n, h in ((B, 2), (B, 2), (1, 1)))
+    cu = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    with pytest.raises(grout.GroutError, match="batch"):
+        grout.attention_prefill_varlen_window(q, kv, kv, out, cu, 1, 1, D, D, 100, num_splits=4)
+    assert torch.cuda.max_memory_allocated() == held
+    grout.attention_prefill_varlen_window(q, kv, kv, out, cu, 1, 1, D, D, 100)
+    torch.cuda.synchronize()
+    grout.check_device_error()
