@@ -539,6 +539,15 @@ void prefill_paged(PyObject* const* a) {
   chunk_call(a + 12, q, g, max_seq, window, sinks, d, dev, g_api.prefill_paged);
 }
 
+// Sets torch.OutOfMemoryError, as every allocation of PyTorch's own does.
+void out_of_memory(const char* what) {
+  PyObject* torch = PyImport_ImportModule("torch");
+  PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+  if (type) PyErr_SetString(type, what);
+  Py_XDECREF(type);
+  Py_XDECREF(torch);
+}
+
 // Runs an entry point; C++ exceptions end here.
 template <void (*kFn)(PyObject* const*), int kArgs>
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -561,7 +570,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
       Py_DECREF(e);
     }
   } catch (const c10::OutOfMemoryError& e) {
-    PyErr_SetString(PyExc_MemoryError, e.what_without_backtrace());
+    out_of_memory(e.what_without_backtrace());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }

@@ -92,3 +92,23 @@ def test_a_split_prefill_of_too_many_sequences_is_refused_before_a_workspace_is_
     grout.attention_prefill_varlen_window(q, kv, kv, out, cu, 1, 1, D, D, 100)
     torch.cuda.synchronize()
     grout.check_device_error()
+
+
+@pytest.mark.parametrize("name", ["decode", "paged", "fp8", "varlen", "chunk"])
+def test_a_workspace_that_cannot_be_had_is_out_of_memory(grout, name):
+    """As PyTorch reports it, so that a caller can make the batch smaller and try
+    again: here PyTorch itself is told to hold no more than it does."""
+    calls = _calls(grout, B=4096, hq=64, hkv=8) if name in ("varlen", "chunk") else _calls(grout, B=64, hq=64, hkv=8)
+    call, most = calls[name]
+    call(num_splits=1)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + 2 ** 28) / torch.cuda.get_device_properties(0).total_memory)
+        with pytest.raises(torch.OutOfMemoryError):
+            call(num_splits=most)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    call(num_splits=most)
+    torch.cuda.synchronize()
+    grout.check_device_error()
