@@ -123,7 +123,7 @@ struct TileList {
     const int first = lo / kKeys;
     sink_tiles = min(first, (int)(((int64_t)nsinks + kKeys - 1) / kKeys));
     skip = first - sink_tiles;
-    n = sink_tiles + (len + kKeys - 1) / kKeys - first;
+    n = sink_tiles + (int)(((uint32_t)len + kKeys - 1) / kKeys) - first;  // (len up to 2^31 - 1)
   }
   __device__ __forceinline__ int key0(int i) const { return (i < sink_tiles ? i : i + skip) * kKeys; }
   __device__ __forceinline__ bool sees(int key) const {

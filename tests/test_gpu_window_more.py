@@ -112,3 +112,33 @@ def test_a_workspace_that_cannot_be_had_is_out_of_memory(grout, name):
     call(num_splits=most)
     torch.cuda.synchronize()
     grout.check_device_error()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("position", [2 ** 31 - 2, 2 ** 31 - 65, 2 ** 31 - 1025])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (70, 5), (2500, 200)])
+def test_decode_next_to_the_last_position(grout, fp8, position, window, sinks):
+    """Tables of 2^31 positions whose pages are freed but for the sinks' and the
+    window's: the counts of tiles and keys stay in 32 bits."""
+    hq, hkv, ps = 8, 2, 1024
+    table = torch.full((1, 2 ** 31 // ps), -1, dtype=torch.int32, device="cuda")
+    table[0, 0] = 3
+    table[0, -4:] = _i32(2, 5, 0, 4)
+    q = normal(40, 1, hq, D, scale=1.5).half()
+    out = torch.full_like(q, NAN)
+    pos = _i32(position)
+    if fp8:
+        (kc, ks), (vc, vs) = (fp8_cache(s, 6, hkv, ps, D) for s in (50, 60))
+        k, v = values(kc, ks), values(vc, vs)
+        call = lambda n: grout.attention_decode_paged_fp8(q, kc, vc, ks, vs, table, pos, out, 2 ** 31 - 1, window, sinks, max_seq=2 ** 31 - 1, num_splits=n)  # noqa: E731
+    else:
+        k, v = (normal(s, 6, hkv, ps, D).half() for s in (50, 60))
+        call = lambda n: grout.attention_decode_paged_window(q, k, v, table, pos, out, 2 ** 31 - 1, window, sinks, max_seq=2 ** 31 - 1, num_splits=n)  # noqa: E731
+    keys = torch.cat([torch.arange(sinks), torch.arange(position - window + 1, position + 1)]).cuda()
+    rows = [x[table[0, keys // ps].long(), :, keys % ps] for x in (k, v)]
+    for n in (None, 1, 3, 20):
+        out.fill_(NAN)
+        call(n)
+        torch.cuda.synchronize()
+        grout.check_device_error()
+        check(out, *attention64(q, *rows, torch.tensor([len(keys) - 1], device="cuda"), 0, 0, SCALE_F16))
