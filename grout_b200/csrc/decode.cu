@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (!pos_ok && split == 0 && kh == 0 && threadIdx.x == 0 && a.err)
     atomicCAS(a.err, 0, DEV_ERR_POSITION);
   const int kv_len = pos_ok ? (int)pos + 1 : 0;
-  const int n_tiles = (kv_len + kKeys - 1) / kKeys;
+  const int n_tiles = (int)(((uint32_t)kv_len + kKeys - 1) / kKeys);  // (kv_len up to 2^31 - 1)
   const int tps = (n_tiles + a.nks - 1) / a.nks;
   const int t0 = split * tps;
   const int t1 = min(t0 + tps, n_tiles);
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int kbase = (t0 + it) * kKeys + 16 * warp;
       if (kPaged && tile_mask[st]) {
         s0 = s1 = s2 = s3 = -INFINITY;
-      } else if (kbase + 16 > kv_len) {
+      } else if (kbase > kv_len - 16) {
         if (kbase + g >= kv_len) s0 = s1 = -INFINITY;
         if (kbase + g + 8 >= kv_len) s2 = s3 = -INFINITY;
       }

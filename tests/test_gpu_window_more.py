@@ -142,3 +142,21 @@ def test_decode_next_to_the_last_position(grout, fp8, position, window, sinks):
         torch.cuda.synchronize()
         grout.check_device_error()
         check(out, *attention64(q, *rows, torch.tensor([len(keys) - 1], device="cuda"), 0, 0, SCALE_F16))
+
+
+def test_plain_decode_next_to_the_last_position(grout):
+    """2^31 - 1 keys, every page but the last one the same: the last tile is
+    attended to and the one key behind the position is not.  Key 1000 of the
+    last page outscores all others by more than 100 (weights below e^-100), the
+    unseen key 1023 would outscore it."""
+    hq, hkv, ps = 8, 1, 1024
+    table = torch.zeros(1, 2 ** 31 // ps, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    k, v = (normal(s, 2, hkv, ps, D, scale=0.01).half() for s in (70, 71))
+    q = torch.full((1, hq, D), 4.0, dtype=torch.float16, device="cuda")
+    k[1, 0, 1000], k[1, 0, 1023] = 4.0, 8.0  # scores 4 * 4 * 128 * scale = 181 and 362; the others are within 10
+    out = torch.full_like(q, NAN)
+    grout.attention_decode_paged(q, k, v, table, _i32(2 ** 31 - 2), out, 2 ** 31 - 1, max_seq=2 ** 31 - 1)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    assert torch.equal(out, v[1, :, 1000].expand_as(out))
