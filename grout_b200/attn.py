@@ -20,6 +20,7 @@ range problems raise GroutError before any launch, like the reference's
 device is not sm_100 the call raises.
 """
 import ctypes
+import importlib.util
 import math
 import os
 
@@ -210,11 +211,16 @@ def _load_bind():
     """The compiled binding of the window and 8-bit cache calls (csrc/bind.cpp),
     which checks their arguments and calls into lib()."""
     global _bind
+    from . import build
+
     L = lib()
+    path = build.bind_path()
     try:
-        from . import _bind as b
+        spec = importlib.util.spec_from_file_location(__package__ + "._bind", path)
+        b = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(b)
     except ImportError as e:
-        raise GroutError(3, f"grout_b200/_bind.so: {e}: run `python -m grout_b200.build`")
+        raise GroutError(3, f"{path} (the binding for this PyTorch and Python): {e}: run `python -m grout_b200.build`")
     b.use(GroutError, tuple(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in _BIND_ENTRIES))
     _bind = b
     return b

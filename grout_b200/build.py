@@ -4,9 +4,11 @@
 
 One object per .cu file under csrc/, linked into grout_b200/libgrout_attn.so
 (static CUDA runtime, so the library carries no dependency beyond the
-driver).  The Python binding csrc/bind.cpp becomes
-grout_b200/_bind.so (g++, PyTorch's headers).  The build is skipped when both are
-newer than every source.
+driver).  The Python binding csrc/bind.cpp becomes bind_path() (g++, PyTorch's
+headers), a file for each PyTorch and Python that it is built for: its compiled
+code holds their object layouts.  The library does not need it, and is there
+without it where PyTorch is missing or the binding does not compile.  Each is
+built where it is missing or older than one of its sources.
 """
 import glob
 import os
@@ -19,7 +21,6 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libgrout_attn.so")
-BIND = os.path.join(HERE, "_bind.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 
 NVCC_FLAGS = [
@@ -41,16 +42,28 @@ def _sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.cu")))
 
 
-def _deps():
-    return _sources() + [os.path.join(CSRC, "bind.cpp")] + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(
-        os.path.join(CSRC, "*.h")) + [os.path.join(ROOT, "include", "grout_attn.h"), __file__]
+def bind_path() -> str:
+    """The binding's file for this PyTorch and Python."""
+    import torch  # only its version is needed
+
+    return os.path.join(HERE, f"_bind.torch-{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
+def _newer(path: str, deps) -> bool:
+    return os.path.exists(path) and all(os.path.getmtime(p) <= os.path.getmtime(path) for p in deps)
+
+
+def _lib_up_to_date() -> bool:
+    return _newer(LIB, _sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + [
+        os.path.join(ROOT, "include", "grout_attn.h"), __file__])
+
+
+def _bind_up_to_date() -> bool:
+    return _newer(bind_path(), [os.path.join(CSRC, "bind.cpp"), os.path.join(ROOT, "include", "grout_attn.h"), __file__])
 
 
 def up_to_date() -> bool:
-    if not (os.path.exists(LIB) and os.path.exists(BIND)):
-        return False
-    t = min(os.path.getmtime(LIB), os.path.getmtime(BIND))
-    return all(os.path.getmtime(p) <= t for p in _deps())
+    return _lib_up_to_date() and _bind_up_to_date()
 
 
 def _bind_command(out: str):
@@ -66,29 +79,44 @@ def _bind_command(out: str):
             "-ltorch_cpu", "-ltorch_python"]
 
 
-def build(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
-    if not force and up_to_date():
-        return LIB
+def _compile(commands) -> None:
+    """Runs the compilers side by side and waits for all of them."""
+    procs = [(subprocess.Popen(cmd), cmd) for cmd in commands]
+    failed = [cmd for p, cmd in procs if p.wait() != 0]
+    if failed:
+        raise RuntimeError("compilation failed: " + "; ".join(" ".join(cmd) for cmd in failed))
+
+
+def _build_lib(verbose: bool, extra_flags) -> None:
     os.makedirs(BUILD_DIR, exist_ok=True)
-    objs = []
-    procs = []
-    for src in _sources():
-        obj = os.path.join(BUILD_DIR, os.path.basename(src)[:-3] + ".o")
-        cmd = [nvcc(), *NVCC_FLAGS, *extra_flags, "-c", src, "-o", obj]
-        if verbose:
+    objs = [os.path.join(BUILD_DIR, os.path.basename(src)[:-3] + ".o") for src in _sources()]
+    commands = [[nvcc(), *NVCC_FLAGS, *extra_flags, "-c", src, "-o", obj] for src, obj in zip(_sources(), objs)]
+    if verbose:
+        for cmd in commands:
             print(" ".join(cmd))
-        procs.append((subprocess.Popen(cmd), cmd))
-        objs.append(obj)
-    cmd = _bind_command(BIND + ".tmp")
-    procs.append((subprocess.Popen(cmd), cmd))
-    for p, cmd in procs:
-        if p.wait() != 0:
-            raise RuntimeError("compilation failed: " + " ".join(cmd))
-    os.replace(BIND + ".tmp", BIND)
+    _compile(commands)
     tmp = LIB + ".tmp"
-    cmd = [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", tmp, *objs]
-    subprocess.check_call(cmd)
+    _compile([[nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", tmp, *objs]])
     os.replace(tmp, LIB)
+
+
+def _build_bind(verbose: bool) -> None:
+    tmp = bind_path() + ".tmp"
+    cmd = _bind_command(tmp)
+    if verbose:
+        print(" ".join(cmd))
+    _compile([cmd])
+    os.replace(tmp, bind_path())
+
+
+def build(force: bool = False, verbose: bool = False, extra_flags=()) -> str:
+    if force or not _lib_up_to_date():
+        _build_lib(verbose, extra_flags)
+    try:
+        if force or not _bind_up_to_date():
+            _build_bind(verbose)
+    except ImportError as e:  # no PyTorch: nobody to call the binding
+        print(f"grout_b200: the Python binding is not built: {e}", file=sys.stderr)
     return LIB
 
 
