@@ -1128,10 +1128,14 @@ static int choose_window_splits(int64_t units, int64_t tiles, int num_sms, bool 
   // Clusters of more than 8 that do not all get an SM per CTA leave SMs idle.
   if (n > 8 && n <= kDecodeMaxClusterSplits && units * n > num_sms)
     n = tiles / 4 > kDecodeMaxClusterSplits ? kDecodeMaxClusterSplits + 1 : 8;
-  // Long splits of a batch that fills the SMs: halve them, so that a ragged
-  // batch evens out.
-  if (n <= 4 && tiles / std::max<int64_t>(n, 1) >= 256 && units * n <= 2 * num_sms) n = 2 * std::max<int64_t>(n, 1);
-  return (int)std::max<int64_t>(n, 1);
+  n = std::max<int64_t>(n, 1);
+  // Long splits of a batch of a few units per SM: halve them, so that the last
+  // round and a ragged batch even out.  Sequences of 16384 keys, us, 1 against 2
+  // splits: 8-bit, 304 units of one length 272 / 229, ragged 152 / 149, 440 units
+  // 324 / 301 and 198 / 200, 512 units 333 / 344 and 220 / 231, 2048 units 1032 / 1075 and 838 / 870; f16, 304 units
+  // 410 / 370 and 251 / 251, 512 units 589 / 591 and 399 / 399.
+  if (n <= 4 && tiles / n >= 256 && units * n <= 3 * num_sms) n *= 2;
+  return (int)n;
 }
 
 int32_t grout_attn_decode_window_splits(int32_t batch, int32_t max_kv_len, int32_t window,

@@ -79,3 +79,17 @@ def test_a_failed_build_leaves_no_compiler_running(monkeypatch, scratch):
         build.build()
     assert len(started) == 2 and all(p.returncode not in (None, 0) for p in started)
     assert not os.path.exists(build.LIB)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_split_count_of_large_batches(fp8):
+    """Long contexts: two splits up to three units (sequence and KV head) per SM,
+    one for batches of more, however many."""
+    count = lambda units, keys: attn.decode_window_splits(units, keys, keys, 0, 4, 1, 1 << 20, fp8=fp8)  # noqa: E731
+    sms = 148  # of a B200, and what is assumed where there is no device
+    for units in (160, 300, 3 * sms):
+        assert count(units, 16384) == 2
+        assert count(units, 1 << 19) == 2
+        assert count(units, 16320) == 1  # 255 tiles
+    for units in (3 * sms + 1, 512, 2048, 65535):
+        assert count(units, 16384) == count(units, 1 << 19) == 1
