@@ -1132,8 +1132,9 @@ static int choose_window_splits(int64_t units, int64_t tiles, int num_sms, bool 
   // Long splits of a batch of a few units per SM: halve them, so that the last
   // round and a ragged batch even out.  Sequences of 16384 keys, us, 1 against 2
   // splits: 8-bit, 304 units of one length 272 / 229, ragged 152 / 149, 440 units
-  // 324 / 301 and 198 / 200, 512 units 333 / 344 and 220 / 231, 2048 units 1032 / 1075 and 838 / 870; f16, 304 units
-  // 410 / 370 and 251 / 251, 512 units 589 / 591 and 399 / 399.
+  // 324 / 301 and 198 / 200, 512 units 333 / 344 and 220 / 231, 2048 units 1032 /
+  // 1075 and 838 / 870; f16, 304 units 410 / 370 and 251 / 251, 512 units 589 /
+  // 591 and 399 / 399.
   if (n <= 4 && tiles / n >= 256 && units * n <= 3 * num_sms) n *= 2;
   return (int)n;
 }

@@ -4,7 +4,7 @@ of many key tiles in one CTA."""
 import pytest
 import torch
 
-from window_ref import D, SCALE_F16, attention64, check, fp8_cache, normal, values
+from window_ref import D, SCALE_F16, attention64, check, fp8_cache, free_pages, normal, page_pool, values
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -160,3 +160,76 @@ def test_plain_decode_next_to_the_last_position(grout):
     torch.cuda.synchronize()
     grout.check_device_error()
     assert torch.equal(out, v[1, :, 1000].expand_as(out))
+
+
+def _hidden(cache, first, last, window, sinks):
+    """A cache [1, Hkv, n, ...] whose rows that no query of positions first .. last sees are NaN (8-bit codes: 0x7F)."""
+    c = cache.clone()
+    low = max(0, first - window + 1)
+    fill = 0x7F if c.dtype is torch.uint8 else NAN
+    c[:, :, last + 1:] = fill
+    if low > sinks:
+        c[:, :, sinks:low] = fill
+    return c
+
+
+@pytest.mark.parametrize("page_size", [0, 64, 192])
+@pytest.mark.parametrize("position,window,sinks", [(5200, 4900, 130), (6100, 9000, 0), (6100, 4160, 64)])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_decode_of_many_tiles_per_cta(grout, page_size, position, window, sinks, splits):
+    """More than 64 tiles of 64 keys in a split (pages are looked up 32 tiles at
+    a time), sinks and window from shuffled pages with freed ones between."""
+    hq, hkv, n = 8, 1, 6200
+    q = normal(80, 1, hq, D, scale=1.5).half()
+    k, v = (_hidden(normal(s, 1, hkv, n, D).half(), position, position, window, sinks) for s in (81, 82))
+    out, pos = torch.full_like(q, NAN), _i32(position)
+    if page_size:
+        (kp, vp), table = page_pool([k, v], page_size, 9)
+        table = free_pages(table, page_size, [position - window + 1], sinks)
+        grout.attention_decode_paged_window(q, kp, vp, table, pos, out, n, window, sinks, num_splits=splits)
+    else:
+        grout.attention_decode_window(q, k, v, pos, out, n, window, sinks, num_splits=splits)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    check(out, *attention64(q, k[0].transpose(0, 1), v[0].transpose(0, 1), pos.long(), window, sinks, SCALE_F16))
+
+
+@pytest.mark.parametrize("page_size", [64, 192])
+@pytest.mark.parametrize("position,window,sinks", [(5200, 4900, 130), (6100, 0, 0), (6100, 4160, 64)])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_8_bit_decode_of_many_tiles_per_cta(grout, page_size, position, window, sinks, splits):
+    hq, hkv, n = 8, 1, 6200
+    q = normal(90, 1, hq, D, scale=1.5).half()
+    (kc, ks), (vc, vs) = (fp8_cache(s, 1, hkv, n, D) for s in (91, 93))
+    parts = [_hidden(x, position, position, window or n, sinks) for x in (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)]
+    pools, table = page_pool(parts, page_size, 9, fill=0x7F)
+    table = free_pages(table, page_size, [position - (window or n) + 1], sinks)
+    pools = [p.view(torch.float8_e4m3fn) for p in pools[:2]] + pools[2:]
+    out, pos = torch.full_like(q, NAN), _i32(position)
+    grout.attention_decode_paged_fp8(q, *pools, table, pos, out, n, window, sinks, num_splits=splits)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    check(out, *attention64(q, values(kc, ks)[0].transpose(0, 1), values(vc, vs)[0].transpose(0, 1), pos.long(), window, sinks, SCALE_F16))
+
+
+@pytest.mark.parametrize("page_size", [0, 64, 192])
+@pytest.mark.parametrize("tokens", [5, 45])
+@pytest.mark.parametrize("position,window,sinks", [(5000, 4500, 130), (5000, 9000, 0), (9000, 4160, 64)])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_prefill_of_many_tiles_per_item(grout, page_size, tokens, position, window, sinks, splits):
+    """More than 32 tiles of 128 keys for a block of rows (pages are looked up 16
+    tiles at a time), by both chains on one query tile and by two query tiles."""
+    hq, hkv, n = 8, 1, position + tokens
+    q = normal(100, tokens, hq, D, scale=1.5).half()
+    k, v = (_hidden(normal(s, 1, hkv, n, D).half(), position, n - 1, window, sinks) for s in (101, 102))
+    out, first = torch.full_like(q, NAN), _i32(position)
+    if page_size:
+        (kp, vp), table = page_pool([k, v], page_size, 9)
+        table = free_pages(table, page_size, [position - window + 1], sinks)
+        grout.attention_prefill_paged_window(q, kp, vp, table, out, window, sinks, position_start=first, num_splits=splits)
+    else:
+        grout.attention_prefill_varlen_window(q, k, v, out, None, tokens, hkv, D, n * D, window, sinks, kv_rows=n, position_start=first, num_splits=splits)
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    pos = position + torch.arange(tokens, device="cuda")
+    check(out, *attention64(q, k[0].transpose(0, 1), v[0].transpose(0, 1), pos, window, sinks))
