@@ -775,7 +775,10 @@ def kv_read_paged_fp8(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v
     device int32.  Rows behind the last sequence are left as they are.
     attention_prefill_varlen(_window) takes the result with kv_row_stride =
     Hkv * 128, kv_head_stride = 128, kv_start = cu_seqlens: attention of a
-    chunk of new tokens over the 8-bit cache."""
+    chunk of new tokens over the 8-bit cache.  With pages freed between the
+    sinks and the window: two sequences here (the same page-table row twice:
+    `sinks` rows from 0, the others from the window's first key on), one there,
+    whose position_start counts the joined rows."""
     (_bind or _load_bind()).kv_read(k_pages, v_pages, k_scales, v_scales, page_table, k_out, v_out, cu_seqlens,
                                     position_start, max_seq)
     return k_out, v_out

@@ -474,7 +474,9 @@ grout_status grout_qk_norm_rope_kv_prefill_paged_fp8(
  * result is what grout_attn_prefill_varlen and
  * grout_attn_prefill_varlen_window take with kv_row_stride = out_row_stride,
  * kv_head_stride = 128 and kv_start = cu_seqlens: attention of a chunk of new
- * tokens over the 8-bit cache. */
+ * tokens over the 8-bit cache.  Sinks and a window with freed pages between
+ * them: two sequences here with the same page-table row, neighbouring in
+ * cu_seqlens, one there, whose positions count the joined rows. */
 grout_status grout_kv_read_paged_fp8(const grout_fp8_pages* pages, const int32_t* page_table,
                                      int32_t table_stride, const int32_t* cu_seqlens,
                                      const int32_t* position_start, int32_t batch, int64_t rows,

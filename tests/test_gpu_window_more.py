@@ -233,3 +233,48 @@ def test_prefill_of_many_tiles_per_item(grout, page_size, tokens, position, wind
     grout.check_device_error()
     pos = position + torch.arange(tokens, device="cuda")
     check(out, *attention64(q, k[0].transpose(0, 1), v[0].transpose(0, 1), pos, window, sinks))
+
+
+def test_chunk_over_the_8_bit_cache_with_sinks_and_freed_pages(grout):
+    """The sinks and the window of each sequence read back as two neighbouring
+    runs (two rows of the page table each); positions count the joined rows.
+    Sequences before and past their windows, freed pages between the runs."""
+    hq, hkv, ps, window, sinks, n = 8, 2, 64, 300, 70, 2000
+    firsts, lens = [1500, 0, 369, 1900, 200], [40, 33, 1, 100, 260]
+    B = len(lens)
+    (kc, ks), (vc, vs) = (fp8_cache(s, B, hkv, n, D) for s in (110, 112))
+    parts = [x.clone() for x in (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)]
+    for x in parts:  # what nobody sees
+        for b in range(B):
+            x[b, :, firsts[b] + lens[b]:] = 0x7F if x.dtype is torch.uint8 else NAN
+            if firsts[b] - window + 1 > sinks:
+                x[b, :, sinks:firsts[b] - window + 1] = 0x7F if x.dtype is torch.uint8 else NAN
+    pools, table = page_pool(parts, ps, 11, fill=0x7F)
+    pools = [p.view(torch.float8_e4m3fn) for p in pools[:2]] + pools[2:]
+    table = free_pages(table, ps, [p - window + 1 for p in firsts], sinks)
+    assert (table == -1).any()
+    runs, starts, at = [], [], []
+    for p, m in zip(firsts, lens):
+        low = p - window + 1
+        if low <= sinks:
+            low, held = 0, 0
+        else:
+            held = sinks
+        runs += [held, p + m - low]
+        starts += [0, low]
+        at.append(held + p - low)
+    ends = torch.tensor([0] + runs).cumsum(0)
+    ko, vo = (torch.empty(int(ends[-1]), hkv, D, dtype=torch.float16, device="cuda") for _ in "kv")
+    grout.kv_read_paged_fp8(*pools, table.repeat_interleave(2, 0), ko, vo, ends.int().cuda(), position_start=_i32(*starts))
+    cu = torch.tensor([0] + lens).cumsum(0).tolist()
+    q = normal(120, cu[-1], hq, D, scale=1.5).half()
+    out = torch.full_like(q, NAN)
+    grout.attention_prefill_varlen_window(q, ko, vo, out, _i32(*cu), max(lens), hkv, hkv * D, D, window, sinks, position_start=_i32(*at),
+                                          kv_start=ends[:-1:2].int().cuda())
+    torch.cuda.synchronize()
+    grout.check_device_error()
+    for b in range(B):
+        rows = slice(cu[b], cu[b + 1])
+        k, v = ((c[b].float() * s[b, ..., None]).half().transpose(0, 1) for c, s in ((kc, ks), (vc, vs)))  # the read-back's roundings
+        pos = firsts[b] + torch.arange(lens[b], device="cuda")
+        check(out[rows], *attention64(q[rows], k, v, pos, window, sinks))
