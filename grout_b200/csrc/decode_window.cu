@@ -35,12 +35,14 @@
 // product, so that whatever they hold (an unwritten page, a NaN) stays out.
 //
 // Measured on B200: f16, 64 sequences, window 4096 behind 64 sinks, 64/8 heads
-// (1.09 GB): 154 us, 7.1 TB/s; 8-bit, 64 ragged sequences of up to 8192 keys,
-// 32/8 heads (0.75 GB): 112 us, 6.7 TB/s.  A 64-key tile of 8-bit keys takes a
-// group about 0.8 us; two CTAs per SM, two groups each, just keep up with the
-// memory.  One sequence is latency: 5.6 us for a window of 1024 (launch, position,
-// first tile, two merges), 19.5 us for 32768 8-bit keys (69 MB; 9 us of it
-// would be there for 1024 keys, the merge launch among them).
+// (1.09 GB): 155 us, 7.1 TB/s; 8-bit, 64 ragged sequences of up to 8192 keys,
+// 32/8 heads (0.75 GB): 112 us, 6.6 TB/s (both in a graph; 160 and 126 us a call
+// in a stream).  A 64-key tile of 8-bit keys takes a group about 0.8 us; two CTAs
+// per SM, two groups each, just keep up with the memory.  One sequence is
+// latency: 5.9 us for a window of 1024 (launch, position, first tile, two
+// merges); 8 heads of 32768 8-bit keys (69 MB) 20 us in 32 splits, of which 9.3
+// are there for 1024 keys in as many splits, 2.5 of them the merge launch (6.8 us
+// in 8 splits, which a cluster merges).
 //
 // Range checks on the device as in decode.cu: a position >= max_seq records
 // 0x200 and the row is zero; a page-table entry outside the pool that holds a
@@ -377,6 +379,9 @@ __global__ void __launch_bounds__(threads(kFp8), 2)
       const float p2 = ex2(s2 - m0), p3 = ex2(s3 - m1);
       l0 += kFp8 ? p0 * iv0 + p2 * iv1 : p0 + p2;
       l1 += kFp8 ? p1 * iv0 + p3 * iv1 : p1 + p3;
+      // The weights are rounded to f16 here (2^-11 relative, 2^-25 of the largest
+      // at least): the product takes both operands in V's type, and f32 ones
+      // would want twice the matrix instructions.  l keeps the f32 values.
       const uint32_t pb0 = movm_t(pack_half2(p0, p1));
       const uint32_t pb1 = movm_t(pack_half2(p2, p3));
 #pragma unroll

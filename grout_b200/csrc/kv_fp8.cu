@@ -85,9 +85,12 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kv_fp8_kernel(const NormRope
 // or K and V of a KV head, over every per-th token: the norm weights stay in
 // registers, the angles are read once for two rows, and the next token's rows
 // are loaded while this one's are worked on.  4096 tokens of 64/8 heads (161
-// MB): 33.3 us, 4.9 TB/s; a row per octet and scalar arithmetic took 35.1 us,
-// the schedulers issuing in 72 % of the cycles and L1 busy with angles for 61 %.
-// 5 blocks of 128 threads (96 registers): 4 % slower with 4, 10 % with 6 (spills).
+// MB): 32.2 us in a graph, 5.0 TB/s (34.8 us a call in a stream); a row per octet
+// and scalar arithmetic took 35.1 us, the schedulers issuing in 72 % of the cycles
+// and L1 busy with angles for 61 %.  Now they issue in 50 % and L1 is busy for 49 %:
+// what is left is latency, four warps a scheduler that wait for loads a third of
+// their time, and more of them want the registers: 5 blocks of 128 threads (96
+// registers) are 4 % faster than 4, 10 % than 6 (spills).
 constexpr int kChunkThreads = 128;
 constexpr int kChunkBlocks = 5;  // per SM
 __global__ void __launch_bounds__(kChunkThreads, kChunkBlocks)

@@ -23,8 +23,8 @@
 // Splits.  Calls with few items and long windows cut each item's keys into
 // nsplit runs of tiles, an item of its own each (kSplit): the output warps store
 // normalised f32 rows and their log2-sum-exp, a second kernel merges them.  One
-// sequence, 5 tokens, 64/8 heads: window 4096 38 -> 18 us (8 splits), 32005 keys
-// 276 -> 40 us (16).
+// sequence, 5 tokens, 64/8 heads: window 4096 39 -> 18 us (8 splits), 32005 keys
+// 272 -> 39 us (16).
 //
 // Keys.  An item streams the 64-key blocks that hold a key one of its rows
 // sees (the sinks' blocks, then from the first row's window on), two blocks
@@ -41,12 +41,14 @@
 // Bound by the tensor cores and the chain S -> P -> PV -> next S of each of two
 // query tiles: in long windows a 128-key tile of both takes 3600 cycles, 2048
 // of them MMA; a chain's turn is 1300 waiting for S (PV and QK are 1024), 480
-// for the maximum, 1290 for the exponentials, 110 for the hand-over.  Measured
-// on B200: 8192 tokens, window 1024, 4 sinks, 32/8 heads: 147 us, 0.88 PFLOP/s
-// of visible keys (0.98 with the blocks' unseen keys); six chunks of up to 700
-// tokens, window 4096, 64/8 heads: 480 us, 0.93 PFLOP/s.  At that rate the GPU
-// is at its power limit (about 1.6 GHz), so that fewer cycles in the softmax
-// (masks in a pass of their own, P handed over in halves) did not shorten it.
+// for the maximum, 1290 for the exponentials, 110 for the hand-over and, spread
+// over an item's tiles, about 440 for the change of items.  Measured on B200:
+// 8192 tokens, window 1024, 4 sinks, 32/8 heads: 148 us, 0.87 PFLOP/s of visible
+// keys (0.97 with the blocks' unseen keys); six chunks of up to 700 tokens,
+// window 4096, 64/8 heads: 432 us, 1.04 PFLOP/s.  Both are bursts of 100 calls in
+// a graph; sustained the GPU is at its power limit (about 1.6 GHz) and they take
+// 171 and 493 us, so that fewer cycles in the softmax (masks in a pass of their
+// own, P handed over in halves) did not shorten it.
 // 64-key blocks with two S buffers per tile took 221 us: the MMA warp could not
 // issue and wait for them as fast.
 #include <algorithm>
@@ -834,6 +836,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 p1 = ex2(x1);
               }
               rsum = fadd2(rsum, f2pack(p0, p1));
+              // f16 (2^-11 relative): both operands of the PV MMA have V's type, and
+              // S leaves no TMEM columns for wider ones.  The row sum keeps f32.
               pk[i] = pack_half2(p0, p1);
             }
             asm volatile(

@@ -491,7 +491,13 @@ grout_status grout_kv_read_paged_fp8(const grout_fp8_pages* pages, const int32_t
  * sinks >= 0; a window of p + 1 or more sees every key.  Keys that no query of
  * a call sees are not read past the 64-key blocks that hold a visible one:
  * pages that lie wholly outside may be freed (any table entry, -1 for one)
- * and their rows may hold anything. */
+ * and their rows may hold anything.
+ * Numbers, as in the plain calls: scores, maxima and sums in f32; the weights
+ * are rounded to f16 for the PV product (2^-11 relative, the sum takes the
+ * unrounded ones; in the prefill calls a quarter of them come from a polynomial
+ * good to 7.6e-5); the result is rounded to f16 (another 2^-11).  A visible NaN or
+ * +infinity in a score makes the row NaN; a row whose visible scores are all
+ * -infinity is zero. */
 
 /* Split count of the window decode entry points for num_splits = 0 (fp8: of
  * grout_attn_decode_paged_fp8; window 0 = the whole context), and the
@@ -534,9 +540,10 @@ size_t grout_attn_prefill_window_workspace_bytes(int64_t q_rows, int32_t num_spl
  * arguments as there; a group of up to 128 query heads per KV head.  Keys
  * stay below kv_rows (varlen: kv_start + position) or dims->max_seq (paged),
  * query rows below q_rows: a sequence that does not is left out, with device
- * error 0x200.  Query rows are worked on in blocks of 2 * floor(128 / group)
- * neighbours: a V row that one of them sees must be finite for the others (a
- * weight of 0 times an infinity is a NaN); all other rows may hold anything.
+ * error 0x200 (as is one past position 2^31 - 4098).  Query rows are worked on
+ * in blocks of 2 * floor(128 / group) neighbours: a V row that one of them sees
+ * must be finite for the others (a weight of 0 times an infinity is a NaN); all
+ * other rows may hold anything.
  * A page outside the pool that holds a visible key reads as zeros (0x201).
  * max_q_len sizes the launch: sequences may be longer or shorter.  num_splits: 1 to
  * 32 runs that each query block's keys are cut into (for few rows over a long

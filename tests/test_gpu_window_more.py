@@ -278,3 +278,28 @@ def test_chunk_over_the_8_bit_cache_with_sinks_and_freed_pages(grout):
         k, v = ((c[b].float() * s[b, ..., None]).half().transpose(0, 1) for c, s in ((kc, ks), (vc, vs)))  # the read-back's roundings
         pos = firsts[b] + torch.arange(lens[b], device="cuda")
         check(out[rows], *attention64(q[rows], k, v, pos, window, sinks))
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+def test_infinite_scores(grout, splits):
+    """+infinity (or NaN) among the visible scores: NaN; -infinity: no weight; nothing but -infinity: zero."""
+    hq, hkv, n, p = 8, 2, 192, 150
+    q = normal(130, 1, hq, D).abs().half() + 1
+    k, v = (normal(s, 1, hkv, n, D).half() for s in (131, 132))
+    pos = _i32(p)
+    for bad, window, want in ((float("-inf"), 1, "zero"), (float("inf"), 1, "nan"), (float("-inf"), 2, "other"), (float("inf"), 100, "nan"), (NAN, 100, "nan")):
+        kb = k.clone()
+        kb[0, 0, p, 3] = bad
+        a, b = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+        grout.attention_decode_window(q, kb, v, pos, a, n, window, 0, num_splits=splits)
+        grout.attention_prefill_varlen_window(q, kb, v, b, None, 1, hkv, D, n * D, window, 0, kv_rows=n, position_start=pos, num_splits=splits)
+        torch.cuda.synchronize()
+        grout.check_device_error()
+        for o in (a, b):
+            if want == "nan":
+                assert torch.isnan(o[0, :4]).all()
+            elif want == "zero":
+                assert (o[0, :4] == 0).all()
+            else:
+                assert torch.equal(o[0, :4], v[0, :1, p - 1].expand(4, D))
+            assert torch.isfinite(o[0, 4:]).all() and (o[0, 4:] != 7.0).any()
